@@ -45,6 +45,9 @@ enum kvb_status {
 
 enum kvb_dtype { KVB_BF16 = 0, KVB_F16 = 1 };
 
+/* Element type of an 8-bit KV cache (see kvb_rope_kv_append_q8). */
+enum kvb_kv_format { KVB_KV_INT8 = 0, KVB_KV_E4M3 = 1 };
+
 /* Message describing the last non-OK status returned on this host thread. */
 const char* kvb_last_error(void);
 const char* kvb_version(void);
@@ -358,6 +361,116 @@ int kvb_rope_attention_decode_paged(kvb_stream_t stream, const void* qkv, size_t
                                     size_t max_len, size_t n_q, size_t n_kv, size_t head_dim,
                                     float scale, void* out, size_t out_row_stride, void* workspace,
                                     size_t workspace_len, int dtype);
+
+/* ---------------------------------------------------------------------------
+ * 8-bit KV cache.  New: the reference's cache is 16-bit (engine/src/gpu/kernels.rs:
+ * 238-371).  A cache row -- one position of one KV head -- is head_dim codes (int8
+ * or e4m3, kv_format) and one f32 scale: with amax = max |x| over the row and top =
+ * 127 (int8) or 448 (e4m3),
+ *     scale = amax / top,  code = round-to-nearest-even(x * (top / amax)),
+ * in f32, and the row stands for code * scale.  A row with amax < 2^-119 is stored
+ * as zeros; a row that holds a NaN or an infinity gets a NaN scale and zero codes,
+ * so that all of it reads back as NaN.  (head_dim + 4) bytes a row, against
+ * 2 head_dim in 16 bits.
+ *
+ * Contiguous caches: sequence b's codes at kc/vc + b * seq_stride (elements; a
+ * multiple of head_dim, at least n_kv * max_seq * head_dim), laid out [n_kv,
+ * max_seq, head_dim], its scales at ks/vs + b * seq_stride / head_dim, laid out
+ * [n_kv, max_seq]; cache_len code elements and scale_len = cache_len / head_dim
+ * scales each.  Paged: pools [n_blocks][n_kv][block_size][head_dim] of codes
+ * (pool_len elements) and [n_blocks][n_kv][block_size] of scales, addressed through
+ * block_table as for kvb_attention_decode_paged.
+ *
+ * RoPE and quantising append: qkv rows b*t .. b*t+t-1 belong to sequence b at
+ * positions pos[b] .. pos[b]+t-1 (pos: device int32 [n_seq]).  q and k heads are
+ * rotated in place as by kvb_rope_kv_append (the same bits; cos_t and sin_t NULL:
+ * no rotation), then the 16-bit k and v rows are quantised into the cache.  A
+ * position outside the cache or the table, or a block entry outside the pool, sets
+ * kvb_device_error code 4 and leaves that row alone.  The rows of one call go to
+ * cache rows of their own.  Any even head_dim up to 256. */
+int kvb_rope_kv_append_q8(kvb_stream_t stream, void* qkv, size_t qkv_len, size_t n_seq, size_t t,
+                          const int32_t* pos, const float* cos_t, const float* sin_t,
+                          size_t table_len, void* kc, void* vc, float* ks, float* vs,
+                          size_t seq_stride, size_t cache_len, size_t scale_len, size_t n_q,
+                          size_t n_kv, size_t head_dim, size_t max_seq, int kv_format, int dtype);
+int kvb_rope_kv_append_q8_paged(kvb_stream_t stream, void* qkv, size_t qkv_len, size_t n_seq,
+                                size_t t, const int32_t* pos, const float* cos_t,
+                                const float* sin_t, size_t table_len, void* k_pool, void* v_pool,
+                                float* k_scales, float* v_scales, size_t pool_len, size_t scale_len,
+                                const int32_t* block_table, size_t max_blocks, size_t block_size,
+                                size_t n_q, size_t n_kv, size_t head_dim, int kv_format, int dtype);
+
+/* Reads cache rows back as 16-bit values: positions pos[b] .. pos[b]+t-1 of sequence
+ * b go to k_out / v_out [n_seq, n_kv, out_rows, head_dim], rows 0 .. t-1 (t <=
+ * out_rows; the rest is not written), as code * scale in f32 rounded once.  With pos
+ * = 0 and out_rows = max_seq the outputs are the 16-bit caches that
+ * kvb_attention_prefill reads.  A position outside the cache or a block entry outside
+ * the pool sets kvb_device_error code 4 and reads as zeros. */
+int kvb_kv_read_q8(kvb_stream_t stream, const void* kc, const void* vc, const float* ks,
+                   const float* vs, size_t seq_stride, size_t cache_len, size_t scale_len,
+                   const int32_t* pos, size_t n_seq, size_t t, size_t n_kv, size_t head_dim,
+                   size_t max_seq, void* k_out, void* v_out, size_t out_len, size_t out_rows,
+                   int kv_format, int dtype);
+int kvb_kv_read_q8_paged(kvb_stream_t stream, const void* k_pool, const void* v_pool,
+                         const float* k_scales, const float* v_scales, size_t pool_len,
+                         size_t scale_len, const int32_t* block_table, size_t max_blocks,
+                         size_t block_size, const int32_t* pos, size_t n_seq, size_t t, size_t n_kv,
+                         size_t head_dim, void* k_out, void* v_out, size_t out_len, size_t out_rows,
+                         int kv_format, int dtype);
+
+/* Batched single-query decode attention over an 8-bit cache: kvb_attention_decode's
+ * arguments and result (f32 scores, sums and accumulation) on the values that the
+ * rows stand for.  Any head_dim up to 256, any group size; a block entry outside the
+ * pool sets kvb_device_error code 4 and those keys read as zeros. */
+int kvb_attention_decode_q8(kvb_stream_t stream, const void* q, size_t q_row_stride, const void* kc,
+                            const void* vc, const float* ks, const float* vs, size_t seq_stride,
+                            size_t cache_len, size_t scale_len, const int32_t* lens, size_t n_seq,
+                            size_t max_len, size_t n_q, size_t n_kv, size_t head_dim,
+                            size_t max_seq, float scale, void* out, size_t out_row_stride,
+                            void* workspace, size_t workspace_len, int kv_format, int dtype);
+int kvb_attention_decode_q8_paged(kvb_stream_t stream, const void* q, size_t q_row_stride,
+                                  const void* k_pool, const void* v_pool, const float* k_scales,
+                                  const float* v_scales, size_t pool_len, size_t scale_len,
+                                  const int32_t* block_table, size_t max_blocks, size_t block_size,
+                                  const int32_t* lens, size_t n_seq, size_t max_len, size_t n_q,
+                                  size_t n_kv, size_t head_dim, float scale, void* out,
+                                  size_t out_row_stride, void* workspace, size_t workspace_len,
+                                  int kv_format, int dtype);
+size_t kvb_attention_decode_q8_workspace_bytes(size_t n_seq, size_t max_len, size_t n_q,
+                                               size_t n_kv, size_t head_dim);
+
+/* Batched single-query decode attention of sequences that share a prefix (16-bit
+ * caches).  New: the reference decodes one sequence (engine/src/gpu/kernels.rs:
+ * 294-371).  Contiguous: every sequence attends to the prefix's keys [0, prefix_len)
+ * of pk / pv [n_kv, prefix_rows, head_dim], then to its own keys [0, lens[b]) of its
+ * cache (kc/vc + b*seq_stride, [n_kv, max_seq, head_dim]; lens does not count the
+ * prefix, 0 <= lens[b] <= max_len <= max_seq).  Positions are the caller's: own keys
+ * are rotated at prefix_len + i.  A sequence with neither gives a zero row.  Paged:
+ * the caches of kvb_attention_decode_paged; the first shared_len keys of every
+ * sequence are the same, and are read through row 0 of the block table (whole blocks
+ * of a prefix appear in every row, a block that the prefix ends in may be copied for
+ * each sequence); lens[b] counts them, and a length below shared_len attends to
+ * that many of them.  Both equal kvb_attention_decode(_paged) over the same keys up
+ * to the order of the f32 sums.  Any head_dim up to 256, any group size. */
+int kvb_attention_decode_shared(kvb_stream_t stream, const void* q, size_t q_row_stride,
+                                const void* pk, const void* pv, size_t prefix_len,
+                                size_t prefix_rows, const void* kc, const void* vc,
+                                size_t seq_stride, size_t cache_len, const int32_t* lens,
+                                size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
+                                size_t head_dim, size_t max_seq, float scale, void* out,
+                                size_t out_row_stride, void* workspace, size_t workspace_len,
+                                int dtype);
+int kvb_attention_decode_shared_paged(kvb_stream_t stream, const void* q, size_t q_row_stride,
+                                      const void* k_pool, const void* v_pool, size_t pool_len,
+                                      const int32_t* block_table, size_t max_blocks,
+                                      size_t block_size, size_t shared_len, const int32_t* lens,
+                                      size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
+                                      size_t head_dim, float scale, void* out,
+                                      size_t out_row_stride, void* workspace, size_t workspace_len,
+                                      int dtype);
+/* max_own: the largest number of own keys (paged: max_len - shared_len). */
+size_t kvb_attention_decode_shared_workspace_bytes(size_t n_seq, size_t shared_len, size_t max_own,
+                                                   size_t n_q, size_t n_kv, size_t head_dim);
 
 /* Greedy sampling: ids[r] = first index of the maximum of logits[r, 0:vocab)
  * (NaN never wins; a row with no value above -inf gives 0).  If advance is

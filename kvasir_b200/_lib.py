@@ -17,6 +17,7 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "kvasir_b200.h")
 (KVB_OK, KVB_ERR_SHAPE, KVB_ERR_CUDA, KVB_ERR_UNSUPPORTED, KVB_ERR_DEVICE, KVB_ERR_CONFIG,
  KVB_ERR_IO) = range(7)
 KVB_BF16, KVB_F16 = 0, 1
+KVB_KV_INT8, KVB_KV_E4M3 = 0, 1
 KVB_CKPT_BF16, KVB_CKPT_F16, KVB_CKPT_F32, KVB_CKPT_OTHER = range(4)
 KVB_NOALLOC_SCRATCH_BYTES = 8 << 20  # include/kvasir_b200.h
 
@@ -113,6 +114,28 @@ SIGNATURES = {
     "kvb_decoder_set_lm_head": (_int, [_p, _p]),
     "kvb_decoder_set_sampling": (_int, [_p, C.c_float, C.c_float, C.c_uint64]),
     "kvb_sample_f32": (_int, [_p, _p, _sz, _sz, C.c_float, C.c_float, C.c_uint64, _p, _p, _p, _p]),
+    "kvb_rope_kv_append_q8": (_int, [_p, _p, _sz, _sz, _sz, _p, _p, _p, _sz, _p, _p, _p, _p, _sz,
+                                     _sz, _sz, _sz, _sz, _sz, _sz, _int, _int]),
+    "kvb_rope_kv_append_q8_paged": (_int, [_p, _p, _sz, _sz, _sz, _p, _p, _p, _sz, _p, _p, _p, _p,
+                                           _sz, _sz, _p, _sz, _sz, _sz, _sz, _sz, _int, _int]),
+    "kvb_kv_read_q8": (_int, [_p, _p, _p, _p, _p, _sz, _sz, _sz, _p, _sz, _sz, _sz, _sz, _sz, _p,
+                              _p, _sz, _sz, _int, _int]),
+    "kvb_kv_read_q8_paged": (_int, [_p, _p, _p, _p, _p, _sz, _sz, _p, _sz, _sz, _p, _sz, _sz, _sz,
+                                    _sz, _p, _p, _sz, _sz, _int, _int]),
+    "kvb_attention_decode_q8": (_int, [_p, _p, _sz, _p, _p, _p, _p, _sz, _sz, _sz, _p, _sz, _sz,
+                                       _sz, _sz, _sz, _sz, C.c_float, _p, _sz, _p, _sz, _int,
+                                       _int]),
+    "kvb_attention_decode_q8_paged": (_int, [_p, _p, _sz, _p, _p, _p, _p, _sz, _sz, _p, _sz, _sz,
+                                             _p, _sz, _sz, _sz, _sz, _sz, C.c_float, _p, _sz, _p,
+                                             _sz, _int, _int]),
+    "kvb_attention_decode_q8_workspace_bytes": (_sz, [_sz, _sz, _sz, _sz, _sz]),
+    "kvb_attention_decode_shared": (_int, [_p, _p, _sz, _p, _p, _sz, _sz, _p, _p, _sz, _sz, _p, _sz,
+                                           _sz, _sz, _sz, _sz, _sz, C.c_float, _p, _sz, _p, _sz,
+                                           _int]),
+    "kvb_attention_decode_shared_paged": (_int, [_p, _p, _sz, _p, _p, _sz, _p, _sz, _sz, _sz, _p,
+                                                 _sz, _sz, _sz, _sz, _sz, C.c_float, _p, _sz, _p,
+                                                 _sz, _int]),
+    "kvb_attention_decode_shared_workspace_bytes": (_sz, [_sz, _sz, _sz, _sz, _sz, _sz]),
     "kvb_checkpoint_open": (_int, [C.POINTER(_p), C.c_char_p]),
     "kvb_checkpoint_close": (_int, [_p]),
     "kvb_checkpoint_num_tensors": (_sz, [_p]),

@@ -13,9 +13,11 @@
 #include <vector>
 
 #include "attn_decode.cuh"
+#include "attn_general_src.cuh"
 #include "attn_generic.cuh"
 #include "attn_prefill.cuh"
 #include "elementwise.cuh"
+#include "kv8.cuh"
 #include "kvb_host.h"
 #include "linear_rows.cuh"
 #include "lm_head.cuh"
@@ -1976,3 +1978,5 @@ int decode_combine_launches(size_t n_seq, size_t max_len, size_t n_q, size_t n_k
 }
 
 }  // namespace kvb
+
+#include "kvb_api_kv8.cuh"

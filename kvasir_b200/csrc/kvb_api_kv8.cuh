@@ -1,0 +1,430 @@
+// kvb_api_kv8.cuh -- launchers and C entry points of the 8-bit KV cache and of the
+// shared-prefix decode attention (part of kvb_api.cu's translation unit, which holds
+// the library's device code).
+#pragma once
+
+namespace kvb {
+
+static bool valid_kv_format(int f) { return f == KVB_KV_INT8 || f == KVB_KV_E4M3; }
+
+// Calls F<T, kFmt>(args...) for the run-time dtype and cache format.
+#define KVB_KV8_DISPATCH(F, dtype, fmt, ...)                                   \
+    ((dtype) == KVB_BF16                                                       \
+         ? ((fmt) == KVB_KV_INT8 ? F<__nv_bfloat16, KVB_KV_INT8>(__VA_ARGS__)  \
+                                 : F<__nv_bfloat16, KVB_KV_E4M3>(__VA_ARGS__)) \
+         : ((fmt) == KVB_KV_INT8 ? F<__half, KVB_KV_INT8>(__VA_ARGS__)         \
+                                 : F<__half, KVB_KV_E4M3>(__VA_ARGS__)))
+
+// ---------------------------------------------------------------- argument checks
+// Contiguous cache: sequence b's rows at b * seq_stride / head_dim, [n_kv][max_seq].
+static int kv8_place_contiguous(const char* name, Kv8Place& c, const void* kc, const void* vc,
+                                const float* ks, const float* vs, size_t seq_stride,
+                                size_t cache_len, size_t scale_len, size_t n_seq, size_t n_kv,
+                                size_t head_dim, size_t max_seq) {
+    KVB_CHECK(head_dim > 0 && head_dim <= 256 && n_kv > 0,
+              "%s: head_dim %zu must be in 1..256 and n_kv > 0", name, head_dim);
+    KVB_CHECK(fits_i32(n_seq) && fits_i32(n_kv) && fits_i32(max_seq) && fits_i32(n_kv * max_seq),
+              "%s: a dimension does not fit in i32", name);
+    const size_t per_seq = n_kv * max_seq * head_dim;
+    KVB_CHECK(seq_stride >= per_seq && seq_stride % head_dim == 0,
+              "%s: seq_stride %zu must be a multiple of head_dim and at least %zu", name,
+              seq_stride, per_seq);
+    KVB_CHECK(n_seq == 0 ||
+                  (cache_len >= per_seq && (n_seq == 1 || (cache_len - per_seq) / (n_seq - 1) >= seq_stride)),
+              "%s: cache of %zu elems is too small", name, cache_len);
+    KVB_CHECK(cache_len % head_dim == 0 && scale_len == cache_len / head_dim,
+              "%s: %zu scales for a cache of %zu elems, want one per %zu", name, scale_len,
+              cache_len, head_dim);
+    KVB_CHECK(kc != nullptr && vc != nullptr && ks != nullptr && vs != nullptr,
+              "%s: null cache or scales", name);
+    memset(&c, 0, sizeof c);
+    c.kc = static_cast<uint8_t*>(const_cast<void*>(kc));
+    c.vc = static_cast<uint8_t*>(const_cast<void*>(vc));
+    c.ks = const_cast<float*>(ks);
+    c.vs = const_cast<float*>(vs);
+    c.seq_rows = (long long)(seq_stride / head_dim);
+    c.n_kv = (int)n_kv;
+    c.hd = (int)head_dim;
+    c.max_seq = (int)max_seq;
+    return KVB_OK;
+}
+
+static int kv8_place_paged(const char* name, Kv8Place& c, const void* k_pool, const void* v_pool,
+                           const float* k_scales, const float* v_scales, size_t pool_len,
+                           size_t scale_len, const int32_t* block_table, size_t max_blocks,
+                           size_t block_size, size_t n_seq, size_t n_kv, size_t head_dim) {
+    KVB_CHECK(head_dim > 0 && head_dim <= 256 && n_kv > 0,
+              "%s: head_dim %zu must be in 1..256 and n_kv > 0", name, head_dim);
+    KVB_CHECK(block_table != nullptr, "%s: null block table", name);
+    KVB_CHECK(block_size > 0 && fits_i32(block_size) && fits_i32(n_kv) &&
+                  fits_i32(n_kv * block_size) && fits_i32(max_blocks) &&
+                  fits_i32(max_blocks * block_size) && fits_i32(n_seq) &&
+                  fits_i32(n_seq * max_blocks),
+              "%s: a dimension does not fit in i32 (or block_size is 0)", name);
+    const size_t per_block = n_kv * block_size * head_dim;
+    KVB_CHECK(pool_len % per_block == 0 && fits_i32(pool_len / per_block),
+              "%s: pool of %zu elems is not a whole number of %zu-elem blocks", name, pool_len,
+              per_block);
+    KVB_CHECK(scale_len == pool_len / head_dim,
+              "%s: %zu scales for a pool of %zu elems, want one per %zu", name, scale_len, pool_len,
+              head_dim);
+    KVB_CHECK(k_pool != nullptr && v_pool != nullptr && k_scales != nullptr && v_scales != nullptr,
+              "%s: null pool or scales", name);
+    memset(&c, 0, sizeof c);
+    c.kc = static_cast<uint8_t*>(const_cast<void*>(k_pool));
+    c.vc = static_cast<uint8_t*>(const_cast<void*>(v_pool));
+    c.ks = const_cast<float*>(k_scales);
+    c.vs = const_cast<float*>(v_scales);
+    c.n_kv = (int)n_kv;
+    c.hd = (int)head_dim;
+    c.max_seq = (int)(max_blocks * block_size);
+    c.block_table = block_table;
+    c.max_blocks = (int)max_blocks;
+    c.block_size = (int)block_size;
+    c.n_blocks = (int)(pool_len / per_block);
+    return KVB_OK;
+}
+
+// ---------------------------------------------------------------- append
+template <typename T, int kFmt>
+static int launch_kv8_append(kvb_stream_t stream, const Kv8AppendArgs& a, size_t rows) {
+    const long long items = (long long)rows * (a.n_q + 2 * a.c.n_kv);
+    const long long grid = (items + 3) / 4;
+    KVB_CHECK(grid <= 0x7fffffffll, "rope_kv_append_q8: too many rows");
+    kv8_append_general_kernel<T, kFmt><<<(unsigned)grid, 128, 0, stream>>>(a, items);
+    KVB_CHECK_LAUNCH("rope_kv_append_q8 launch");
+    return KVB_OK;
+}
+
+static int kv8_append(const char* name, kvb_stream_t stream, void* qkv, size_t qkv_len,
+                      size_t n_seq, size_t t, const int32_t* pos, const float* cos_t,
+                      const float* sin_t, size_t table_len, const Kv8Place& c, size_t n_q,
+                      int kv_format, int dtype) {
+    const size_t hd = (size_t)c.hd, stride = (n_q + 2 * (size_t)c.n_kv) * hd;
+    KVB_CHECK(hd % 2 == 0, "%s: odd head_dim %zu", name, hd);
+    KVB_CHECK(fits_i32(n_q) && fits_i32(stride) && fits_i32(t) && fits_i32(n_seq * t),
+              "%s: a dimension does not fit in i32", name);
+    KVB_CHECK(qkv_len == n_seq * t * stride, "%s: qkv has %zu elems, want %zux%zux%zu", name,
+              qkv_len, n_seq, t, stride);
+    KVB_CHECK((cos_t == nullptr) == (sin_t == nullptr), "%s: one of cos / sin is null", name);
+    KVB_CHECK(!cos_t || (table_len % (hd / 2) == 0 && fits_i32(table_len / (hd / 2))),
+              "%s: bad cos/sin table sizes", name);
+    if (n_seq == 0 || t == 0) return KVB_OK;
+    KVB_CHECK(qkv != nullptr && pos != nullptr, "%s: null qkv or position array", name);
+    Kv8AppendArgs a;
+    a.qkv = static_cast<uint16_t*>(qkv);
+    a.n_q = (int)n_q;
+    a.row_stride = (int)stride;
+    a.rows_per_seq = (int)t;
+    a.pos = pos;
+    a.cos_t = cos_t;
+    a.sin_t = sin_t;
+    a.max_pos = cos_t ? (int)(table_len / (hd / 2)) : 0;
+    a.c = c;
+    return KVB_KV8_DISPATCH(launch_kv8_append, dtype, kv_format, stream, a, n_seq * t);
+}
+
+// ---------------------------------------------------------------- read back
+template <typename T, int kFmt>
+static int launch_kv8_read(kvb_stream_t stream, const Kv8ReadArgs& a, size_t n_seq) {
+    const long long items = (long long)n_seq * a.t * a.c.n_kv * 2;
+    const long long grid = (items + 3) / 4;
+    KVB_CHECK(grid <= 0x7fffffffll, "kv_read_q8: too many rows");
+    kv8_read_general_kernel<T, kFmt><<<(unsigned)grid, 128, 0, stream>>>(a, items);
+    KVB_CHECK_LAUNCH("kv_read_q8 launch");
+    return KVB_OK;
+}
+
+static int kv8_read(const char* name, kvb_stream_t stream, const Kv8Place& c, const int32_t* pos,
+                    size_t n_seq, size_t t, void* k_out, void* v_out, size_t out_len,
+                    size_t out_rows, int kv_format, int dtype) {
+    KVB_CHECK(fits_i32(t) && fits_i32(out_rows) && fits_i32(n_seq * t),
+              "%s: a dimension does not fit in i32", name);
+    KVB_CHECK(t <= out_rows, "%s: %zu rows into outputs of %zu", name, t, out_rows);
+    KVB_CHECK(out_len == n_seq * (size_t)c.n_kv * out_rows * (size_t)c.hd,
+              "%s: outputs of %zu elems, want %zux%dx%zux%d", name, out_len, n_seq, c.n_kv,
+              out_rows, c.hd);
+    if (n_seq == 0 || t == 0) return KVB_OK;
+    KVB_CHECK(pos != nullptr && k_out != nullptr && v_out != nullptr,
+              "%s: null positions or outputs", name);
+    Kv8ReadArgs a;
+    a.c = c;
+    a.pos = pos;
+    a.t = (int)t;
+    a.out_rows = (int)out_rows;
+    a.k_out = static_cast<uint16_t*>(k_out);
+    a.v_out = static_cast<uint16_t*>(v_out);
+    return KVB_KV8_DISPATCH(launch_kv8_read, dtype, kv_format, stream, a, n_seq);
+}
+
+// ---------------------------------------------------------------- decode attention
+static int decode_args(const char* name, GeneralDecodeArgs& a, const void* q, size_t q_row_stride,
+                       const int32_t* lens, size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
+                       size_t head_dim, float scale, void* out, size_t out_row_stride) {
+    KVB_CHECK(n_kv > 0 && n_q > 0 && n_q % n_kv == 0, "%s: n_q %zu not a multiple of n_kv %zu", name,
+              n_q, n_kv);
+    KVB_CHECK(head_dim > 0 && head_dim <= 256, "%s: head_dim %zu must be in 1..256", name, head_dim);
+    KVB_CHECK(fits_i32(n_seq) && fits_i32(max_len) && fits_i32(n_q * head_dim),
+              "%s: a dimension does not fit in i32", name);
+    KVB_CHECK(q_row_stride >= n_q * head_dim, "%s: q_row_stride too small", name);
+    KVB_CHECK(out_row_stride >= n_q * head_dim, "%s: out_row_stride too small", name);
+    KVB_CHECK(n_seq == 0 || (q != nullptr && lens != nullptr && out != nullptr),
+              "%s: null q, lengths or output", name);
+    a.q = static_cast<const uint16_t*>(q);
+    a.q_row_stride = (long long)q_row_stride;
+    a.lens = lens;
+    a.max_len = (int)max_len;
+    a.n_q = (int)n_q;
+    a.n_kv = (int)n_kv;
+    a.hd = (int)head_dim;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.out = static_cast<uint16_t*>(out);
+    a.out_row_stride = (long long)out_row_stride;
+    return KVB_OK;
+}
+
+template <typename T, int kFmt>
+static int launch_q8_decode(kvb_stream_t stream, const GeneralDecodeArgs& a, const Kv8Place& c,
+                            size_t n_seq, void* ws, size_t ws_len) {
+    Q8Source<T, kFmt> src;
+    src.c = c;
+    const dim3 grid((unsigned)n_seq, (unsigned)((a.n_q + 3) / 4));
+    attn_general_src_kernel<T, Q8Source<T, kFmt>><<<grid, 128, 0, stream>>>(a, src);
+    KVB_CHECK_LAUNCH("attention_decode_q8 launch");
+    return KVB_OK;
+}
+
+template <typename T>
+static int launch_shared(kvb_stream_t stream, const GeneralDecodeArgs& a, const SharedSource<T>& src,
+                         size_t n_seq, void* ws, size_t ws_len) {
+    const dim3 grid((unsigned)n_seq, (unsigned)((a.n_q + 3) / 4));
+    attn_general_src_kernel<T, SharedSource<T>><<<grid, 128, 0, stream>>>(a, src);
+    KVB_CHECK_LAUNCH("attention_decode_shared launch");
+    return KVB_OK;
+}
+
+}  // namespace kvb
+
+extern "C" {
+
+int kvb_rope_kv_append_q8(kvb_stream_t stream, void* qkv, size_t qkv_len, size_t n_seq, size_t t,
+                          const int32_t* pos, const float* cos_t, const float* sin_t,
+                          size_t table_len, void* kc, void* vc, float* ks, float* vs,
+                          size_t seq_stride, size_t cache_len, size_t scale_len, size_t n_q,
+                          size_t n_kv, size_t head_dim, size_t max_seq, int kv_format, int dtype) {
+    KVB_CHECK_DTYPE(dtype);
+    KVB_CHECK(valid_kv_format(kv_format), "unknown KV format %d", kv_format);
+    Kv8Place c;
+    const int st = kv8_place_contiguous("rope_kv_append_q8", c, kc, vc, ks, vs, seq_stride,
+                                        cache_len, scale_len, n_seq, n_kv, head_dim, max_seq);
+    if (st) return st;
+    return kv8_append("rope_kv_append_q8", stream, qkv, qkv_len, n_seq, t, pos, cos_t, sin_t,
+                      table_len, c, n_q, kv_format, dtype);
+}
+
+int kvb_rope_kv_append_q8_paged(kvb_stream_t stream, void* qkv, size_t qkv_len, size_t n_seq,
+                                size_t t, const int32_t* pos, const float* cos_t,
+                                const float* sin_t, size_t table_len, void* k_pool, void* v_pool,
+                                float* k_scales, float* v_scales, size_t pool_len, size_t scale_len,
+                                const int32_t* block_table, size_t max_blocks, size_t block_size,
+                                size_t n_q, size_t n_kv, size_t head_dim, int kv_format,
+                                int dtype) {
+    KVB_CHECK_DTYPE(dtype);
+    KVB_CHECK(valid_kv_format(kv_format), "unknown KV format %d", kv_format);
+    Kv8Place c;
+    const int st = kv8_place_paged("rope_kv_append_q8_paged", c, k_pool, v_pool, k_scales, v_scales,
+                                   pool_len, scale_len, block_table, max_blocks, block_size, n_seq,
+                                   n_kv, head_dim);
+    if (st) return st;
+    return kv8_append("rope_kv_append_q8_paged", stream, qkv, qkv_len, n_seq, t, pos, cos_t, sin_t,
+                      table_len, c, n_q, kv_format, dtype);
+}
+
+int kvb_kv_read_q8(kvb_stream_t stream, const void* kc, const void* vc, const float* ks,
+                   const float* vs, size_t seq_stride, size_t cache_len, size_t scale_len,
+                   const int32_t* pos, size_t n_seq, size_t t, size_t n_kv, size_t head_dim,
+                   size_t max_seq, void* k_out, void* v_out, size_t out_len, size_t out_rows,
+                   int kv_format, int dtype) {
+    KVB_CHECK_DTYPE(dtype);
+    KVB_CHECK(valid_kv_format(kv_format), "unknown KV format %d", kv_format);
+    Kv8Place c;
+    const int st = kv8_place_contiguous("kv_read_q8", c, kc, vc, ks, vs, seq_stride, cache_len,
+                                        scale_len, n_seq, n_kv, head_dim, max_seq);
+    if (st) return st;
+    return kv8_read("kv_read_q8", stream, c, pos, n_seq, t, k_out, v_out, out_len, out_rows,
+                    kv_format, dtype);
+}
+
+int kvb_kv_read_q8_paged(kvb_stream_t stream, const void* k_pool, const void* v_pool,
+                         const float* k_scales, const float* v_scales, size_t pool_len,
+                         size_t scale_len, const int32_t* block_table, size_t max_blocks,
+                         size_t block_size, const int32_t* pos, size_t n_seq, size_t t, size_t n_kv,
+                         size_t head_dim, void* k_out, void* v_out, size_t out_len,
+                         size_t out_rows, int kv_format, int dtype) {
+    KVB_CHECK_DTYPE(dtype);
+    KVB_CHECK(valid_kv_format(kv_format), "unknown KV format %d", kv_format);
+    Kv8Place c;
+    const int st = kv8_place_paged("kv_read_q8_paged", c, k_pool, v_pool, k_scales, v_scales,
+                                   pool_len, scale_len, block_table, max_blocks, block_size, n_seq,
+                                   n_kv, head_dim);
+    if (st) return st;
+    return kv8_read("kv_read_q8_paged", stream, c, pos, n_seq, t, k_out, v_out, out_len, out_rows,
+                    kv_format, dtype);
+}
+
+size_t kvb_attention_decode_q8_workspace_bytes(size_t n_seq, size_t max_len, size_t n_q,
+                                               size_t n_kv, size_t head_dim) {
+    (void)n_seq, (void)max_len, (void)n_q, (void)n_kv, (void)head_dim;
+    return 0;
+}
+
+int kvb_attention_decode_q8(kvb_stream_t stream, const void* q, size_t q_row_stride, const void* kc,
+                            const void* vc, const float* ks, const float* vs, size_t seq_stride,
+                            size_t cache_len, size_t scale_len, const int32_t* lens, size_t n_seq,
+                            size_t max_len, size_t n_q, size_t n_kv, size_t head_dim,
+                            size_t max_seq, float scale, void* out, size_t out_row_stride,
+                            void* workspace, size_t workspace_len, int kv_format, int dtype) {
+    KVB_CHECK_DTYPE(dtype);
+    KVB_CHECK(valid_kv_format(kv_format), "unknown KV format %d", kv_format);
+    GeneralDecodeArgs a;
+    int st = decode_args("attention_decode_q8", a, q, q_row_stride, lens, n_seq, max_len, n_q, n_kv,
+                         head_dim, scale, out, out_row_stride);
+    if (st) return st;
+    KVB_CHECK(max_len <= max_seq, "attention_decode_q8: max_len %zu exceeds max_seq %zu", max_len,
+              max_seq);
+    Kv8Place c;
+    st = kv8_place_contiguous("attention_decode_q8", c, kc, vc, ks, vs, seq_stride, cache_len,
+                              scale_len, n_seq, n_kv, head_dim, max_seq);
+    if (st) return st;
+    if (n_seq == 0) return KVB_OK;
+    return KVB_KV8_DISPATCH(launch_q8_decode, dtype, kv_format, stream, a, c, n_seq, workspace,
+                            workspace_len);
+}
+
+int kvb_attention_decode_q8_paged(kvb_stream_t stream, const void* q, size_t q_row_stride,
+                                  const void* k_pool, const void* v_pool, const float* k_scales,
+                                  const float* v_scales, size_t pool_len, size_t scale_len,
+                                  const int32_t* block_table, size_t max_blocks, size_t block_size,
+                                  const int32_t* lens, size_t n_seq, size_t max_len, size_t n_q,
+                                  size_t n_kv, size_t head_dim, float scale, void* out,
+                                  size_t out_row_stride, void* workspace, size_t workspace_len,
+                                  int kv_format, int dtype) {
+    KVB_CHECK_DTYPE(dtype);
+    KVB_CHECK(valid_kv_format(kv_format), "unknown KV format %d", kv_format);
+    GeneralDecodeArgs a;
+    int st = decode_args("attention_decode_q8_paged", a, q, q_row_stride, lens, n_seq, max_len, n_q,
+                         n_kv, head_dim, scale, out, out_row_stride);
+    if (st) return st;
+    Kv8Place c;
+    st = kv8_place_paged("attention_decode_q8_paged", c, k_pool, v_pool, k_scales, v_scales,
+                         pool_len, scale_len, block_table, max_blocks, block_size, n_seq, n_kv,
+                         head_dim);
+    if (st) return st;
+    KVB_CHECK(max_len <= max_blocks * block_size,
+              "attention_decode_q8_paged: max_len %zu exceeds %zu blocks of %zu", max_len,
+              max_blocks, block_size);
+    if (n_seq == 0) return KVB_OK;
+    return KVB_KV8_DISPATCH(launch_q8_decode, dtype, kv_format, stream, a, c, n_seq, workspace,
+                            workspace_len);
+}
+
+size_t kvb_attention_decode_shared_workspace_bytes(size_t n_seq, size_t shared_len, size_t max_own,
+                                                   size_t n_q, size_t n_kv, size_t head_dim) {
+    (void)n_seq, (void)shared_len, (void)max_own, (void)n_q, (void)n_kv, (void)head_dim;
+    return 0;
+}
+
+int kvb_attention_decode_shared(kvb_stream_t stream, const void* q, size_t q_row_stride,
+                                const void* pk, const void* pv, size_t prefix_len,
+                                size_t prefix_rows, const void* kc, const void* vc,
+                                size_t seq_stride, size_t cache_len, const int32_t* lens,
+                                size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
+                                size_t head_dim, size_t max_seq, float scale, void* out,
+                                size_t out_row_stride, void* workspace, size_t workspace_len,
+                                int dtype) {
+    KVB_CHECK_DTYPE(dtype);
+    GeneralDecodeArgs a;
+    const int st = decode_args("attention_decode_shared", a, q, q_row_stride, lens, n_seq, max_len,
+                               n_q, n_kv, head_dim, scale, out, out_row_stride);
+    if (st) return st;
+    KVB_CHECK(prefix_len <= prefix_rows && fits_i32(n_kv * prefix_rows) &&
+                  fits_i32(prefix_len + max_len),
+              "attention_decode_shared: prefix of %zu keys in buffers of %zu", prefix_len,
+              prefix_rows);
+    KVB_CHECK(max_len <= max_seq && fits_i32(max_seq) && fits_i32(n_kv * max_seq),
+              "attention_decode_shared: max_len %zu exceeds max_seq %zu", max_len, max_seq);
+    const size_t per_seq = n_kv * max_seq * head_dim;
+    KVB_CHECK(seq_stride >= per_seq && seq_stride % head_dim == 0,
+              "attention_decode_shared: seq_stride %zu must be a multiple of head_dim and at least "
+              "%zu", seq_stride, per_seq);
+    KVB_CHECK(n_seq == 0 ||
+                  (cache_len >= per_seq && (n_seq == 1 || (cache_len - per_seq) / (n_seq - 1) >= seq_stride)),
+              "attention_decode_shared: cache of %zu elems is too small", cache_len);
+    KVB_CHECK((max_len == 0 || (kc != nullptr && vc != nullptr)) &&
+                  (prefix_len == 0 || (pk != nullptr && pv != nullptr)),
+              "attention_decode_shared: null cache");
+    if (n_seq == 0) return KVB_OK;
+    auto go = [&](auto tag) {
+        SharedSource<decltype(tag)> s;
+        memset(&s, 0, sizeof s);
+        s.pk = static_cast<const uint16_t*>(pk);
+        s.pv = static_cast<const uint16_t*>(pv);
+        s.prefix = (int)prefix_len;
+        s.prefix_rows = (int)prefix_rows;
+        s.kc = static_cast<const uint16_t*>(kc);
+        s.vc = static_cast<const uint16_t*>(vc);
+        s.seq_rows = (long long)(seq_stride / head_dim);
+        s.n_kv = (int)n_kv;
+        s.hd = (int)head_dim;
+        s.max_seq = (int)max_seq;
+        return launch_shared(stream, a, s, n_seq, workspace, workspace_len);
+    };
+    return dtype == KVB_BF16 ? go(__nv_bfloat16()) : go(__half());
+}
+
+int kvb_attention_decode_shared_paged(kvb_stream_t stream, const void* q, size_t q_row_stride,
+                                      const void* k_pool, const void* v_pool, size_t pool_len,
+                                      const int32_t* block_table, size_t max_blocks,
+                                      size_t block_size, size_t shared_len, const int32_t* lens,
+                                      size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
+                                      size_t head_dim, float scale, void* out,
+                                      size_t out_row_stride, void* workspace, size_t workspace_len,
+                                      int dtype) {
+    KVB_CHECK_DTYPE(dtype);
+    GeneralDecodeArgs a;
+    const int st = decode_args("attention_decode_shared_paged", a, q, q_row_stride, lens, n_seq,
+                               max_len, n_q, n_kv, head_dim, scale, out, out_row_stride);
+    if (st) return st;
+    KVB_CHECK(block_table != nullptr, "attention_decode_shared_paged: null block table");
+    KVB_CHECK(block_size > 0 && fits_i32(block_size) && fits_i32(n_kv * block_size) &&
+                  fits_i32(max_blocks) && fits_i32(max_blocks * block_size) &&
+                  fits_i32(n_seq * max_blocks),
+              "attention_decode_shared_paged: a dimension does not fit in i32 (or block_size is 0)");
+    const size_t per_block = n_kv * block_size * head_dim;
+    KVB_CHECK(pool_len % per_block == 0 && fits_i32(pool_len / per_block),
+              "attention_decode_shared_paged: pool of %zu elems is not a whole number of %zu-elem "
+              "blocks", pool_len, per_block);
+    KVB_CHECK(max_len <= max_blocks * block_size && shared_len <= max_blocks * block_size,
+              "attention_decode_shared_paged: max_len %zu or shared_len %zu exceeds %zu blocks of %zu",
+              max_len, shared_len, max_blocks, block_size);
+    KVB_CHECK(k_pool != nullptr && v_pool != nullptr, "attention_decode_shared_paged: null pool");
+    if (n_seq == 0) return KVB_OK;
+    auto go = [&](auto tag) {
+        SharedSource<decltype(tag)> s;
+        memset(&s, 0, sizeof s);
+        s.prefix = (int)shared_len;
+        s.kc = static_cast<const uint16_t*>(k_pool);
+        s.vc = static_cast<const uint16_t*>(v_pool);
+        s.n_kv = (int)n_kv;
+        s.hd = (int)head_dim;
+        s.max_seq = (int)(max_blocks * block_size);
+        s.block_table = block_table;
+        s.max_blocks = (int)max_blocks;
+        s.block_size = (int)block_size;
+        s.n_blocks = (int)(pool_len / per_block);
+        return launch_shared(stream, a, s, n_seq, workspace, workspace_len);
+    };
+    return dtype == KVB_BF16 ? go(__nv_bfloat16()) : go(__half());
+}
+
+}  // extern "C"

@@ -66,6 +66,15 @@ def dtype_tag(t: torch.Tensor) -> int:
     raise ShapeError(f"unsupported element type {t.dtype} (bf16 or f16)")
 
 
+def kv_format(t: torch.Tensor) -> int:
+    """Tag of an 8-bit KV cache's element type."""
+    if t.dtype == torch.int8:
+        return L.KVB_KV_INT8
+    if t.dtype == torch.float8_e4m3fn:
+        return L.KVB_KV_E4M3
+    raise ShapeError(f"unsupported KV cache element type {t.dtype} (int8 or float8_e4m3fn)")
+
+
 def _ptr(t):
     if t is None:
         return None
@@ -322,6 +331,184 @@ class Gpu:
                                                   _ptr(vc), kc.numel(), _ptr(out), out.numel(),
                                                   n_seq, t, pos0, n_q, n_kv, head_dim, max_seq,
                                                   dtype_tag(qkv)))
+
+    # ------------------------------------------------ 8-bit KV cache
+    def _check_on(self, name, i32, f32, *others):
+        """Device and element types of the tensors of one call."""
+        if torch.cuda.current_device() != self.device.index:
+            raise ShapeError(f"{name}: the current device is not {self.device}")
+        for t in (*i32, *f32, *others):
+            if t is not None and t.device != self.device:
+                raise ShapeError(f"{name}: a tensor is on {t.device}, not on {self.device}")
+        for t in i32:
+            if t.dtype != torch.int32:
+                raise ShapeError(f"{name}: positions, lengths and block tables must be int32")
+        for t in f32:
+            if t is not None and t.dtype != torch.float32:
+                raise ShapeError(f"{name}: scales and cos/sin tables must be float32")
+
+    def _check_q8(self, name, kc, vc, ks, vs):
+        if kc.dtype != vc.dtype or kc.numel() != vc.numel() or ks.numel() != vs.numel():
+            raise ShapeError(f"{name}: K and V caches (or their scales) differ")
+        return kv_format(kc)
+
+    def rope_kv_append_q8(self, qkv, n_seq, t, pos, cos, sin, kc, vc, ks, vs, seq_stride, n_q,
+                          n_kv, head_dim, max_seq):
+        """kvb_rope_kv_append_q8: rows of sequence b at positions pos[b].. rotated in place,
+        their k and v quantised into the 8-bit cache (codes kc / vc, int8 or float8_e4m3fn;
+        f32 scales ks / vs, one per position and KV head).  cos = sin = None: no rotation."""
+        self._check_on("rope_kv_append_q8", (pos,), (cos, sin, ks, vs), qkv, kc, vc)
+        fmt = self._check_q8("rope_kv_append_q8", kc, vc, ks, vs)
+        if pos.numel() != n_seq or (cos is not None and sin is not None
+                                    and cos.numel() != sin.numel()):
+            raise ShapeError("rope_kv_append_q8: one position per sequence, cos and sin alike")
+        check(self._lib.kvb_rope_kv_append_q8(
+            self._s, _ptr(qkv), qkv.numel(), n_seq, t, _ptr(pos), _ptr(cos), _ptr(sin),
+            cos.numel() if cos is not None else 0, _ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs),
+            seq_stride, kc.numel(), ks.numel(), n_q, n_kv, head_dim, max_seq, fmt,
+            dtype_tag(qkv)))
+
+    def rope_kv_append_q8_paged(self, qkv, n_seq, t, pos, cos, sin, k_pool, v_pool, k_scales,
+                                v_scales, block_table, max_blocks, block_size, n_q, n_kv,
+                                head_dim):
+        """kvb_rope_kv_append_q8_paged: the same into pools [n_blocks, n_kv, block_size,
+        head_dim] of codes and [n_blocks, n_kv, block_size] of scales."""
+        self._check_on("rope_kv_append_q8_paged", (pos, block_table), (cos, sin, k_scales, v_scales),
+                       qkv, k_pool, v_pool)
+        fmt = self._check_q8("rope_kv_append_q8_paged", k_pool, v_pool, k_scales, v_scales)
+        if pos.numel() != n_seq or block_table.numel() != n_seq * max_blocks or (
+                cos is not None and sin is not None and cos.numel() != sin.numel()):
+            raise ShapeError("rope_kv_append_q8_paged: one position and one table row per sequence, "
+                             "cos and sin alike")
+        check(self._lib.kvb_rope_kv_append_q8_paged(
+            self._s, _ptr(qkv), qkv.numel(), n_seq, t, _ptr(pos), _ptr(cos), _ptr(sin),
+            cos.numel() if cos is not None else 0, _ptr(k_pool), _ptr(v_pool), _ptr(k_scales),
+            _ptr(v_scales), k_pool.numel(), k_scales.numel(), _ptr(block_table), max_blocks,
+            block_size, n_q, n_kv, head_dim, fmt, dtype_tag(qkv)))
+
+    def kv_read_q8(self, kc, vc, ks, vs, seq_stride, pos, n_seq, t, n_kv, head_dim, max_seq, k_out,
+                   v_out, out_rows):
+        """kvb_kv_read_q8: positions pos[b] .. pos[b]+t-1 of an 8-bit cache as 16-bit rows
+        0 .. t-1 of k_out / v_out [n_seq, n_kv, out_rows, head_dim]."""
+        self._check_on("kv_read_q8", (pos,), (ks, vs), kc, vc, k_out, v_out)
+        fmt = self._check_q8("kv_read_q8", kc, vc, ks, vs)
+        if pos.numel() != n_seq or k_out.dtype != v_out.dtype or k_out.numel() != v_out.numel():
+            raise ShapeError("kv_read_q8: one position per sequence, k_out and v_out alike")
+        check(self._lib.kvb_kv_read_q8(
+            self._s, _ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs), seq_stride, kc.numel(), ks.numel(),
+            _ptr(pos), n_seq, t, n_kv, head_dim, max_seq, _ptr(k_out), _ptr(v_out), k_out.numel(),
+            out_rows, fmt, dtype_tag(k_out)))
+
+    def kv_read_q8_paged(self, k_pool, v_pool, k_scales, v_scales, block_table, max_blocks,
+                         block_size, pos, n_seq, t, n_kv, head_dim, k_out, v_out, out_rows):
+        """kvb_kv_read_q8_paged: kv_read_q8 through a block table."""
+        self._check_on("kv_read_q8_paged", (pos, block_table), (k_scales, v_scales), k_pool, v_pool,
+                       k_out, v_out)
+        fmt = self._check_q8("kv_read_q8_paged", k_pool, v_pool, k_scales, v_scales)
+        if (pos.numel() != n_seq or block_table.numel() != n_seq * max_blocks
+                or k_out.dtype != v_out.dtype or k_out.numel() != v_out.numel()):
+            raise ShapeError("kv_read_q8_paged: one position and one table row per sequence, "
+                             "k_out and v_out alike")
+        check(self._lib.kvb_kv_read_q8_paged(
+            self._s, _ptr(k_pool), _ptr(v_pool), _ptr(k_scales), _ptr(v_scales), k_pool.numel(),
+            k_scales.numel(), _ptr(block_table), max_blocks, block_size, _ptr(pos), n_seq, t, n_kv,
+            head_dim, _ptr(k_out), _ptr(v_out), k_out.numel(), out_rows, fmt, dtype_tag(k_out)))
+
+    def attention_decode_q8_workspace_bytes(self, n_seq, max_len, n_q, n_kv, head_dim) -> int:
+        return int(self._lib.kvb_attention_decode_q8_workspace_bytes(n_seq, max_len, n_q, n_kv,
+                                                                     head_dim))
+
+    @staticmethod
+    def _check_rows(name, t, n_seq, row_stride, n_q, head_dim):
+        """t holds n_seq rows of n_q * head_dim elements, row_stride apart."""
+        if n_seq and t.numel() < (n_seq - 1) * row_stride + n_q * head_dim:
+            raise ShapeError(f"{name}: {t.numel()} elements hold no {n_seq} rows {row_stride} apart")
+
+    def _check_attention(self, name, q, q_row_stride, out, out_row_stride, n_seq, n_q, head_dim,
+                         *caches):
+        if out.dtype != q.dtype or any(c.dtype != q.dtype for c in caches):
+            raise ShapeError(f"{name}: q, out and 16-bit caches must have one type")
+        self._check_rows(name, q, n_seq, q_row_stride, n_q, head_dim)
+        self._check_rows(name, out, n_seq, out_row_stride, n_q, head_dim)
+
+    def attention_decode_q8(self, q, q_row_stride, kc, vc, ks, vs, seq_stride, lens, max_len, n_q,
+                            n_kv, head_dim, max_seq, out, out_row_stride, scale=None,
+                            workspace=None):
+        """kvb_attention_decode_q8: attention_decode over an 8-bit cache."""
+        self._check_on("attention_decode_q8", (lens,), (ks, vs), q, kc, vc, out, workspace)
+        fmt = self._check_q8("attention_decode_q8", kc, vc, ks, vs)
+        self._check_attention("attention_decode_q8", q, q_row_stride, out, out_row_stride,
+                              lens.numel(), n_q, head_dim)
+        scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
+        ws_len = workspace.numel() * workspace.element_size() if workspace is not None else 0
+        check(self._lib.kvb_attention_decode_q8(
+            self._s, _ptr(q), q_row_stride, _ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs), seq_stride,
+            kc.numel(), ks.numel(), _ptr(lens), lens.numel(), max_len, n_q, n_kv, head_dim, max_seq,
+            scale, _ptr(out), out_row_stride, _ptr(workspace), ws_len, fmt, dtype_tag(q)))
+
+    def attention_decode_q8_paged(self, q, q_row_stride, k_pool, v_pool, k_scales, v_scales,
+                                  block_table, max_blocks, block_size, lens, max_len, n_q, n_kv,
+                                  head_dim, out, out_row_stride, scale=None, workspace=None):
+        """kvb_attention_decode_q8_paged: attention_decode_paged over 8-bit pools."""
+        self._check_on("attention_decode_q8_paged", (lens, block_table), (k_scales, v_scales), q,
+                       k_pool, v_pool, out, workspace)
+        fmt = self._check_q8("attention_decode_q8_paged", k_pool, v_pool, k_scales, v_scales)
+        if block_table.numel() != lens.numel() * max_blocks:
+            raise ShapeError("attention_decode_q8_paged: one table row per sequence")
+        self._check_attention("attention_decode_q8_paged", q, q_row_stride, out, out_row_stride,
+                              lens.numel(), n_q, head_dim)
+        scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
+        ws_len = workspace.numel() * workspace.element_size() if workspace is not None else 0
+        check(self._lib.kvb_attention_decode_q8_paged(
+            self._s, _ptr(q), q_row_stride, _ptr(k_pool), _ptr(v_pool), _ptr(k_scales),
+            _ptr(v_scales), k_pool.numel(), k_scales.numel(), _ptr(block_table), max_blocks,
+            block_size, _ptr(lens), lens.numel(), max_len, n_q, n_kv, head_dim, scale, _ptr(out),
+            out_row_stride, _ptr(workspace), ws_len, fmt, dtype_tag(q)))
+
+    # ------------------------------------------------ shared-prefix decode attention
+    def attention_decode_shared_workspace_bytes(self, n_seq, shared_len, max_own, n_q, n_kv,
+                                                head_dim) -> int:
+        """max_own: the largest number of own keys (paged: max_len - shared_len)."""
+        return int(self._lib.kvb_attention_decode_shared_workspace_bytes(n_seq, shared_len, max_own,
+                                                                         n_q, n_kv, head_dim))
+
+    def attention_decode_shared(self, q, q_row_stride, pk, pv, prefix_len, prefix_rows, kc, vc,
+                                seq_stride, lens, max_len, n_q, n_kv, head_dim, max_seq, out,
+                                out_row_stride, scale=None, workspace=None):
+        """kvb_attention_decode_shared: every sequence attends to the keys [0, prefix_len) of
+        pk / pv [n_kv, prefix_rows, head_dim], read once for all, then to its own lens[b]."""
+        self._check_on("attention_decode_shared", (lens,), (), q, pk, pv, kc, vc, out, workspace)
+        if (kc.numel() != vc.numel() or pk.numel() != pv.numel()
+                or pk.numel() != n_kv * prefix_rows * head_dim):
+            raise ShapeError("attention_decode_shared: bad cache or prefix sizes")
+        self._check_attention("attention_decode_shared", q, q_row_stride, out, out_row_stride,
+                              lens.numel(), n_q, head_dim, pk, pv, kc, vc)
+        scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
+        ws_len = workspace.numel() * workspace.element_size() if workspace is not None else 0
+        check(self._lib.kvb_attention_decode_shared(
+            self._s, _ptr(q), q_row_stride, _ptr(pk), _ptr(pv), prefix_len, prefix_rows, _ptr(kc),
+            _ptr(vc), seq_stride, kc.numel(), _ptr(lens), lens.numel(), max_len, n_q, n_kv, head_dim,
+            max_seq, scale, _ptr(out), out_row_stride, _ptr(workspace), ws_len, dtype_tag(q)))
+
+    def attention_decode_shared_paged(self, q, q_row_stride, k_pool, v_pool, block_table,
+                                      max_blocks, block_size, shared_len, lens, max_len, n_q, n_kv,
+                                      head_dim, out, out_row_stride, scale=None, workspace=None):
+        """kvb_attention_decode_shared_paged: attention_decode_paged where the first shared_len
+        keys of every sequence are the same (read through row 0 of the block table)."""
+        self._check_on("attention_decode_shared_paged", (lens, block_table), (), q, k_pool, v_pool,
+                       out, workspace)
+        if k_pool.numel() != v_pool.numel() or block_table.numel() != lens.numel() * max_blocks:
+            raise ShapeError("attention_decode_shared_paged: pool sizes differ, or not one table "
+                             "row per sequence")
+        self._check_attention("attention_decode_shared_paged", q, q_row_stride, out, out_row_stride,
+                              lens.numel(), n_q, head_dim, k_pool, v_pool)
+        scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
+        ws_len = workspace.numel() * workspace.element_size() if workspace is not None else 0
+        check(self._lib.kvb_attention_decode_shared_paged(
+            self._s, _ptr(q), q_row_stride, _ptr(k_pool), _ptr(v_pool), k_pool.numel(),
+            _ptr(block_table), max_blocks, block_size, shared_len, _ptr(lens), lens.numel(), max_len,
+            n_q, n_kv, head_dim, scale, _ptr(out), out_row_stride, _ptr(workspace), ws_len,
+            dtype_tag(q)))
 
     def lm_head_argmax(self, x, w, rows, hidden, vocab, ids, workspace=None, advance=None,
                        advance2=None):

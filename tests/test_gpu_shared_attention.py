@@ -1,0 +1,253 @@
+"""Decode attention of sequences that share a prefix, contiguous and paged, against f64."""
+import numpy as np
+import pytest
+import torch
+
+import kv8_ref as R
+from gpu_util import dev, normal16
+from oracle import oracle as O
+
+pytestmark = pytest.mark.gpu
+
+# Weights of the softmax: head + remainder in bf16 (16 bits: 2^-15 with the truncated head),
+# one f16 for f16 inputs (half a step, 2^-11).
+W_EPS = {"bf16": 2.0 ** -15, "f16": 2.0 ** -11}
+
+
+@pytest.fixture(scope="module")
+def g():
+    from kvasir_b200 import Gpu
+    return Gpu(0)
+
+
+def _f64(bits, dtype, *shape):
+    return O.to_f32(bits, dtype).astype(np.float64).reshape(shape)
+
+
+class Case:
+    """Prefix rows [n_kv, P, hd], own rows [n_seq, n_kv, own_max, hd], as bits and f64."""
+
+    def __init__(self, rng, prefix, lens, n_q, n_kv, hd, dtype, q_std=1.0):
+        self.prefix, self.lens, self.n_q, self.n_kv, self.hd, self.dtype = prefix, lens, n_q, n_kv, hd, dtype
+        self.n_seq, self.max_seq = len(lens), max(lens) + 5
+        nan = 0x7FFF
+        self.q = normal16(rng, self.n_seq * n_q * hd, std=q_std, dtype=dtype)
+        self.rows = prefix + 3  # rows past the prefix hold garbage
+        self.pk, self.pv = (normal16(rng, n_kv * self.rows * hd, dtype=dtype).reshape(n_kv, self.rows, hd)
+                            for _ in range(2))
+        self.kc, self.vc = (normal16(rng, self.n_seq * n_kv * self.max_seq * hd, dtype=dtype).reshape(
+            self.n_seq, n_kv, self.max_seq, hd) for _ in range(2))
+        self.qf = _f64(self.q, dtype, self.n_seq, n_q, hd)
+        self.f = [_f64(x.ravel(), dtype, *x.shape) for x in (self.pk, self.pv, self.kc, self.vc)]
+        for x in (self.pk, self.pv):
+            x[:, prefix:] = nan
+        for x in (self.kc, self.vc):
+            for b, n in enumerate(lens):
+                x[b, :, n:] = nan
+        self.ld = torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+    def kv_of(self, b, h):
+        p, n = self.prefix, self.lens[b]
+        return tuple(np.concatenate([self.f[i][h, :p], self.f[i + 2][b, h, :n]]) for i in (0, 1))
+
+    def out(self):
+        return torch.full((self.n_seq, self.n_q * self.hd), 9.0, dtype=R.TDT[self.dtype], device="cuda")
+
+    def ws(self, g, own):
+        n = g.attention_decode_shared_workspace_bytes(self.n_seq, self.prefix, own, self.n_q, self.n_kv,
+                                                      self.hd)
+        return torch.empty(max(16, n), dtype=torch.uint8, device="cuda")
+
+    def contiguous(self, g, workspace=True):
+        d, out = self.dtype, self.out()
+        g.attention_decode_shared(dev(self.q, d), self.n_q * self.hd, dev(self.pk, d), dev(self.pv, d),
+                                  self.prefix, self.rows, dev(self.kc, d), dev(self.vc, d),
+                                  self.n_kv * self.max_seq * self.hd, self.ld, max(self.lens), self.n_q,
+                                  self.n_kv, self.hd, self.max_seq, out, self.n_q * self.hd,
+                                  workspace=self.ws(g, max(self.lens)) if workspace else None)
+        return out
+
+    def pools(self, block, seed=3):
+        """One pool: the prefix's whole blocks once, the rest of each sequence by itself."""
+        whole = self.prefix // block
+        total = self.prefix + self.max_seq
+        per = -(-total // block)
+        rng = np.random.default_rng(seed)
+        n_blocks = whole + self.n_seq * (per - whole) + 3
+        ids = rng.permutation(n_blocks).astype(np.int32)
+        table = np.empty((self.n_seq, per), np.int32)
+        table[:, :whole] = ids[:whole]
+        table[:, whole:] = ids[whole:whole + self.n_seq * (per - whole)].reshape(self.n_seq, -1)
+        pools = []
+        for p, own in ((self.pk, self.kc), (self.pv, self.vc)):
+            pool = np.full((n_blocks, self.n_kv, block, self.hd), 0x7FFF, np.uint16)
+            for b in range(self.n_seq):
+                x = np.full((self.n_kv, per * block, self.hd), 0x7FFF, np.uint16)
+                x[:, :self.prefix] = p[:, :self.prefix]
+                x[:, self.prefix:total] = own[b]
+                for i in range(per):
+                    pool[table[b, i]] = x[:, i * block:(i + 1) * block]
+            pools.append(pool)
+        for b, n in enumerate(self.lens):
+            table[b, -(-(self.prefix + n) // block):] = -1
+        return pools, table
+
+    def paged(self, g, block, workspace=True):
+        d, out = self.dtype, self.out()
+        (kp, vp), table = self.pools(block)
+        g.attention_decode_shared_paged(dev(self.q, d), self.n_q * self.hd, dev(kp, d), dev(vp, d),
+                                        torch.from_numpy(table).cuda(), table.shape[1], block,
+                                        self.prefix, self.ld + self.prefix,
+                                        self.prefix + max(self.lens), self.n_q, self.n_kv, self.hd, out,
+                                        self.n_q * self.hd,
+                                        workspace=self.ws(g, max(self.lens)) if workspace else None)
+        return out
+
+    def check(self, out, name=""):
+        R.check_attention(out, self.qf, self.kv_of, self.n_kv, R.default_scale(self.hd), self.dtype,
+                          W_EPS[self.dtype], name)
+
+
+@pytest.mark.parametrize("prefix", [0, 1, 63, 64, 65, 96, 300, 1000])
+@pytest.mark.parametrize("n_q,n_kv,hd", [(32, 8, 64), (4, 4, 64), (6, 2, 64), (14, 2, 64), (16, 1, 64),
+                                         (20, 1, 64), (4, 2, 128), (4, 2, 80)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_against_f64(g, prefix, n_q, n_kv, hd, dtype):
+    c = Case(np.random.default_rng(prefix + n_q), prefix, [1, 0, 64, 65, 200, 31, 7], n_q, n_kv, hd, dtype)
+    for ws in (True, False):
+        c.check(c.contiguous(g, ws), "contiguous")
+        c.check(c.paged(g, 64, ws), "paged")
+    assert g.device_error() == 0
+
+
+@pytest.mark.parametrize("n_seq", [1, 2, 31, 32, 33, 64, 100])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_batch_sizes(g, n_seq, dtype):
+    """Row tiles with one row left over, filled exactly, and less than one."""
+    rng = np.random.default_rng(n_seq)
+    c = Case(rng, 700, [int(x) for x in rng.integers(0, 90, n_seq)] or [1], 8, 2, 64, dtype)
+    c.check(c.contiguous(g), "contiguous")
+    c.check(c.paged(g, 128), "paged")
+    assert g.device_error() == 0
+
+
+@pytest.mark.parametrize("block", [8, 16, 32, 64, 96, 256])
+def test_block_sizes(g, block):
+    c = Case(np.random.default_rng(block), 515, [1, 100, 40], 8, 2, 64, "bf16")
+    c.check(c.paged(g, block))
+    assert g.device_error() == 0
+
+
+def test_long_prefix_and_peaked_rows(g):
+    """Keys split over CTAs and joined; large scores (a few keys take all the weight)."""
+    for q_std, dtype in ((1.0, "bf16"), (6.0, "bf16"), (6.0, "f16")):
+        c = Case(np.random.default_rng(5), 9000, [500, 0, 3, 1500], 8, 2, 64, dtype, q_std)
+        out = c.contiguous(g)
+        c.check(out)
+        assert torch.equal(out, c.contiguous(g))
+        paged = c.paged(g, 64)
+        c.check(paged)
+        assert torch.equal(paged, c.paged(g, 64))
+    assert g.device_error() == 0
+
+
+def test_empty_rows(g):
+    """No prefix and no keys: zeros."""
+    c = Case(np.random.default_rng(6), 0, [0, 5, 0], 8, 2, 64, "bf16")
+    for out in (c.contiguous(g), c.paged(g, 64)):
+        assert bool((out[[0, 2]] == 0).all())
+        c.check(out)
+
+
+@pytest.mark.parametrize("hd", [64, 80])
+def test_paged_lengths_below_the_prefix(g, hd):
+    """A sequence shorter than shared_len attends to its own first keys only; 0 gives zeros."""
+    c = Case(np.random.default_rng(7), 300, [10, 20, 30, 40], 8, 2, hd, "bf16")
+    (kp, vp), table = c.pools(64)
+    short = [0, 1, 130, 299]
+    out = c.out()
+    g.attention_decode_shared_paged(dev(c.q), c.n_q * hd, dev(kp), dev(vp), torch.from_numpy(table).cuda(),
+                                    table.shape[1], 64, 300,
+                                    torch.tensor(short, dtype=torch.int32, device="cuda"), 340, c.n_q,
+                                    c.n_kv, hd, out, c.n_q * hd, workspace=c.ws(g, 40))
+    assert g.device_error() == 0
+    R.check_attention(out, c.qf, lambda b, h: (c.f[0][h, :short[b]], c.f[1][h, :short[b]]), c.n_kv,
+                      R.default_scale(hd), "bf16", W_EPS["bf16"])
+    assert bool((out[0] == 0).all())
+
+
+@pytest.mark.parametrize("hd", [64, 80])
+def test_bad_lengths_and_blocks_are_reported(g, hd):
+    c = Case(np.random.default_rng(8), 128, [64, 64, 64], 4, 1, hd, "bf16")
+    good = c.contiguous(g)
+    c.ld = torch.tensor([-1, 64, 70], dtype=torch.int32, device="cuda")
+    out = c.contiguous(g)
+    assert g.device_error() == 2
+    assert torch.equal(out[1:], good[1:])
+    R.check_attention(out[:1], c.qf[:1], lambda b, h: (c.f[0][h, :128], c.f[1][h, :128]), c.n_kv,
+                      R.default_scale(hd), "bf16", W_EPS["bf16"])
+    # paged: a bad entry among the prefix's and one among a sequence's own
+    (kp, vp), table = c.pools(64)
+    table[0, 1], table[2, 2] = kp.shape[0], -7
+    out = c.out()
+    g.attention_decode_shared_paged(dev(c.q), c.n_q * hd, dev(kp), dev(vp), torch.from_numpy(table).cuda(),
+                                    table.shape[1], 64, 128,
+                                    torch.full((3,), 192, dtype=torch.int32, device="cuda"), 192, c.n_q,
+                                    c.n_kv, hd, out, c.n_q * hd, workspace=c.ws(g, 64))
+    assert g.device_error() == 4
+
+    def zeroed(b, h):
+        k, v = c.kv_of(b, h)
+        k[64:128], v[64:128] = 0, 0
+        if b == 2:
+            k[128:], v[128:] = 0, 0
+        return k, v
+    R.check_attention(out, c.qf, zeroed, c.n_kv, R.default_scale(hd), "bf16", W_EPS["bf16"])
+
+
+def test_equals_decode_over_the_same_keys(g):
+    """attention_decode on caches that hold prefix and own keys together, to the bound twice."""
+    c = Case(np.random.default_rng(12), 320, [100, 50, 1, 200], 32, 8, 64, "bf16")
+    shared = c.contiguous(g)
+    max_seq = 320 + c.max_seq
+    k, v = (np.concatenate([np.broadcast_to(p[None, :, :320], (4, 8, 320, 64)), own], 2)
+            for p, own in ((c.pk, c.kc), (c.pv, c.vc)))
+    out = c.out()
+    g.attention_decode(dev(c.q), 32 * 64, dev(k), dev(v), 8 * max_seq * 64, c.ld + 320, 520, 32, 8, 64,
+                       max_seq, out, 32 * 64)
+    c.check(shared)
+    c.check(out)
+
+
+@pytest.mark.parametrize("hd", [64, 80])
+def test_strides_graph_and_stream(g, hd):
+    from kvasir_b200 import Gpu
+    c = Case(np.random.default_rng(13), 500, [70, 3, 64], 8, 2, hd, "bf16")
+    want = c.contiguous(g)
+    n_q = c.n_q
+    qs, os_ = (n_q + 2 * c.n_kv) * hd, n_q * hd + 8
+    q = torch.full((3, qs), float("nan"), dtype=torch.bfloat16, device="cuda")
+    q[:, :n_q * hd] = dev(c.q).view(3, -1)
+    out = torch.full((3, os_), 7.0, dtype=torch.bfloat16, device="cuda")
+    s = torch.cuda.Stream()
+    gs = Gpu(0, stream=s)
+    pk, pv, kc, vc, ws = dev(c.pk), dev(c.pv), dev(c.kc), dev(c.vc), c.ws(g, 70)
+
+    def call():
+        gs.attention_decode_shared(q, qs, pk, pv, 500, c.rows, kc, vc, c.n_kv * c.max_seq * hd, c.ld, 70,
+                                   n_q, c.n_kv, hd, c.max_seq, out, os_, workspace=ws)
+    torch.cuda.synchronize()
+    call()
+    s.synchronize()
+    assert torch.equal(out[:, :n_q * hd], want) and bool((out[:, n_q * hd:] == 7.0).all())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        call()
+    for _ in range(2):
+        out.fill_(1.0)
+        ws.fill_(255)  # what an earlier call left in the workspace does not matter
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[:, :n_q * hd], want) and bool((out[:, n_q * hd:] == 1.0).all())
+    assert g.device_error() == 0
