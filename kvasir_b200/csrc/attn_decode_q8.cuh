@@ -1,0 +1,583 @@
+// attn_decode_q8.cuh -- split-KV GQA decode attention over an 8-bit KV cache, head_dim 64
+// or 128, up to 16 query heads per KV head.
+//
+// Work unit: one CTA per (key chunk, KV head, sequence); its four warps take interleaved
+// tiles of 64 keys (head_dim 128: 32), 4 KB of K codes and 4 KB of V codes, each warp
+// through a ring of its own.  The transposed products put the keys on the MMA's 16-row
+// side and the group's heads on its 8-column side, so a group of up to 8 heads wastes no
+// rows and takes half the instructions of a 16-row query tile:
+//   S^T = K Q^T    m16n8k16, A = K codes as f16 (ldmatrix; a lane's four bytes are four
+//                  neighbouring dims, so the K side of the product runs over the dims in
+//                  the order (4c, 4c+1 | 4c+2, 4c+3), and Q's fragments are loaded so)
+//   O^T += V^T P^T m16n8k16, A = V codes as f16 (ldmatrix.trans moves byte pairs: row g of
+//                  a tile is dim 2g and row g + 8 is dim 2g + 1), B = P through movmatrix
+// Codes are exact in f16: int8 through the bytes of 1024 + 128 + code, e4m3 by cvt.  The
+// K scale multiplies the f32 score of its key; the V scale multiplies the key's weight.
+//
+// Precision.  Q: f16 as it is; bf16 scaled by a power of two to a largest element in
+// [2^14, 2^15) and rounded to f16, which is exact for elements down to 2^-31 of the
+// largest.  Weights: w = p * v_scale * 2^n, n such that the largest V scale seen makes
+// w < 2^14, rounded once to f16 (half a step, 2^-11 of a weight; steps of 2^-24 below
+// 2^-14, so a key whose V scale is 2^28 times smaller than the largest keeps ten bits).
+// A remainder as in the 16-bit kernels would double the P V products; the codes
+// themselves are within 2^-8 of a row's largest value at best.  Scores, the running
+// maximum, the sums and O are f32.
+#pragma once
+
+#include "kv8.cuh"
+
+namespace kvb {
+
+constexpr int kQ8Warps = 4;
+constexpr int kQ8Stages = 2;
+constexpr int kQ8TileBytes = 4096;  // K codes (or V codes) of a tile
+constexpr int kQ8RingBytes = kQ8Warps * kQ8Stages * 2 * kQ8TileBytes;
+constexpr int kQ8ScaleBytes = kQ8Warps * kQ8Stages * 2 * 64 * 4;
+constexpr int kQ8SmemBytes = kQ8RingBytes + kQ8ScaleBytes + 1024;
+constexpr int kQ8MaxGroup = 16;
+
+__host__ __device__ constexpr int q8_tile_keys(int hd) { return kQ8TileBytes / hd; }
+
+struct Q8DecodeArgs {
+    const uint16_t* q;
+    long long q_row_stride;
+    const int32_t* lens;
+    int max_len, group;
+    float scale_log2;
+    uint16_t* out;
+    long long out_row_stride;
+    float* ws;       // split partials: per part O[group][hd], m[group], l[group]
+    int chunk_keys;  // keys per CTA, a multiple of kQ8Warps tiles
+    int max_chunks;
+    int fold;        // chunks of a (sequence, KV head) folded through a cluster
+    int piece;       // rows per tensor copy: a whole tile, or gcd(block_size, tile) paged
+    int total_rows;  // rows of the code arrays (a row past the end reads as zeros)
+    Kv8Place c;
+};
+
+__device__ __forceinline__ int q8_len(const int32_t* lens, int max_len, int b) {
+    int len = lens[b];
+    if (len < 0 || len > max_len) {
+        if (threadIdx.x == 0) raise_dev_error(kDevErrBadLength);
+        len = len < 0 ? 0 : max_len;
+    }
+    return len;
+}
+
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
+    return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t low16) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}"
+        : "=r"(r)
+        : "r"(low16));
+    return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2_hi_to_f16x2(uint32_t v) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}"
+        : "=r"(r)
+        : "r"(v));
+    return r;
+}
+// f16 pair of bytes u (codes + 128): 0x64uu is 1024 + u, less 1152 gives the code, exactly.
+__device__ __forceinline__ uint32_t biased_to_f16x2(uint32_t u, uint32_t sel) {
+    uint32_t r;
+    const uint32_t t = prmt(u, 0x64646464u, sel);
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(0x64806480u));
+    return r;
+}
+// Four codes -> f16 pairs (bytes 0, 1) and (2, 3).
+template <int kFmt>
+__device__ __forceinline__ void codes_pairs(uint32_t v, uint32_t& p01, uint32_t& p23) {
+    if (kFmt == KVB_KV_INT8) {
+        const uint32_t u = v ^ 0x80808080u;
+        p01 = biased_to_f16x2(u, 0x4140u);
+        p23 = biased_to_f16x2(u, 0x4342u);
+    } else {
+        p01 = e4m3x2_to_f16x2(v);
+        p23 = e4m3x2_hi_to_f16x2(v);
+    }
+}
+// Four codes -> f16 pairs (bytes 0, 2) and (1, 3).
+template <int kFmt>
+__device__ __forceinline__ void codes_evens_odds(uint32_t v, uint32_t& p02, uint32_t& p13) {
+    if (kFmt == KVB_KV_INT8) {
+        const uint32_t u = v ^ 0x80808080u;
+        p02 = biased_to_f16x2(u, 0x4240u);
+        p13 = biased_to_f16x2(u, 0x4341u);
+    } else {
+        const uint32_t u = prmt(v, 0u, 0x3120u);
+        p02 = e4m3x2_to_f16x2(u);
+        p13 = e4m3x2_hi_to_f16x2(u);
+    }
+}
+__device__ __forceinline__ uint32_t movmatrix_t(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// 4-byte asynchronous copy to shared memory; bytes == 0 writes zero and reads nothing.
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+                 : "memory");
+}
+// Arrives on the barrier once this thread's earlier cp.async copies have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+
+// Byte offset of 16-byte chunk `ch` of row r in a tile that the tensor copy wrote with a
+// 64-byte (head_dim 64) or 128-byte swizzle.
+template <int HD>
+__device__ __forceinline__ uint32_t q8_smem_off(int r, int ch) {
+    return HD == 64 ? (uint32_t)(r * 64 + ((ch ^ ((r >> 1) & 3)) << 4))
+                    : (uint32_t)(r * 128 + ((ch ^ (r & 7)) << 4));
+}
+
+// Grid (KV head, sequence, chunk slot), or with a.fold (chunk slot, KV head, sequence) in
+// clusters of max_chunks CTAs; slots count chunks from the end of the sequence, so full
+// chunks are dispatched first (as attn_decode.cuh).
+template <typename T, int kFmt, int HD, int NT>
+__global__ void __launch_bounds__(128, 3)
+    attn_decode_q8_kernel(const __grid_constant__ CUtensorMap kmap,
+                          const __grid_constant__ CUtensorMap vmap, Q8DecodeArgs a) {
+    constexpr int KT = q8_tile_keys(HD);  // keys per tile
+    constexpr int MT = KT / 16;           // 16-key MMA rows of S^T, k-steps of P V
+    constexpr int DT = HD / 16;           // 16-dim chunks: k-steps of K Q, MMA rows of O^T
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[kQ8Warps][kQ8Stages];
+    __shared__ float w_ml[kQ8Warps][2][kQ8MaxGroup];
+    __shared__ float fold_ml[2][kQ8MaxGroup];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                               ~uintptr_t(1023));
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, c = lane & 3;
+    const int slot = a.fold ? (int)blockIdx.x : (int)blockIdx.z;
+    const int kvh = a.fold ? (int)blockIdx.y : (int)blockIdx.x;
+    const int b = a.fold ? (int)blockIdx.z : (int)blockIdx.y;
+    const int G = a.group;
+    if (threadIdx.x < kQ8Warps * kQ8Stages)
+        mbar_init(&bars[0][0] + threadIdx.x, 1 + 32);  // one expect_tx, 32 scale arrivals
+    fence_mbar_init();
+    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    const int len = q8_len(a.lens, a.max_len, b);
+    const int n_chunks = (len + a.chunk_keys - 1) / a.chunk_keys;
+    const int from_end = a.max_chunks - 1 - slot;
+    T* outb = reinterpret_cast<T*>(a.out) + (size_t)b * a.out_row_stride + (size_t)kvh * G * HD;
+    if (len == 0) {  // no keys: a zero row (the whole cluster returns here)
+        if (from_end == 0)
+            for (int i = threadIdx.x; i < G * HD; i += blockDim.x) outb[i] = Elem<T>::from_f(0.f);
+        return;
+    }
+    const bool active = from_end < n_chunks;
+    float* wo = reinterpret_cast<float*>(smem + warp * kQ8Stages * 2 * kQ8TileBytes);  // [16][HD]
+    float* fold_o = reinterpret_cast<float*>(smem + 2 * kQ8TileBytes);  // warp 0's second stage
+    if (active) {
+        const int chunk = n_chunks - 1 - from_end;
+        const int key_begin = chunk * a.chunk_keys;
+        const int key_end = min(len, key_begin + a.chunk_keys);
+        uint8_t* ring = smem + warp * kQ8Stages * 2 * kQ8TileBytes;
+        float* scales = reinterpret_cast<float*>(smem + kQ8RingBytes) + warp * kQ8Stages * 128;
+        const int row_base = (int)(b * a.c.seq_rows + (long long)kvh * a.c.max_seq);
+        const int pshift = __ffs(a.piece) - 1;
+
+        // Paged: this lane's piece of the next tile to be requested, read a tile ahead.
+        auto block_of = [&](int kt0) -> int {
+            const int k = kt0 + (lane << pshift);
+            if (!a.c.block_table || lane >= (KT >> pshift) || k >= key_end) return 0;
+            return a.c.block_table[(size_t)b * a.c.max_blocks + k / a.c.block_size];
+        };
+        int kt_issue = key_begin + warp * KT;
+        int blk = block_of(kt_issue);
+        // Requests the warp's next tile into stage st: codes by tensor copies, scales by 4-byte
+        // copies (zero past the last key), all counted on the stage's barrier.
+        auto issue = [&](int st) {
+            const int kt0 = kt_issue;
+            if (kt0 >= key_end) return;
+            const int nk = min(KT, key_end - kt0);
+            const int n_pieces = a.c.block_table ? (nk + a.piece - 1) >> pshift : 1;
+            int row = a.total_rows;  // past the end: zeros
+            if (lane < n_pieces) {
+                if (!a.c.block_table) {
+                    row = row_base + kt0;
+                } else if (blk < 0 || blk >= a.c.n_blocks) {
+                    raise_dev_error(kDevErrBadPosition);
+                } else {
+                    row = (blk * a.c.n_kv + kvh) * a.c.block_size +
+                          (kt0 + (lane << pshift)) % a.c.block_size;
+                }
+            }
+            kt_issue += kQ8Warps * KT;
+            blk = block_of(kt_issue);
+            uint64_t* bar = &bars[warp][st];
+            uint8_t* kdst = ring + st * 2 * kQ8TileBytes;
+            if (lane == 0) mbar_expect_tx(bar, (uint32_t)(2 * n_pieces * a.piece * HD));
+            __syncwarp();
+            if (lane < n_pieces) {
+                const int off = (lane << pshift) * HD;
+                tma_load_2d(kdst + off, &kmap, bar, 0, row);
+                tma_load_2d(kdst + kQ8TileBytes + off, &vmap, bar, 0, row);
+            }
+            const uint32_t sdst = smem_u32(scales + st * 128);
+#pragma unroll
+            for (int u = 0; u < KT / 32; ++u) {
+                const int k = lane + 32 * u;
+                const int r0 = __shfl_sync(0xffffffffu, row, k >> pshift);
+                const bool ok = k < nk && r0 < a.total_rows;
+                const size_t r = ok ? (size_t)r0 + (k & (a.piece - 1)) : 0;
+                cp_async4(sdst + 4 * k, a.c.ks + r, ok ? 4 : 0);
+                cp_async4(sdst + 256 + 4 * k, a.c.vs + r, ok ? 4 : 0);
+            }
+            cp_async_arrive(bar);
+        };
+#pragma unroll
+        for (int s = 0; s < kQ8Stages; ++s) issue(s);
+
+        // Q fragments (B operand): column g = head 8 nt + g, dims 16 j + 4c .. + 3.
+        uint32_t qf[DT][NT][2];
+        float qs[NT][2];  // score factor of heads 8 nt + 2c, + 1
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int h = 8 * nt + g;
+            const T* qr = reinterpret_cast<const T*>(a.q) + (size_t)b * a.q_row_stride +
+                          (size_t)(kvh * G + min(h, G - 1)) * HD;
+            uint2 v[DT];
+#pragma unroll
+            for (int j = 0; j < DT; ++j)
+                v[j] = h < G ? *reinterpret_cast<const uint2*>(qr + 16 * j + 4 * c) : make_uint2(0u, 0u);
+            float f = a.scale_log2;
+            if (Elem<T>::kDtype == KVB_BF16) {
+                uint32_t mx = 0;  // largest exponent of the head's elements
+#pragma unroll
+                for (int j = 0; j < DT; ++j)
+                    mx = max(max(mx, max(v[j].x & 0x7fffu, (v[j].x >> 16) & 0x7fffu)),
+                             max(v[j].y & 0x7fffu, (v[j].y >> 16) & 0x7fffu));
+                mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                // biased exponent, kept where 2^(14 - e) and its inverse are normal numbers
+                const int e = min(max((int)(mx >> 7), 16), 254);
+                const float up = __uint_as_float((uint32_t)(268 - e) << 23);  // 2^(141 - e)
+                f *= __uint_as_float((uint32_t)(e - 14) << 23);               // 2^(e - 141)
+#pragma unroll
+                for (int j = 0; j < DT; ++j) {
+                    const float2 x = Elem<T>::unpack(v[j].x), y = Elem<T>::unpack(v[j].y);
+                    v[j].x = f16x2(x.x * up, x.y * up);
+                    v[j].y = f16x2(y.x * up, y.y * up);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < DT; ++j) {
+                qf[j][nt][0] = v[j].x;
+                qf[j][nt][1] = v[j].y;
+            }
+            qs[nt][0] = __shfl_sync(0xffffffffu, f, 8 * c);
+            qs[nt][1] = __shfl_sync(0xffffffffu, f, 8 * c + 4);
+        }
+
+        float o[DT][NT][4];
+        float m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+            for (int j = 0; j < DT; ++j) o[j][nt][0] = o[j][nt][1] = o[j][nt][2] = o[j][nt][3] = 0.f;
+        }
+        int ev = 14;  // biased exponent of the largest V scale seen; O is in units of 2^(ev - 140)
+        bool ok = true;
+        int it = 0;
+        for (int kt0 = key_begin + warp * KT; kt0 < key_end; kt0 += kQ8Warps * KT, ++it) {
+            const int st = it % kQ8Stages;
+            const int nk = min(KT, key_end - kt0);
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][st], (it / kQ8Stages) & 1));
+            if (!ok) break;
+            const uint32_t kb = smem_u32(ring + st * 2 * kQ8TileBytes), vb = kb + kQ8TileBytes;
+            const float* ks = scales + st * 128;
+            const float* vs = ks + 64;
+
+            // ---- S^T = K Q^T
+            float s[MT][NT][4];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) s[t][nt][0] = s[t][nt][1] = s[t][nt][2] = s[t][nt][3] = 0.f;
+                const int r = 16 * t + (lane & 15);
+#pragma unroll
+                for (int j = 0; j < DT; j += 2) {
+                    uint32_t w0, w1, w2, w3, af[4];
+                    ldsm_x4(kb + q8_smem_off<HD>(r, j + (lane >> 4)), w0, w1, w2, w3);
+                    codes_pairs<kFmt>(w0, af[0], af[2]);
+                    codes_pairs<kFmt>(w1, af[1], af[3]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        mma_16816<__half>(s[t][nt], af, qf[j][nt][0], qf[j][nt][1]);
+                    codes_pairs<kFmt>(w2, af[0], af[2]);
+                    codes_pairs<kFmt>(w3, af[1], af[3]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        mma_16816<__half>(s[t][nt], af, qf[j + 1][nt][0], qf[j + 1][nt][1]);
+                }
+            }
+            // ---- scale and mask; element e: key 16 t + g + 8 (e >> 1), head 8 nt + 2c + (e & 1)
+            float mx[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const float k0 = ks[16 * t + g], k1 = ks[16 * t + g + 8];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[t][nt][e] *= (e < 2 ? k0 : k1) * qs[nt][e & 1];
+            }
+            if (nk < KT) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (16 * t + g + 8 * (e >> 1) >= nk) s[t][nt][e] = -INFINITY;
+                if (kFmt == KVB_KV_E4M3) {  // V codes past the last key may be NaN: 0 * NaN
+                    const uint32_t z = 0;
+                    for (int i = nk * HD / 16 + lane; i < KT * HD / 16; i += 32)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vb + 16 * i), "r"(z)
+                                     : "memory");
+                    __syncwarp();
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    mx[nt][0] = fmaxf(mx[nt][0], fmaxf(s[t][nt][0], s[t][nt][2]));
+                    mx[nt][1] = fmaxf(mx[nt][1], fmaxf(s[t][nt][1], s[t][nt][3]));
+                }
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) {
+                    mx[nt][0] = fmaxf(mx[nt][0], __shfl_xor_sync(0xffffffffu, mx[nt][0], x));
+                    mx[nt][1] = fmaxf(mx[nt][1], __shfl_xor_sync(0xffffffffu, mx[nt][1], x));
+                }
+            }
+            // ---- V scale exponent: rescale O where a larger one appears
+            uint32_t vmax = __float_as_uint(vs[lane]) & 0x7fffffffu;
+            if (KT == 64) vmax = max(vmax, __float_as_uint(vs[lane + 32]) & 0x7fffffffu);
+            const int en = max(ev, (int)(__reduce_max_sync(0xffffffffu, vmax) >> 23));
+            const float vf = __uint_as_float((uint32_t)(267 - en) << 23);  // 2^(140 - en)
+            const int down = 127 + ev - en;  // exponent field of 2^(ev - en)
+            const float rv = down > 0 ? __uint_as_float((uint32_t)down << 23) : 0.f;
+            ev = en;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float mn = fmaxf(m[nt][e], mx[nt][e]);
+                    const float ref = mn == -INFINITY ? 0.f : mn;
+                    const float al = ex2_approx(m[nt][e] - ref);
+                    m[nt][e] = mn;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        s[t][nt][e] = ex2_approx(s[t][nt][e] - ref);
+                        s[t][nt][e + 2] = ex2_approx(s[t][nt][e + 2] - ref);
+                        sum += s[t][nt][e] + s[t][nt][e + 2];
+                    }
+                    l[nt][e] = l[nt][e] * al + sum;  // this lane's keys; summed over lanes at the end
+                    const float ao = al * rv;
+#pragma unroll
+                    for (int j = 0; j < DT; ++j) {
+                        o[j][nt][e] *= ao;
+                        o[j][nt][e + 2] *= ao;
+                    }
+                }
+            // ---- O^T += V^T P^T
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const float v0 = vs[16 * t + g] * vf, v1 = vs[16 * t + g + 8] * vf;
+                uint32_t pf[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    pf[nt][0] = movmatrix_t(f16x2(s[t][nt][0] * v0, s[t][nt][1] * v0));
+                    pf[nt][1] = movmatrix_t(f16x2(s[t][nt][2] * v1, s[t][nt][3] * v1));
+                }
+                const int r = 16 * t + (lane & 15);
+#pragma unroll
+                for (int j = 0; j < DT; j += 2) {
+                    uint32_t w0, w1, w2, w3, af[4];
+                    ldsm_x4_t(vb + q8_smem_off<HD>(r, j + (lane >> 4)), w0, w1, w2, w3);
+                    codes_evens_odds<kFmt>(w0, af[0], af[1]);
+                    codes_evens_odds<kFmt>(w1, af[2], af[3]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_16816<__half>(o[j][nt], af, pf[nt][0], pf[nt][1]);
+                    codes_evens_odds<kFmt>(w2, af[0], af[1]);
+                    codes_evens_odds<kFmt>(w3, af[2], af[3]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        mma_16816<__half>(o[j + 1][nt], af, pf[nt][0], pf[nt][1]);
+                }
+            }
+            __syncwarp();
+            fence_async_smem();  // these reads precede the next copies into the stage
+            issue(st);
+        }
+        if (!ok) {
+            // A copy did not complete in time (the error word is set): wait once more, bounded,
+            // for every stage still outstanding, and contribute an empty state.
+            for (int i = it; i < it + kQ8Stages; ++i)
+                if (key_begin + (warp + i * kQ8Warps) * KT < key_end)
+                    mbar_wait(&bars[warp][i % kQ8Stages], (i / kQ8Stages) & 1);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                m[nt][0] = m[nt][1] = -INFINITY;
+                l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+                for (int j = 0; j < DT; ++j) o[j][nt][0] = o[j][nt][1] = o[j][nt][2] = o[j][nt][3] = 0.f;
+            }
+            __syncwarp();
+        }
+        // ---- merge the four warps' states through shared memory
+        const float unit = __uint_as_float((uint32_t)(ev - 13) << 23);  // 2^(ev - 140)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
+                const int h = 8 * nt + 2 * c + e;
+                if (g == 0) {
+                    w_ml[warp][0][h] = m[nt][e];
+                    w_ml[warp][1][h] = l[nt][e];
+                }
+#pragma unroll
+                for (int j = 0; j < DT; ++j)
+                    *reinterpret_cast<float2*>(wo + h * HD + 16 * j + 2 * g) =
+                        make_float2(o[j][nt][e] * unit, o[j][nt][e + 2] * unit);
+            }
+        }
+        __syncthreads();
+        float* wsb = nullptr;
+        float* mlb = nullptr;
+        if (n_chunks > 1) {
+            wsb = a.fold ? fold_o
+                         : a.ws + (((size_t)b * a.c.n_kv + kvh) * a.max_chunks + chunk) *
+                                      (size_t)(G * (HD + 2));
+            mlb = a.fold ? &fold_ml[0][0] : wsb + G * HD;
+        }
+        const int ml_step = a.fold ? kQ8MaxGroup : G;
+        for (int i = threadIdx.x; i < G * HD; i += blockDim.x) {
+            const int r = i / HD;
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kQ8Warps; ++w) M = fmaxf(M, w_ml[w][0][r]);
+            float L = 0.f, O = 0.f;
+#pragma unroll
+            for (int w = 0; w < kQ8Warps; ++w) {
+                const float mw = w_ml[w][0][r];
+                const float f = mw == -INFINITY ? 0.f : exp2f(mw - M);
+                // a warp whose scores were all NaN keeps -inf as its maximum and a NaN sum
+                const float lw = w_ml[w][1][r];
+                L += lw != lw ? lw : lw * f;
+                O += reinterpret_cast<const float*>(smem + w * kQ8Stages * 2 * kQ8TileBytes)[i] * f;
+            }
+            if (n_chunks == 1) {
+                outb[i] = Elem<T>::from_f(O / L);
+            } else {
+                wsb[i] = O;
+                if (i % HD == 0) {
+                    mlb[r] = M;
+                    mlb[ml_step + r] = L;
+                }
+            }
+        }
+    }
+    if (!a.fold) return;
+    cluster_sync();  // every chunk's state is in its CTA's shared memory
+    if (n_chunks > 1 && slot == a.max_chunks - 1) {
+        const uint32_t r0 = (uint32_t)(a.max_chunks - n_chunks);
+        for (int i = threadIdx.x; i < G * HD; i += blockDim.x) {
+            const int r = i / HD;
+            float M = -INFINITY;
+            for (int k = 0; k < n_chunks; ++k) M = fmaxf(M, dsmem_ld(&fold_ml[0][r], r0 + k));
+            float L = 0.f, O = 0.f;
+            for (int k = 0; k < n_chunks; ++k) {
+                const float mk = dsmem_ld(&fold_ml[0][r], r0 + k), lk = dsmem_ld(&fold_ml[1][r], r0 + k);
+                const float f = mk == -INFINITY ? 0.f : exp2f(mk - M);
+                L += lk != lk ? lk : lk * f;
+                O += dsmem_ld(fold_o + i, r0 + k) * f;
+            }
+            outb[i] = Elem<T>::from_f(O / L);
+        }
+    }
+    cluster_sync();  // no CTA leaves while its state may still be read
+}
+
+// Joins the partial states of every (sequence, KV head): parts 0 .. fixed - 1, which every
+// sequence has, then one for each chunk of its keys past key0.  Written rows: those with more
+// than one part (write_all: every row, zeros where a sequence has none).  A programmatic
+// dependent of the kernel that writes the partials.  The CTA first turns the parts' (m, l)
+// into weights in shared memory, then each thread sums its outputs over the parts with
+// coalesced loads: two rounds of memory latency.
+struct JoinArgs {
+    const float* ws;
+    const int32_t* lens;
+    int max_len, key0, chunk_keys;
+    int fixed, max_parts;
+    int n_kv, group, hd;
+    int write_all;
+    uint16_t* out;
+    long long out_row_stride;
+};
+constexpr int kJoinThreads = 256;
+constexpr int kJoinMaxParts = 512;  // weights: parts x group floats of shared memory
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(JoinArgs a) {
+    extern __shared__ float w[];  // [parts][group]
+    __shared__ float inv_l[kQ8MaxGroup];
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int kvh = blockIdx.x, b = blockIdx.y, G = a.group, hd = a.hd;
+    const int len = q8_len(a.lens, a.max_len, b);
+    const int own = len > a.key0 ? (len - a.key0 + a.chunk_keys - 1) / a.chunk_keys : 0;
+    const int parts = a.fixed + own;
+    if (!a.write_all && parts <= 1) return;
+    T* outb = reinterpret_cast<T*>(a.out) + (size_t)b * a.out_row_stride + (size_t)kvh * G * hd;
+    const size_t per = (size_t)G * (hd + 2);
+    const float* base = a.ws + ((size_t)b * a.n_kv + kvh) * a.max_parts * per;
+    for (int r = threadIdx.x >> 5; r < G; r += kJoinThreads / 32) {  // a warp per head
+        const int lane = threadIdx.x & 31;
+        float M = -INFINITY, L = 0.f;
+        for (int p = lane; p < parts; p += 32) M = fmaxf(M, base[p * per + G * hd + r]);
+        M = warp_max(M);
+        for (int p = lane; p < parts; p += 32) {
+            const float mp = base[p * per + G * hd + r], lp = base[p * per + G * hd + G + r];
+            const float f = mp == -INFINITY ? 0.f : exp2f(mp - M);
+            w[p * G + r] = f;
+            L += lp != lp ? lp : lp * f;
+        }
+        L = warp_sum(L);
+        if (lane == 0) inv_l[r] = L == 0.f ? 0.f : 1.f / L;  // no keys at all: zeros
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < G * hd; i += kJoinThreads) {
+        const int r = i / hd;
+        float O = 0.f;
+#pragma unroll 8
+        for (int p = 0; p < parts; ++p) O += base[p * per + i] * w[p * G + r];
+        outb[i] = Elem<T>::from_f(O * inv_l[r]);
+    }
+}
+
+}  // namespace kvb

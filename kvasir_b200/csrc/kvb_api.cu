@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "attn_decode.cuh"
+#include "attn_decode_q8.cuh"
 #include "attn_general_src.cuh"
 #include "attn_generic.cuh"
 #include "attn_prefill.cuh"

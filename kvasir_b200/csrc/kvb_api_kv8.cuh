@@ -183,15 +183,156 @@ static int decode_args(const char* name, GeneralDecodeArgs& a, const void* q, si
     return KVB_OK;
 }
 
+// 2-D tensor map of `rows` rows of row_bytes 8-bit elements, copied box_rows at a time;
+// swizzled over the row (64 or 128 bytes).
+static int encode_tmap_rows8(CUtensorMap* map, const void* base, size_t row_bytes, size_t rows,
+                             int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(KVB_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[2] = {row_bytes, rows}, strides[1] = {row_bytes};
+    const cuuint32_t box[2] = {(cuuint32_t)row_bytes, (cuuint32_t)box_rows}, step[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
+                          strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(KVB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return KVB_OK;
+}
+
+static bool q8_tensor_shape(size_t head_dim, size_t n_q, size_t n_kv) {
+    return (head_dim == 64 || head_dim == 128) && n_kv > 0 && n_q % n_kv == 0 &&
+           n_q / n_kv <= (size_t)kQ8MaxGroup;
+}
+
+// Keys per CTA of a split call: as decode_chunk_keys (about five waves of three CTAs per SM
+// over the worst case; one tile per warp at least, four once the (sequence, KV head) pairs
+// alone fill the SMs), and at most kJoinMaxParts chunks.
+static int q8_chunk_keys(size_t n_seq, size_t n_kv, size_t max_len, size_t head_dim) {
+    const size_t kt = (size_t)q8_tile_keys((int)head_dim);
+    const size_t tiles = (max_len + kt - 1) / kt;
+    const size_t target = (size_t)num_sms() * 3 * 5;
+    size_t per_cta = (n_seq * n_kv * tiles + target - 1) / target;
+    const size_t min_tiles = kQ8Warps * (n_seq * n_kv >= (size_t)num_sms() ? 4 : 1);
+    if (per_cta < min_tiles) per_cta = min_tiles;
+    if (per_cta * kJoinMaxParts < tiles) per_cta = (tiles + kJoinMaxParts - 1) / kJoinMaxParts;
+    if (per_cta > tiles) per_cta = tiles;
+    if (per_cta < 1) per_cta = 1;
+    return (int)((per_cta + kQ8Warps - 1) / kQ8Warps * kQ8Warps * kt);
+}
+
+static size_t q8_ws_bytes(size_t n_seq, size_t max_len, size_t n_q, size_t n_kv, size_t head_dim) {
+    if (!q8_tensor_shape(head_dim, n_q, n_kv) || max_len == 0) return 0;
+    const size_t ck = (size_t)q8_chunk_keys(n_seq, n_kv, max_len, head_dim);
+    const size_t chunks = (max_len + ck - 1) / ck;
+    return chunks <= 1 ? 0 : n_seq * chunks * n_q * (head_dim + 2) * sizeof(float);
+}
+
+static int launch_join(kvb_stream_t stream, const JoinArgs& a, size_t n_seq, int dtype) {
+    const dim3 grid((unsigned)a.n_kv, (unsigned)n_seq);
+    const size_t smem = (size_t)a.max_parts * a.group * sizeof(float);
+    const cudaError_t e =
+        dtype == KVB_BF16
+            ? launch_pdl(attn_join_kernel<__nv_bfloat16>, grid, dim3(kJoinThreads), smem, stream, a)
+            : launch_pdl(attn_join_kernel<__half>, grid, dim3(kJoinThreads), smem, stream, a);
+    if (e != cudaSuccess) return cuda_fail(e, "attention join launch");
+    return KVB_OK;
+}
+
+template <typename T, int kFmt, int HD, int NT>
+static int launch_q8_tensor(kvb_stream_t stream, Q8DecodeArgs& a, size_t n_seq, size_t cache_rows,
+                            void* ws, size_t ws_len) {
+    constexpr int KT = q8_tile_keys(HD);
+    a.piece = KT;
+    if (a.c.block_table)
+        while (a.c.block_size % a.piece) a.piece /= 2;
+    a.total_rows = (int)cache_rows;
+    CUtensorMap kmap, vmap;
+    int st = encode_tmap_rows8(&kmap, a.c.kc, HD, cache_rows, a.piece);
+    if (st) return st;
+    st = encode_tmap_rows8(&vmap, a.c.vc, HD, cache_rows, a.piece);
+    if (st) return st;
+    const size_t n_kv = (size_t)a.c.n_kv, max_len = (size_t)a.max_len;
+    const size_t need = q8_ws_bytes(n_seq, max_len, n_kv * a.group, n_kv, HD);
+    const bool split = need > 0 && ws != nullptr && ws_len >= need && aligned(ws, 16);
+    a.chunk_keys = q8_chunk_keys(n_seq, n_kv, max_len, HD);
+    if (!split) a.chunk_keys = (int)((max_len + kQ8Warps * KT - 1) / (kQ8Warps * KT) * (kQ8Warps * KT));
+    if (a.chunk_keys == 0) a.chunk_keys = kQ8Warps * KT;
+    a.max_chunks = (int)((max_len + a.chunk_keys - 1) / a.chunk_keys);
+    if (a.max_chunks < 1) a.max_chunks = 1;
+    a.ws = split ? static_cast<float*>(ws) : nullptr;
+    // Small split grids fold their chunks through a cluster, as kvb_attention_decode does.
+    a.fold = a.max_chunks >= 2 && a.max_chunks <= 8 &&
+             n_kv * n_seq * a.max_chunks <= (size_t)num_sms() * 3;
+    auto* kernel = attn_decode_q8_kernel<T, kFmt, HD, NT>;
+    set_max_smem(kernel, kQ8SmemBytes);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = a.fold ? dim3((unsigned)a.max_chunks, (unsigned)n_kv, (unsigned)n_seq)
+                         : dim3((unsigned)n_kv, (unsigned)n_seq, (unsigned)a.max_chunks);
+    cfg.blockDim = dim3(kQ8Warps * 32);
+    cfg.dynamicSmemBytes = kQ8SmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)a.max_chunks;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.fold ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, kmap, vmap, a);
+    if (e != cudaSuccess) return cuda_fail(e, "attention_decode_q8 launch");
+    if (a.fold || a.max_chunks == 1) return KVB_OK;
+    JoinArgs j;
+    j.ws = a.ws;
+    j.lens = a.lens;
+    j.max_len = a.max_len;
+    j.key0 = 0;
+    j.chunk_keys = a.chunk_keys;
+    j.fixed = 0;
+    j.max_parts = a.max_chunks;
+    j.n_kv = a.c.n_kv;
+    j.group = a.group;
+    j.hd = HD;
+    j.write_all = 0;
+    j.out = a.out;
+    j.out_row_stride = a.out_row_stride;
+    return launch_join(stream, j, n_seq, Elem<T>::kDtype);
+}
+
+// The tensor-core kernel where shape and alignment allow it (cache_rows: rows of the code
+// arrays), else the general one.
 template <typename T, int kFmt>
 static int launch_q8_decode(kvb_stream_t stream, const GeneralDecodeArgs& a, const Kv8Place& c,
-                            size_t n_seq, void* ws, size_t ws_len) {
-    Q8Source<T, kFmt> src;
-    src.c = c;
-    const dim3 grid((unsigned)n_seq, (unsigned)((a.n_q + 3) / 4));
-    attn_general_src_kernel<T, Q8Source<T, kFmt>><<<grid, 128, 0, stream>>>(a, src);
-    KVB_CHECK_LAUNCH("attention_decode_q8 launch");
-    return KVB_OK;
+                            size_t cache_rows, size_t n_seq, void* ws, size_t ws_len) {
+    const bool tensor = q8_tensor_shape((size_t)a.hd, (size_t)a.n_q, (size_t)a.n_kv) &&
+                        (!c.block_table || c.block_size % 16 == 0) && a.q_row_stride % 4 == 0 &&
+                        aligned(a.q, 8) && aligned(c.kc, 16) && aligned(c.vc, 16) &&
+                        aligned(c.ks, 4) && aligned(c.vs, 4) && n_seq <= 65535 &&
+                        a.n_kv <= 65535 && fits_i32(cache_rows + 64);
+    if (!tensor) {
+        Q8Source<T, kFmt> src;
+        src.c = c;
+        const dim3 grid((unsigned)n_seq, (unsigned)((a.n_q + 3) / 4));
+        attn_general_src_kernel<T, Q8Source<T, kFmt>><<<grid, 128, 0, stream>>>(a, src);
+        KVB_CHECK_LAUNCH("attention_decode_q8 launch");
+        return KVB_OK;
+    }
+    Q8DecodeArgs d;
+    d.q = a.q;
+    d.q_row_stride = a.q_row_stride;
+    d.lens = a.lens;
+    d.max_len = a.max_len;
+    d.group = a.n_q / a.n_kv;
+    d.scale_log2 = a.scale_log2;
+    d.out = a.out;
+    d.out_row_stride = a.out_row_stride;
+    d.c = c;
+    if (a.hd == 64)
+        return d.group <= 8 ? launch_q8_tensor<T, kFmt, 64, 1>(stream, d, n_seq, cache_rows, ws, ws_len)
+                            : launch_q8_tensor<T, kFmt, 64, 2>(stream, d, n_seq, cache_rows, ws, ws_len);
+    return d.group <= 8 ? launch_q8_tensor<T, kFmt, 128, 1>(stream, d, n_seq, cache_rows, ws, ws_len)
+                        : launch_q8_tensor<T, kFmt, 128, 2>(stream, d, n_seq, cache_rows, ws, ws_len);
 }
 
 template <typename T>
@@ -274,8 +415,7 @@ int kvb_kv_read_q8_paged(kvb_stream_t stream, const void* k_pool, const void* v_
 
 size_t kvb_attention_decode_q8_workspace_bytes(size_t n_seq, size_t max_len, size_t n_q,
                                                size_t n_kv, size_t head_dim) {
-    (void)n_seq, (void)max_len, (void)n_q, (void)n_kv, (void)head_dim;
-    return 0;
+    return q8_ws_bytes(n_seq, max_len, n_q, n_kv, head_dim);
 }
 
 int kvb_attention_decode_q8(kvb_stream_t stream, const void* q, size_t q_row_stride, const void* kc,
@@ -297,8 +437,9 @@ int kvb_attention_decode_q8(kvb_stream_t stream, const void* q, size_t q_row_str
                               scale_len, n_seq, n_kv, head_dim, max_seq);
     if (st) return st;
     if (n_seq == 0) return KVB_OK;
-    return KVB_KV8_DISPATCH(launch_q8_decode, dtype, kv_format, stream, a, c, n_seq, workspace,
-                            workspace_len);
+    const size_t cache_rows = scale_len;
+    return KVB_KV8_DISPATCH(launch_q8_decode, dtype, kv_format, stream, a, c, cache_rows, n_seq,
+                            workspace, workspace_len);
 }
 
 int kvb_attention_decode_q8_paged(kvb_stream_t stream, const void* q, size_t q_row_stride,
@@ -324,8 +465,9 @@ int kvb_attention_decode_q8_paged(kvb_stream_t stream, const void* q, size_t q_r
               "attention_decode_q8_paged: max_len %zu exceeds %zu blocks of %zu", max_len,
               max_blocks, block_size);
     if (n_seq == 0) return KVB_OK;
-    return KVB_KV8_DISPATCH(launch_q8_decode, dtype, kv_format, stream, a, c, n_seq, workspace,
-                            workspace_len);
+    const size_t cache_rows = scale_len;
+    return KVB_KV8_DISPATCH(launch_q8_decode, dtype, kv_format, stream, a, c, cache_rows, n_seq,
+                            workspace, workspace_len);
 }
 
 size_t kvb_attention_decode_shared_workspace_bytes(size_t n_seq, size_t shared_len, size_t max_own,
