@@ -67,6 +67,9 @@ struct DecodeArgs {
     // be running writes them: the decode-step driver's launches).  The first K/V tiles
     // are then requested before griddepcontrol.wait; otherwise nothing is read before it.
     int kv_ready;
+    // Partial form (kPart, kvb_attention_decode_shared): keys [key0, lens[b]), key0 a multiple
+    // of 64; every chunk's state goes to the workspace as part part0 + chunk of max_parts.
+    int key0 = 0, part0 = 0, max_parts = 0;
 };
 
 // First row (of 64 elements) of the 64-key tile starting at key kt0 (a multiple of
@@ -101,7 +104,7 @@ __device__ __forceinline__ int decode_len(const DecodeArgs& a, int b) {
 // the sequence) of kv head kvh of sequence b.  Called by every thread of the CTA.
 // Its result goes to the output row (a one-chunk sequence), to `fold` (this CTA's
 // shared memory, for the cluster fold) or to the workspace.
-template <typename T, bool kRope>
+template <typename T, bool kRope, bool kPart>
 __device__ __forceinline__ void decode_chunk(const CUtensorMap& kmap, const CUtensorMap& vmap,
                                              const DecodeArgs& a, uint8_t* smem, uint64_t* bars,
                                              int kvh, int b, int from_end, float* fold) {
@@ -110,8 +113,10 @@ __device__ __forceinline__ void decode_chunk(const CUtensorMap& kmap, const CUte
     const int G = a.group;
 
     const int len = decode_len(a, b);
-    const int n_chunks = (len + a.chunk_keys - 1) / a.chunk_keys;
+    const int key0 = kPart ? a.key0 : 0;
+    const int n_chunks = (len - key0 + a.chunk_keys - 1) / a.chunk_keys;
     T* outb = reinterpret_cast<T*>(a.out) + (size_t)b * a.out_row_stride + (size_t)kvh * G * 64;
+    if (kPart && len <= key0) return;  // no own keys: no part
     if (len == 0) {  // no keys: defined as a zero output row
         if (a.kv_ready) asm volatile("griddepcontrol.wait;" ::: "memory");
         if (from_end == 0)
@@ -120,7 +125,7 @@ __device__ __forceinline__ void decode_chunk(const CUtensorMap& kmap, const CUte
     }
     if (from_end >= n_chunks) return;
     const int chunk = n_chunks - 1 - from_end;
-    const int key_begin = chunk * a.chunk_keys;
+    const int key_begin = key0 + chunk * a.chunk_keys;
     const int key_end = min(len, key_begin + a.chunk_keys);
 
     int rope_p = -1;  // fused RoPE: the new token's position (-1: none, or out of range)
@@ -404,7 +409,9 @@ __device__ __forceinline__ void decode_chunk(const CUtensorMap& kmap, const CUte
     }
     __syncthreads();
     float* wsb = nullptr;
-    if (n_chunks > 1)
+    if (kPart)
+        wsb = a.ws + (((size_t)b * a.n_kv + kvh) * a.max_parts + a.part0 + chunk) * (size_t)G * 66;
+    else if (n_chunks > 1)
         wsb = fold ? fold : a.ws + (((size_t)b * a.n_kv + kvh) * a.max_chunks + chunk) * (size_t)G * 66;
     for (int i = threadIdx.x; i < G * 64; i += blockDim.x) {
         const int r = i >> 6, d = i & 63;
@@ -421,7 +428,7 @@ __device__ __forceinline__ void decode_chunk(const CUtensorMap& kmap, const CUte
             L += base[16 * 64 + 16 + r] * f;
             O += base[r * 64 + d] * f;
         }
-        if (n_chunks == 1) {
+        if (!kPart && n_chunks == 1) {
             outb[i] = Elem<T>::from_f(L > 0.f ? O / L : 0.f);
         } else {
             wsb[i] = O;
@@ -450,7 +457,10 @@ __device__ __forceinline__ void decode_chunk(const CUtensorMap& kmap, const CUte
 // place of the workspace and the combine pass.  For small grids, where every
 // cluster is resident at once.  Every CTA of a cluster with keys passes both
 // cluster barriers; a cluster of an empty sequence passes none.
-template <typename T, bool kRope>
+// kPart: launched as a programmatic dependent of the prefix's kernel, from which it reads
+// nothing (everything before that kernel has completed when it starts); it waits for it
+// only before it ends, so that the join pass after this grid finds both kernels' parts.
+template <typename T, bool kRope, bool kPart = false>
 __global__ void __launch_bounds__(128, 3) attn_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                                                              const __grid_constant__ CUtensorMap vmap,
                                                              DecodeArgs a) {
@@ -459,13 +469,18 @@ __global__ void __launch_bounds__(128, 3) attn_decode_kernel(const __grid_consta
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~uintptr_t(1023));
     asm volatile("griddepcontrol.launch_dependents;");
-    if (!a.kv_ready) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!kPart && !a.kv_ready) asm volatile("griddepcontrol.wait;" ::: "memory");
     const int slot = a.fold ? (int)blockIdx.x : (int)blockIdx.z;
     const int kvh = a.fold ? (int)blockIdx.y : (int)blockIdx.x;
     const int b = a.fold ? (int)blockIdx.z : (int)blockIdx.y;
     const int from_end = a.max_chunks - 1 - slot;
     float* st = reinterpret_cast<float*>(smem + kDecWarps * 2 * kDecTileBytes);  // [G][66]
-    decode_chunk<T, kRope>(kmap, vmap, a, smem, bars, kvh, b, from_end, a.fold ? st : nullptr);
+    decode_chunk<T, kRope, kPart>(kmap, vmap, a, smem, bars, kvh, b, from_end,
+                                  !kPart && a.fold ? st : nullptr);
+    if (kPart) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
     if (!a.fold) return;
     const int G = a.group;
     const int len = decode_len(a, b);

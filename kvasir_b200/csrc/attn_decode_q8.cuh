@@ -575,7 +575,11 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(JoinArgs a) {
         const int r = i / hd;
         float O = 0.f;
 #pragma unroll 8
-        for (int p = 0; p < parts; ++p) O += base[p * per + i] * w[p * G + r];
+        for (int p = 0; p < parts; ++p) {
+            // a part without weight may hold anything (0 * NaN where every key was masked)
+            const float wp = w[p * G + r], op = base[p * per + i];
+            O += wp == 0.f ? 0.f : op * wp;
+        }
         outb[i] = Elem<T>::from_f(O * inv_l[r]);
     }
 }

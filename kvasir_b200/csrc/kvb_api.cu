@@ -17,6 +17,7 @@
 #include "attn_general_src.cuh"
 #include "attn_generic.cuh"
 #include "attn_prefill.cuh"
+#include "attn_shared.cuh"
 #include "elementwise.cuh"
 #include "kv8.cuh"
 #include "kvb_host.h"

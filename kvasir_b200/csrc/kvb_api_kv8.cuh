@@ -335,9 +335,173 @@ static int launch_q8_decode(kvb_stream_t stream, const GeneralDecodeArgs& a, con
                         : launch_q8_tensor<T, kFmt, 128, 2>(stream, d, n_seq, cache_rows, ws, ws_len);
 }
 
+// How a shared-prefix call runs on the tensor-core kernels: the prefix's 96-key tiles dealt to
+// `splits` slices, the own keys in chunks.  Slices: the number that takes the least time by
+// waves of two CTAs per SM x (tiles of the longest slice + ~4 tiles of start and end).
+struct SharedPlan {
+    int key0;  // keys computed for all sequences at once
+    int seqs_per_tile, row_tiles, n_tiles, splits;
+    int chunk_keys, max_chunks;
+    size_t ws_bytes;
+};
+static SharedPlan shared_plan(size_t n_seq, size_t prefix, size_t max_own, size_t n_q, size_t n_kv) {
+    SharedPlan p;
+    const size_t group = n_q / n_kv;
+    p.key0 = (int)prefix;
+    p.seqs_per_tile = (int)(kPfRows / group);
+    p.row_tiles = (int)((n_seq + p.seqs_per_tile - 1) / p.seqs_per_tile);
+    p.n_tiles = (int)((prefix + kPfKeys - 1) / kPfKeys);
+    p.splits = 0;
+    const size_t slots = (size_t)num_sms() * kPfCtasPerSm, pairs = (size_t)p.row_tiles * n_kv;
+    size_t best = ~(size_t)0;
+    for (int s = 1; s <= p.n_tiles && s <= 64; ++s) {
+        const size_t cost = ((pairs * s + slots - 1) / slots) * ((size_t)(p.n_tiles + s - 1) / s + 4);
+        if (cost < best) {
+            best = cost;
+            p.splits = s;
+        }
+    }
+    size_t ck = max_own ? (size_t)decode_chunk_keys(n_seq, n_kv, max_own) : 256;
+    const size_t most = kJoinMaxParts - 64;
+    if ((max_own + ck - 1) / ck > most) ck = ((max_own + most - 1) / most + 255) / 256 * 256;
+    p.chunk_keys = (int)ck;
+    p.max_chunks = (int)((max_own + ck - 1) / ck);
+    p.ws_bytes = n_seq * n_q * (size_t)(p.splits + p.max_chunks) * 66 * sizeof(float);
+    return p;
+}
+
+template <typename T>
+static int launch_shared_tensor(kvb_stream_t stream, const GeneralDecodeArgs& a,
+                                const SharedSource<T>& src, const SharedPlan& p, size_t n_seq,
+                                size_t own_rows, float* ws) {
+    const int group = a.n_q / a.n_kv, max_parts = p.splits + p.max_chunks;
+    const bool paged = src.block_table != nullptr;
+    const int dtype = Elem<T>::kDtype;
+    const size_t total_rows =
+        paged ? (size_t)src.n_blocks * src.n_kv * src.block_size : own_rows;
+    if (p.splits > 0) {
+        CUtensorMap qmap, kmap, vmap;
+        {
+            const uint64_t dims[3] = {64, (uint64_t)a.n_q, n_seq};
+            const uint64_t strides[2] = {128, (uint64_t)a.q_row_stride * 2};
+            const uint32_t box[3] = {64, (uint32_t)group, (uint32_t)p.seqs_per_tile};
+            const int st = encode_tmap(&qmap, a.q, 3, dims, strides, box, dtype);
+            if (st) return st;
+        }
+        int st;
+        if (paged) {
+            const uint64_t dims[2] = {64, total_rows}, strides[1] = {128};
+            const uint32_t box[2] = {64, (uint32_t)kPfPagedPiece};
+            st = encode_tmap(&kmap, src.kc, 2, dims, strides, box, dtype);
+            if (!st) st = encode_tmap(&vmap, src.vc, 2, dims, strides, box, dtype);
+        } else {
+            const uint64_t dims[3] = {64, (uint64_t)p.key0, (uint64_t)a.n_kv};
+            const uint64_t strides[2] = {128, (uint64_t)src.prefix_rows * 128};
+            const uint32_t box[3] = {64, (uint32_t)kPfKeys, 1};
+            st = encode_tmap(&kmap, src.pk, 3, dims, strides, box, dtype);
+            if (!st) st = encode_tmap(&vmap, src.pv, 3, dims, strides, box, dtype);
+        }
+        if (st) return st;
+        SharedPrefixArgs s;
+        s.n_seq = (int)n_seq;
+        s.n_kv = a.n_kv;
+        s.group = group;
+        s.seqs_per_tile = p.seqs_per_tile;
+        s.prefix = p.key0;
+        s.n_tiles = p.n_tiles;
+        s.splits = p.splits;
+        s.scale_log2 = a.scale_log2;
+        s.lens = paged ? a.lens : nullptr;
+        s.max_len = a.max_len;
+        s.ws = ws;
+        s.max_parts = max_parts;
+        s.block_table = src.block_table;
+        s.block_size = src.block_size;
+        s.n_blocks = src.n_blocks;
+        set_max_smem(attn_shared_prefix_kernel<T>, kPfSmemBytes);
+        attn_shared_prefix_kernel<T>
+            <<<dim3((unsigned)a.n_kv, (unsigned)p.splits, (unsigned)p.row_tiles), kPfThreads,
+               kPfSmemBytes, stream>>>(qmap, kmap, vmap, s);
+        KVB_CHECK_LAUNCH("attention_decode_shared prefix launch");
+    }
+    if (p.max_chunks > 0) {
+        CUtensorMap kmap, vmap;
+        const uint64_t dims[2] = {64, total_rows}, strides[1] = {128};
+        const uint32_t box[2] = {64, 64};
+        int st = encode_tmap(&kmap, src.kc, 2, dims, strides, box, dtype);
+        if (!st) st = encode_tmap(&vmap, src.vc, 2, dims, strides, box, dtype);
+        if (st) return st;
+        DecodeArgs d = {};
+        d.q = a.q;
+        d.q_row_stride = a.q_row_stride;
+        d.lens = a.lens;
+        d.max_len = a.max_len;
+        d.n_kv = a.n_kv;
+        d.group = group;
+        d.max_seq = src.max_seq;
+        d.seq_rows = src.seq_rows;
+        d.scale_log2 = a.scale_log2;
+        d.ws = ws;
+        d.chunk_keys = p.chunk_keys;
+        d.max_chunks = p.max_chunks;
+        d.block_table = src.block_table;
+        d.max_blocks = src.max_blocks;
+        d.block_size = src.block_size;
+        d.n_blocks = src.n_blocks;
+        d.key0 = paged ? p.key0 : 0;
+        d.part0 = p.splits;
+        d.max_parts = max_parts;
+        auto* kernel = attn_decode_kernel<T, false, true>;
+        set_max_smem(kernel, kDecSmemBytes);
+        const dim3 grid((unsigned)a.n_kv, (unsigned)n_seq, (unsigned)p.max_chunks);
+        cudaError_t e;
+        if (p.splits > 0) {
+            e = launch_pdl(kernel, grid, dim3(128), kDecSmemBytes, stream, kmap, vmap, d);
+        } else {  // nothing before it in this call: an ordinary launch
+            kernel<<<grid, 128, kDecSmemBytes, stream>>>(kmap, vmap, d);
+            e = cudaGetLastError();
+        }
+        if (e != cudaSuccess) return cuda_fail(e, "attention_decode_shared launch");
+    }
+    JoinArgs j;
+    j.ws = ws;
+    j.lens = a.lens;
+    j.max_len = a.max_len;
+    j.key0 = paged ? p.key0 : 0;
+    j.chunk_keys = p.chunk_keys;
+    j.fixed = p.splits;
+    j.max_parts = max_parts > 0 ? max_parts : 1;
+    j.n_kv = a.n_kv;
+    j.group = group;
+    j.hd = 64;
+    j.write_all = 1;
+    j.out = a.out;
+    j.out_row_stride = a.out_row_stride;
+    return launch_join(stream, j, n_seq, dtype);
+}
+
+// The tensor-core kernels where shape, alignment and workspace allow them (own_rows: rows of 64
+// elements of the contiguous caches), else the general kernel.
 template <typename T>
 static int launch_shared(kvb_stream_t stream, const GeneralDecodeArgs& a, const SharedSource<T>& src,
-                         size_t n_seq, void* ws, size_t ws_len) {
+                         size_t n_seq, size_t own_rows, void* ws, size_t ws_len) {
+    const bool paged = src.block_table != nullptr;
+    if (a.hd == 64 && a.n_q / a.n_kv <= kQ8MaxGroup && a.q_row_stride % 8 == 0 && aligned(a.q, 16) &&
+        aligned(src.kc, 16) && aligned(src.vc, 16) && aligned(src.pk, 16) && aligned(src.pv, 16) &&
+        n_seq <= 65535 && a.n_kv <= 65535 && ws != nullptr && aligned(ws, 16) &&
+        (paged ? src.block_size % 64 == 0 &&
+                     fits_i32((size_t)src.n_blocks * src.n_kv * src.block_size + 64)
+               : fits_i32(own_rows + 64))) {
+        // Paged: whole 64-key tiles of the prefix for all at once; each sequence reads the rest
+        // through its own table row.  Contiguous: all of the prefix.
+        const size_t shared = paged ? (size_t)src.prefix / 64 * 64 : (size_t)src.prefix;
+        const size_t own = paged ? (size_t)(a.max_len > (int)shared ? a.max_len - (int)shared : 0)
+                                 : (size_t)a.max_len;
+        const SharedPlan p = shared_plan(n_seq, shared, own, (size_t)a.n_q, (size_t)a.n_kv);
+        if (ws_len >= p.ws_bytes)
+            return launch_shared_tensor<T>(stream, a, src, p, n_seq, own_rows,
+                                           static_cast<float*>(ws));
+    }
     const dim3 grid((unsigned)n_seq, (unsigned)((a.n_q + 3) / 4));
     attn_general_src_kernel<T, SharedSource<T>><<<grid, 128, 0, stream>>>(a, src);
     KVB_CHECK_LAUNCH("attention_decode_shared launch");
@@ -472,8 +636,13 @@ int kvb_attention_decode_q8_paged(kvb_stream_t stream, const void* q, size_t q_r
 
 size_t kvb_attention_decode_shared_workspace_bytes(size_t n_seq, size_t shared_len, size_t max_own,
                                                    size_t n_q, size_t n_kv, size_t head_dim) {
-    (void)n_seq, (void)shared_len, (void)max_own, (void)n_q, (void)n_kv, (void)head_dim;
-    return 0;
+    if (head_dim != 64 || n_seq == 0 || n_kv == 0 || n_q % n_kv != 0 || n_q / n_kv == 0 ||
+        n_q / n_kv > (size_t)kQ8MaxGroup || !fits_i32(shared_len) || !fits_i32(max_own))
+        return 0;
+    // contiguous, or paged with the prefix cut to whole 64-key tiles: the larger need
+    const size_t a = shared_plan(n_seq, shared_len, max_own, n_q, n_kv).ws_bytes;
+    const size_t b = shared_plan(n_seq, shared_len / 64 * 64, max_own + shared_len % 64, n_q, n_kv).ws_bytes;
+    return a > b ? a : b;
 }
 
 int kvb_attention_decode_shared(kvb_stream_t stream, const void* q, size_t q_row_stride,
@@ -519,7 +688,7 @@ int kvb_attention_decode_shared(kvb_stream_t stream, const void* q, size_t q_row
         s.n_kv = (int)n_kv;
         s.hd = (int)head_dim;
         s.max_seq = (int)max_seq;
-        return launch_shared(stream, a, s, n_seq, workspace, workspace_len);
+        return launch_shared(stream, a, s, n_seq, cache_len / head_dim, workspace, workspace_len);
     };
     return dtype == KVB_BF16 ? go(__nv_bfloat16()) : go(__half());
 }
@@ -564,7 +733,7 @@ int kvb_attention_decode_shared_paged(kvb_stream_t stream, const void* q, size_t
         s.max_blocks = (int)max_blocks;
         s.block_size = (int)block_size;
         s.n_blocks = (int)(pool_len / per_block);
-        return launch_shared(stream, a, s, n_seq, workspace, workspace_len);
+        return launch_shared(stream, a, s, n_seq, 0, workspace, workspace_len);
     };
     return dtype == KVB_BF16 ? go(__nv_bfloat16()) : go(__half());
 }
