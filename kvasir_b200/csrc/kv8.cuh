@@ -173,6 +173,105 @@ __global__ void __launch_bounds__(128) kv8_append_general_kernel(Kv8AppendArgs a
     if (lane == 0) (is_v ? a.c.vs : a.c.ks)[crow] = rs.scale;
 }
 
+// Eight codes of values x (already 16-bit values in f32), packed in order.
+// int8: x * inv plus 1.5 * 2^23 leaves the integer rounded to nearest even in the low bits
+// of the sum; the multiply and the add are kept apart, as the definition rounds the product.
+template <int kFmt>
+__device__ __forceinline__ uint2 kv8_codes8(const float* x, float inv) {
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (kFmt == KVB_KV_INT8) {
+            uint32_t v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                v[k] = __float_as_uint(__fadd_rn(__fmul_rn(x[4 * i + k], inv), 12582912.f));
+            uint32_t lo, hi;
+            asm("prmt.b32 %0, %1, %2, 0x0040;" : "=r"(lo) : "r"(v[0]), "r"(v[1]));
+            asm("prmt.b32 %0, %1, %2, 0x0040;" : "=r"(hi) : "r"(v[2]), "r"(v[3]));
+            asm("prmt.b32 %0, %1, %2, 0x5410;" : "=r"(w[i]) : "r"(lo), "r"(hi));
+        } else {
+            w[i] = kv8_codes2<kFmt>(x[4 * i], x[4 * i + 1], inv) |
+                   (kv8_codes2<kFmt>(x[4 * i + 2], x[4 * i + 3], inv) << 16);
+        }
+    }
+    return inv == 0.f ? make_uint2(0u, 0u) : make_uint2(w[0], w[1]);
+}
+
+// head_dim = 16 CPR (64 or 128), 16-byte aligned rows and tables: one CTA per qkv row, a
+// thread per chunk of 8 pairs (elements 8j .. and 8j + head_dim / 2 ..) of a head, so that
+// the CPR threads of a head are neighbours and its largest magnitude takes log2 CPR
+// shuffles.  Both 16-byte loads of a thread are issued before its position is known.
+template <typename T, int kFmt, int CPR>
+__global__ void __launch_bounds__(1024) kv8_append_vec_kernel(Kv8AppendArgs a) {
+    constexpr int hd = 16 * CPR, half = 8 * CPR;
+    const int row = blockIdx.x;
+    const int seq = row / a.rows_per_seq;
+    const int heads = a.n_q + 2 * a.c.n_kv, items = heads * CPR;
+    const int n_rot = a.n_q + a.c.n_kv;
+    uint16_t* rowp = a.qkv + (size_t)row * a.row_stride;
+    bool placed = false;
+    size_t crow0 = 0, head_rows = 0;
+    // whole warps take part (shuffles); threads past the last item only keep them company
+    for (int it0 = threadIdx.x & ~31; it0 < items; it0 += blockDim.x) {
+        const int it = it0 + (threadIdx.x & 31);
+        const bool have = it < items;
+        const int h = it / CPR, j = it % CPR;
+        uint4* pa = reinterpret_cast<uint4*>(rowp + h * hd + 8 * j);
+        uint4* pb = reinterpret_cast<uint4*>(rowp + h * hd + 8 * j + half);
+        uint4 va = make_uint4(0u, 0u, 0u, 0u), vb = va;
+        if (have) {
+            va = *pa;
+            vb = *pb;
+        }
+        const int p = a.pos[seq] + (row - seq * a.rows_per_seq);
+        if (!placed) {
+            placed = true;
+            if (p < 0 || p >= a.c.max_seq || (a.cos_t && p >= a.max_pos)) {
+                if (threadIdx.x == 0) raise_dev_error(kDevErrBadPosition);
+                return;
+            }
+            if (!kv8_row(a.c, seq, p, crow0, head_rows, threadIdx.x == 0)) return;
+        }
+        float x0[8], x1[8];
+        unpack8<T>(va, x0);
+        unpack8<T>(vb, x1);
+        if (have && a.cos_t && h < n_rot) {
+            const float4* c4 = reinterpret_cast<const float4*>(a.cos_t + (size_t)p * half + 8 * j);
+            const float4* s4 = reinterpret_cast<const float4*>(a.sin_t + (size_t)p * half + 8 * j);
+            const float4 c0 = c4[0], c1 = c4[1], s0 = s4[0], s1 = s4[1];
+            const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+            const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+            float ra[8], rb[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                ra[e] = rot_a(x0[e], x1[e], c[e], sn[e]);
+                rb[e] = rot_b(x0[e], x1[e], c[e], sn[e]);
+            }
+            va = pack8<T>(ra);
+            vb = pack8<T>(rb);
+            *pa = va;
+            *pb = vb;
+            unpack8<T>(va, x0);
+            unpack8<T>(vb, x1);
+        }
+        if (it0 + 31 < a.n_q * CPR) continue;  // a warp of query heads
+        uint32_t mx = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx = max(mx, max(abs_bits(x0[e]), abs_bits(x1[e])));
+#pragma unroll
+        for (int o = 1; o < CPR; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        if (!have || h < a.n_q) continue;
+        const RowScale rs = kv8_row_scale<kFmt>(mx);
+        const bool is_v = h >= n_rot;
+        const size_t crow = crow0 + (size_t)(h - (is_v ? n_rot : a.n_q)) * head_rows;
+        uint8_t* dst = (is_v ? a.c.vc : a.c.kc) + crow * hd + 8 * j;
+        *reinterpret_cast<uint2*>(dst) = kv8_codes8<kFmt>(x0, rs.inv);
+        *reinterpret_cast<uint2*>(dst + half) = kv8_codes8<kFmt>(x1, rs.inv);
+        if (j == 0) (is_v ? a.c.vs : a.c.ks)[crow] = rs.scale;
+    }
+}
+
 struct Kv8ReadArgs {
     Kv8Place c;
     const int32_t* pos;
@@ -203,6 +302,45 @@ __global__ void __launch_bounds__(128) kv8_read_general_kernel(Kv8ReadArgs a, lo
     const uint8_t* src = (is_v ? a.c.vc : a.c.kc) + row * a.c.hd;
     for (int d = lane; d < a.c.hd; d += 32)
         out[d] = Elem<T>::from_f(ok ? kv8_value<kFmt>(src[d]) * scale : 0.f);
+}
+
+// head_dim a multiple of 16 (16-byte loads of codes), 16-byte aligned buffers: a thread
+// per 16 codes of a K row and the same codes of its V row.  blockIdx.y: (sequence, KV head).
+template <typename T, int kFmt>
+__global__ void __launch_bounds__(256) kv8_read_vec_kernel(Kv8ReadArgs a, int chunks_per_row) {
+    const int bh = blockIdx.y;
+    const int b = bh / a.c.n_kv, kvh = bh - b * a.c.n_kv;
+    const int it = blockIdx.x * 256 + threadIdx.x;
+    const int i = it / chunks_per_row, ch = it - i * chunks_per_row;
+    if (i >= a.t) return;
+    const int p = a.pos[b] + i;
+    size_t row = 0, head_rows = 0;
+    bool ok = p >= 0 && p < a.c.max_seq;
+    if (!ok && ch == 0) raise_dev_error(kDevErrBadPosition);
+    ok = ok && kv8_row(a.c, b, p, row, head_rows, ch == 0);
+    row += (size_t)kvh * head_rows;
+    uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
+    float fk = 0.f, fv = 0.f;
+    if (ok) {
+        k = ld_stream(a.c.kc + row * a.c.hd + 16 * ch);
+        v = ld_stream(a.c.vc + row * a.c.hd + 16 * ch);
+        fk = a.c.ks[row];
+        fv = a.c.vs[row];
+    }
+    const size_t o = ((size_t)bh * a.out_rows + i) * a.c.hd + 16 * ch;
+    auto expand = [](const uint4& codes, float f, uint16_t* out) {
+        const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                x[e] = kv8_value<kFmt>((uint8_t)(w[2 * u + e / 4] >> (8 * (e % 4)))) * f;
+            *reinterpret_cast<uint4*>(out + 8 * u) = pack8<T>(x);
+        }
+    };
+    expand(k, fk, a.k_out + o);
+    expand(v, fv, a.v_out + o);
 }
 
 }  // namespace kvb

@@ -88,6 +88,16 @@ static int kv8_place_paged(const char* name, Kv8Place& c, const void* k_pool, co
 // ---------------------------------------------------------------- append
 template <typename T, int kFmt>
 static int launch_kv8_append(kvb_stream_t stream, const Kv8AppendArgs& a, size_t rows) {
+    if ((a.c.hd == 64 || a.c.hd == 128) && aligned(a.qkv, 16) && aligned(a.cos_t, 16) &&
+        aligned(a.sin_t, 16) && aligned(a.c.kc, 8) && aligned(a.c.vc, 8)) {
+        const int cpr = a.c.hd / 16;
+        const long long items = (long long)(a.n_q + 2 * a.c.n_kv) * cpr;
+        const unsigned threads = items >= 1024 ? 1024u : (unsigned)((items + 31) / 32 * 32);
+        if (cpr == 4) kv8_append_vec_kernel<T, kFmt, 4><<<(unsigned)rows, threads, 0, stream>>>(a);
+        else kv8_append_vec_kernel<T, kFmt, 8><<<(unsigned)rows, threads, 0, stream>>>(a);
+        KVB_CHECK_LAUNCH("rope_kv_append_q8 launch");
+        return KVB_OK;
+    }
     const long long items = (long long)rows * (a.n_q + 2 * a.c.n_kv);
     const long long grid = (items + 3) / 4;
     KVB_CHECK(grid <= 0x7fffffffll, "rope_kv_append_q8: too many rows");
@@ -127,6 +137,15 @@ static int kv8_append(const char* name, kvb_stream_t stream, void* qkv, size_t q
 // ---------------------------------------------------------------- read back
 template <typename T, int kFmt>
 static int launch_kv8_read(kvb_stream_t stream, const Kv8ReadArgs& a, size_t n_seq) {
+    const int chunks = a.c.hd / 16;
+    const long long per_head = (long long)a.t * chunks;
+    if (a.c.hd % 16 == 0 && n_seq * a.c.n_kv <= 65535 && per_head <= 0x7fffff00ll &&
+        aligned(a.c.kc, 16) && aligned(a.c.vc, 16) && aligned(a.k_out, 16) && aligned(a.v_out, 16)) {
+        const dim3 grid((unsigned)((per_head + 255) / 256), (unsigned)(n_seq * a.c.n_kv));
+        kv8_read_vec_kernel<T, kFmt><<<grid, 256, 0, stream>>>(a, chunks);
+        KVB_CHECK_LAUNCH("kv_read_q8 launch");
+        return KVB_OK;
+    }
     const long long items = (long long)n_seq * a.t * a.c.n_kv * 2;
     const long long grid = (items + 3) / 4;
     KVB_CHECK(grid <= 0x7fffffffll, "kv_read_q8: too many rows");

@@ -333,39 +333,43 @@ class Gpu:
                                                   dtype_tag(qkv)))
 
     # ------------------------------------------------ 8-bit KV cache
-    def _check_on(self, name, i32, f32, *others):
-        """Device and element types of the tensors of one call."""
-        if torch.cuda.current_device() != self.device.index:
+    def _ptrs(self, name, *tensors):
+        """Addresses of contiguous tensors on this Gpu's device (None for None)."""
+        index = self.device.index
+        if torch.cuda.current_device() != index:
             raise ShapeError(f"{name}: the current device is not {self.device}")
-        for t in (*i32, *f32, *others):
-            if t is not None and t.device != self.device:
+        got = []
+        for t in tensors:
+            if t is None:
+                got.append(None)
+                continue
+            if t.get_device() != index:
                 raise ShapeError(f"{name}: a tensor is on {t.device}, not on {self.device}")
-        for t in i32:
-            if t.dtype != torch.int32:
-                raise ShapeError(f"{name}: positions, lengths and block tables must be int32")
-        for t in f32:
-            if t is not None and t.dtype != torch.float32:
-                raise ShapeError(f"{name}: scales and cos/sin tables must be float32")
+            if not t.is_contiguous():
+                raise ShapeError(f"{name}: buffers must be contiguous")
+            got.append(t.data_ptr())
+        return got
 
-    def _check_q8(self, name, kc, vc, ks, vs):
-        if kc.dtype != vc.dtype or kc.numel() != vc.numel() or ks.numel() != vs.numel():
-            raise ShapeError(f"{name}: K and V caches (or their scales) differ")
-        return kv_format(kc)
+    @staticmethod
+    def _check_types(name, dtype, *tensors):
+        for t in tensors:
+            if t is not None and t.dtype is not dtype:
+                raise ShapeError(f"{name}: a tensor is {t.dtype}, {dtype} expected")
 
     def rope_kv_append_q8(self, qkv, n_seq, t, pos, cos, sin, kc, vc, ks, vs, seq_stride, n_q,
                           n_kv, head_dim, max_seq):
         """kvb_rope_kv_append_q8: rows of sequence b at positions pos[b].. rotated in place,
         their k and v quantised into the 8-bit cache (codes kc / vc, int8 or float8_e4m3fn;
         f32 scales ks / vs, one per position and KV head).  cos = sin = None: no rotation."""
-        self._check_on("rope_kv_append_q8", (pos,), (cos, sin, ks, vs), qkv, kc, vc)
-        fmt = self._check_q8("rope_kv_append_q8", kc, vc, ks, vs)
-        if pos.numel() != n_seq or (cos is not None and sin is not None
-                                    and cos.numel() != sin.numel()):
-            raise ShapeError("rope_kv_append_q8: one position per sequence, cos and sin alike")
+        name = "rope_kv_append_q8"
+        p = self._ptrs(name, qkv, pos, cos, sin, kc, vc, ks, vs)
+        fmt, table = self._check_q8(name, kc, vc, ks, vs), self._check_table(name, cos, sin)
+        self._check_types(name, torch.int32, pos)
+        if pos.numel() != n_seq:
+            raise ShapeError(f"{name}: one position per sequence")
         check(self._lib.kvb_rope_kv_append_q8(
-            self._s, _ptr(qkv), qkv.numel(), n_seq, t, _ptr(pos), _ptr(cos), _ptr(sin),
-            cos.numel() if cos is not None else 0, _ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs),
-            seq_stride, kc.numel(), ks.numel(), n_q, n_kv, head_dim, max_seq, fmt,
+            self.stream.cuda_stream, p[0], qkv.numel(), n_seq, t, p[1], p[2], p[3], table, p[4],
+            p[5], p[6], p[7], seq_stride, kc.numel(), ks.numel(), n_q, n_kv, head_dim, max_seq, fmt,
             dtype_tag(qkv)))
 
     def rope_kv_append_q8_paged(self, qkv, n_seq, t, pos, cos, sin, k_pool, v_pool, k_scales,
@@ -373,97 +377,111 @@ class Gpu:
                                 head_dim):
         """kvb_rope_kv_append_q8_paged: the same into pools [n_blocks, n_kv, block_size,
         head_dim] of codes and [n_blocks, n_kv, block_size] of scales."""
-        self._check_on("rope_kv_append_q8_paged", (pos, block_table), (cos, sin, k_scales, v_scales),
-                       qkv, k_pool, v_pool)
-        fmt = self._check_q8("rope_kv_append_q8_paged", k_pool, v_pool, k_scales, v_scales)
-        if pos.numel() != n_seq or block_table.numel() != n_seq * max_blocks or (
-                cos is not None and sin is not None and cos.numel() != sin.numel()):
-            raise ShapeError("rope_kv_append_q8_paged: one position and one table row per sequence, "
-                             "cos and sin alike")
+        name = "rope_kv_append_q8_paged"
+        p = self._ptrs(name, qkv, pos, cos, sin, k_pool, v_pool, k_scales, v_scales, block_table)
+        fmt = self._check_q8(name, k_pool, v_pool, k_scales, v_scales)
+        table = self._check_table(name, cos, sin)
+        self._check_types(name, torch.int32, pos, block_table)
+        if pos.numel() != n_seq or block_table.numel() != n_seq * max_blocks:
+            raise ShapeError(f"{name}: one position and one table row per sequence")
         check(self._lib.kvb_rope_kv_append_q8_paged(
-            self._s, _ptr(qkv), qkv.numel(), n_seq, t, _ptr(pos), _ptr(cos), _ptr(sin),
-            cos.numel() if cos is not None else 0, _ptr(k_pool), _ptr(v_pool), _ptr(k_scales),
-            _ptr(v_scales), k_pool.numel(), k_scales.numel(), _ptr(block_table), max_blocks,
-            block_size, n_q, n_kv, head_dim, fmt, dtype_tag(qkv)))
+            self.stream.cuda_stream, p[0], qkv.numel(), n_seq, t, p[1], p[2], p[3], table, p[4],
+            p[5], p[6], p[7], k_pool.numel(), k_scales.numel(), p[8], max_blocks, block_size, n_q,
+            n_kv, head_dim, fmt, dtype_tag(qkv)))
 
     def kv_read_q8(self, kc, vc, ks, vs, seq_stride, pos, n_seq, t, n_kv, head_dim, max_seq, k_out,
                    v_out, out_rows):
         """kvb_kv_read_q8: positions pos[b] .. pos[b]+t-1 of an 8-bit cache as 16-bit rows
         0 .. t-1 of k_out / v_out [n_seq, n_kv, out_rows, head_dim]."""
-        self._check_on("kv_read_q8", (pos,), (ks, vs), kc, vc, k_out, v_out)
-        fmt = self._check_q8("kv_read_q8", kc, vc, ks, vs)
+        name = "kv_read_q8"
+        p = self._ptrs(name, kc, vc, ks, vs, pos, k_out, v_out)
+        fmt = self._check_q8(name, kc, vc, ks, vs)
+        self._check_types(name, torch.int32, pos)
         if pos.numel() != n_seq or k_out.dtype != v_out.dtype or k_out.numel() != v_out.numel():
-            raise ShapeError("kv_read_q8: one position per sequence, k_out and v_out alike")
+            raise ShapeError(f"{name}: one position per sequence, k_out and v_out alike")
         check(self._lib.kvb_kv_read_q8(
-            self._s, _ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs), seq_stride, kc.numel(), ks.numel(),
-            _ptr(pos), n_seq, t, n_kv, head_dim, max_seq, _ptr(k_out), _ptr(v_out), k_out.numel(),
-            out_rows, fmt, dtype_tag(k_out)))
+            self.stream.cuda_stream, p[0], p[1], p[2], p[3], seq_stride, kc.numel(), ks.numel(),
+            p[4], n_seq, t, n_kv, head_dim, max_seq, p[5], p[6], k_out.numel(), out_rows, fmt,
+            dtype_tag(k_out)))
 
     def kv_read_q8_paged(self, k_pool, v_pool, k_scales, v_scales, block_table, max_blocks,
                          block_size, pos, n_seq, t, n_kv, head_dim, k_out, v_out, out_rows):
         """kvb_kv_read_q8_paged: kv_read_q8 through a block table."""
-        self._check_on("kv_read_q8_paged", (pos, block_table), (k_scales, v_scales), k_pool, v_pool,
-                       k_out, v_out)
-        fmt = self._check_q8("kv_read_q8_paged", k_pool, v_pool, k_scales, v_scales)
+        name = "kv_read_q8_paged"
+        p = self._ptrs(name, k_pool, v_pool, k_scales, v_scales, block_table, pos, k_out, v_out)
+        fmt = self._check_q8(name, k_pool, v_pool, k_scales, v_scales)
+        self._check_types(name, torch.int32, pos, block_table)
         if (pos.numel() != n_seq or block_table.numel() != n_seq * max_blocks
                 or k_out.dtype != v_out.dtype or k_out.numel() != v_out.numel()):
-            raise ShapeError("kv_read_q8_paged: one position and one table row per sequence, "
-                             "k_out and v_out alike")
+            raise ShapeError(f"{name}: one position and one table row per sequence, k_out and "
+                             "v_out alike")
         check(self._lib.kvb_kv_read_q8_paged(
-            self._s, _ptr(k_pool), _ptr(v_pool), _ptr(k_scales), _ptr(v_scales), k_pool.numel(),
-            k_scales.numel(), _ptr(block_table), max_blocks, block_size, _ptr(pos), n_seq, t, n_kv,
-            head_dim, _ptr(k_out), _ptr(v_out), k_out.numel(), out_rows, fmt, dtype_tag(k_out)))
+            self.stream.cuda_stream, p[0], p[1], p[2], p[3], k_pool.numel(), k_scales.numel(), p[4],
+            max_blocks, block_size, p[5], n_seq, t, n_kv, head_dim, p[6], p[7], k_out.numel(),
+            out_rows, fmt, dtype_tag(k_out)))
 
     def attention_decode_q8_workspace_bytes(self, n_seq, max_len, n_q, n_kv, head_dim) -> int:
         return int(self._lib.kvb_attention_decode_q8_workspace_bytes(n_seq, max_len, n_q, n_kv,
                                                                      head_dim))
 
-    @staticmethod
-    def _check_rows(name, t, n_seq, row_stride, n_q, head_dim):
-        """t holds n_seq rows of n_q * head_dim elements, row_stride apart."""
-        if n_seq and t.numel() < (n_seq - 1) * row_stride + n_q * head_dim:
-            raise ShapeError(f"{name}: {t.numel()} elements hold no {n_seq} rows {row_stride} apart")
+    def _check_q8(self, name, kc, vc, ks, vs):
+        if kc.dtype is not vc.dtype or kc.numel() != vc.numel() or ks.numel() != vs.numel():
+            raise ShapeError(f"{name}: K and V caches (or their scales) differ")
+        self._check_types(name, torch.float32, ks, vs)
+        return kv_format(kc)
 
-    def _check_attention(self, name, q, q_row_stride, out, out_row_stride, n_seq, n_q, head_dim,
-                         *caches):
-        if out.dtype != q.dtype or any(c.dtype != q.dtype for c in caches):
-            raise ShapeError(f"{name}: q, out and 16-bit caches must have one type")
-        self._check_rows(name, q, n_seq, q_row_stride, n_q, head_dim)
-        self._check_rows(name, out, n_seq, out_row_stride, n_q, head_dim)
+    def _check_table(self, name, cos, sin):
+        """Elements of the cos / sin tables (0 without)."""
+        self._check_types(name, torch.float32, cos, sin)
+        if (cos is None) != (sin is None) or (cos is not None and cos.numel() != sin.numel()):
+            raise ShapeError(f"{name}: bad cos/sin table sizes")
+        return cos.numel() if cos is not None else 0
+
+    def _check_attention(self, name, q, q_row_stride, lens, out, out_row_stride, row, *caches):
+        """lens is int32; q and out hold rows of `row` elements, their strides apart; one
+        16-bit type."""
+        self._check_types(name, torch.int32, lens)
+        self._check_types(name, q.dtype, out, *caches)
+        n = lens.numel()
+        if n and (q.numel() < (n - 1) * q_row_stride + row
+                  or out.numel() < (n - 1) * out_row_stride + row):
+            raise ShapeError(f"{name}: q or out holds no {n} rows of {row} elements")
+        return n
 
     def attention_decode_q8(self, q, q_row_stride, kc, vc, ks, vs, seq_stride, lens, max_len, n_q,
                             n_kv, head_dim, max_seq, out, out_row_stride, scale=None,
                             workspace=None):
         """kvb_attention_decode_q8: attention_decode over an 8-bit cache."""
-        self._check_on("attention_decode_q8", (lens,), (ks, vs), q, kc, vc, out, workspace)
-        fmt = self._check_q8("attention_decode_q8", kc, vc, ks, vs)
-        self._check_attention("attention_decode_q8", q, q_row_stride, out, out_row_stride,
-                              lens.numel(), n_q, head_dim)
+        name = "attention_decode_q8"
+        p = self._ptrs(name, q, kc, vc, ks, vs, lens, out, workspace)
+        fmt = self._check_q8(name, kc, vc, ks, vs)
+        n_seq = self._check_attention(name, q, q_row_stride, lens, out, out_row_stride,
+                                      n_q * head_dim)
         scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
-        ws_len = workspace.numel() * workspace.element_size() if workspace is not None else 0
         check(self._lib.kvb_attention_decode_q8(
-            self._s, _ptr(q), q_row_stride, _ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs), seq_stride,
-            kc.numel(), ks.numel(), _ptr(lens), lens.numel(), max_len, n_q, n_kv, head_dim, max_seq,
-            scale, _ptr(out), out_row_stride, _ptr(workspace), ws_len, fmt, dtype_tag(q)))
+            self.stream.cuda_stream, p[0], q_row_stride, p[1], p[2], p[3], p[4], seq_stride,
+            kc.numel(), ks.numel(), p[5], n_seq, max_len, n_q, n_kv, head_dim, max_seq, scale, p[6],
+            out_row_stride, p[7], workspace.nbytes if workspace is not None else 0, fmt,
+            dtype_tag(q)))
 
     def attention_decode_q8_paged(self, q, q_row_stride, k_pool, v_pool, k_scales, v_scales,
                                   block_table, max_blocks, block_size, lens, max_len, n_q, n_kv,
                                   head_dim, out, out_row_stride, scale=None, workspace=None):
         """kvb_attention_decode_q8_paged: attention_decode_paged over 8-bit pools."""
-        self._check_on("attention_decode_q8_paged", (lens, block_table), (k_scales, v_scales), q,
-                       k_pool, v_pool, out, workspace)
-        fmt = self._check_q8("attention_decode_q8_paged", k_pool, v_pool, k_scales, v_scales)
-        if block_table.numel() != lens.numel() * max_blocks:
-            raise ShapeError("attention_decode_q8_paged: one table row per sequence")
-        self._check_attention("attention_decode_q8_paged", q, q_row_stride, out, out_row_stride,
-                              lens.numel(), n_q, head_dim)
+        name = "attention_decode_q8_paged"
+        p = self._ptrs(name, q, k_pool, v_pool, k_scales, v_scales, block_table, lens, out, workspace)
+        fmt = self._check_q8(name, k_pool, v_pool, k_scales, v_scales)
+        n_seq = self._check_attention(name, q, q_row_stride, lens, out, out_row_stride,
+                                      n_q * head_dim)
+        self._check_types(name, torch.int32, block_table)
+        if block_table.numel() != n_seq * max_blocks:
+            raise ShapeError(f"{name}: one table row per sequence")
         scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
-        ws_len = workspace.numel() * workspace.element_size() if workspace is not None else 0
         check(self._lib.kvb_attention_decode_q8_paged(
-            self._s, _ptr(q), q_row_stride, _ptr(k_pool), _ptr(v_pool), _ptr(k_scales),
-            _ptr(v_scales), k_pool.numel(), k_scales.numel(), _ptr(block_table), max_blocks,
-            block_size, _ptr(lens), lens.numel(), max_len, n_q, n_kv, head_dim, scale, _ptr(out),
-            out_row_stride, _ptr(workspace), ws_len, fmt, dtype_tag(q)))
+            self.stream.cuda_stream, p[0], q_row_stride, p[1], p[2], p[3], p[4], k_pool.numel(),
+            k_scales.numel(), p[5], max_blocks, block_size, p[6], n_seq, max_len, n_q, n_kv,
+            head_dim, scale, p[7], out_row_stride, p[8],
+            workspace.nbytes if workspace is not None else 0, fmt, dtype_tag(q)))
 
     # ------------------------------------------------ shared-prefix decode attention
     def attention_decode_shared_workspace_bytes(self, n_seq, shared_len, max_own, n_q, n_kv,
@@ -477,37 +495,37 @@ class Gpu:
                                 out_row_stride, scale=None, workspace=None):
         """kvb_attention_decode_shared: every sequence attends to the keys [0, prefix_len) of
         pk / pv [n_kv, prefix_rows, head_dim], read once for all, then to its own lens[b]."""
-        self._check_on("attention_decode_shared", (lens,), (), q, pk, pv, kc, vc, out, workspace)
+        name = "attention_decode_shared"
+        p = self._ptrs(name, q, pk, pv, kc, vc, lens, out, workspace)
+        n_seq = self._check_attention(name, q, q_row_stride, lens, out, out_row_stride,
+                                      n_q * head_dim, pk, pv, kc, vc)
         if (kc.numel() != vc.numel() or pk.numel() != pv.numel()
                 or pk.numel() != n_kv * prefix_rows * head_dim):
-            raise ShapeError("attention_decode_shared: bad cache or prefix sizes")
-        self._check_attention("attention_decode_shared", q, q_row_stride, out, out_row_stride,
-                              lens.numel(), n_q, head_dim, pk, pv, kc, vc)
+            raise ShapeError(f"{name}: bad cache or prefix sizes")
         scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
-        ws_len = workspace.numel() * workspace.element_size() if workspace is not None else 0
         check(self._lib.kvb_attention_decode_shared(
-            self._s, _ptr(q), q_row_stride, _ptr(pk), _ptr(pv), prefix_len, prefix_rows, _ptr(kc),
-            _ptr(vc), seq_stride, kc.numel(), _ptr(lens), lens.numel(), max_len, n_q, n_kv, head_dim,
-            max_seq, scale, _ptr(out), out_row_stride, _ptr(workspace), ws_len, dtype_tag(q)))
+            self.stream.cuda_stream, p[0], q_row_stride, p[1], p[2], prefix_len, prefix_rows, p[3],
+            p[4], seq_stride, kc.numel(), p[5], n_seq, max_len, n_q, n_kv, head_dim, max_seq, scale,
+            p[6], out_row_stride, p[7], workspace.nbytes if workspace is not None else 0,
+            dtype_tag(q)))
 
     def attention_decode_shared_paged(self, q, q_row_stride, k_pool, v_pool, block_table,
                                       max_blocks, block_size, shared_len, lens, max_len, n_q, n_kv,
                                       head_dim, out, out_row_stride, scale=None, workspace=None):
         """kvb_attention_decode_shared_paged: attention_decode_paged where the first shared_len
         keys of every sequence are the same (read through row 0 of the block table)."""
-        self._check_on("attention_decode_shared_paged", (lens, block_table), (), q, k_pool, v_pool,
-                       out, workspace)
-        if k_pool.numel() != v_pool.numel() or block_table.numel() != lens.numel() * max_blocks:
-            raise ShapeError("attention_decode_shared_paged: pool sizes differ, or not one table "
-                             "row per sequence")
-        self._check_attention("attention_decode_shared_paged", q, q_row_stride, out, out_row_stride,
-                              lens.numel(), n_q, head_dim, k_pool, v_pool)
+        name = "attention_decode_shared_paged"
+        p = self._ptrs(name, q, k_pool, v_pool, block_table, lens, out, workspace)
+        n_seq = self._check_attention(name, q, q_row_stride, lens, out, out_row_stride,
+                                      n_q * head_dim, k_pool, v_pool)
+        self._check_types(name, torch.int32, block_table)
+        if k_pool.numel() != v_pool.numel() or block_table.numel() != n_seq * max_blocks:
+            raise ShapeError(f"{name}: pool sizes differ, or not one table row per sequence")
         scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
-        ws_len = workspace.numel() * workspace.element_size() if workspace is not None else 0
         check(self._lib.kvb_attention_decode_shared_paged(
-            self._s, _ptr(q), q_row_stride, _ptr(k_pool), _ptr(v_pool), k_pool.numel(),
-            _ptr(block_table), max_blocks, block_size, shared_len, _ptr(lens), lens.numel(), max_len,
-            n_q, n_kv, head_dim, scale, _ptr(out), out_row_stride, _ptr(workspace), ws_len,
+            self.stream.cuda_stream, p[0], q_row_stride, p[1], p[2], k_pool.numel(), p[3],
+            max_blocks, block_size, shared_len, p[4], n_seq, max_len, n_q, n_kv, head_dim, scale,
+            p[5], out_row_stride, p[6], workspace.nbytes if workspace is not None else 0,
             dtype_tag(q)))
 
     def lm_head_argmax(self, x, w, rows, hidden, vocab, ids, workspace=None, advance=None,
