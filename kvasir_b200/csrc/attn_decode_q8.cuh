@@ -2,8 +2,7 @@
 // or 128, up to 16 query heads per KV head.
 //
 // Work unit: one CTA per (key chunk, KV head, sequence); its four warps take interleaved
-// tiles of 64 keys (head_dim 128: 32), 4 KB of K codes and 4 KB of V codes, each warp
-// through a ring of its own.  The transposed products put the keys on the MMA's 16-row
+// tiles of 64 keys (head_dim 128: 32), 4 KB of K codes and 4 KB of V codes.  The transposed products put the keys on the MMA's 16-row
 // side and the group's heads on its 8-column side, so a group of up to 8 heads wastes no
 // rows and takes half the instructions of a 16-row query tile:
 //   S^T = K Q^T    m16n8k16, A = K codes as f16 (ldmatrix; a lane's four bytes are four
@@ -29,12 +28,17 @@
 namespace kvb {
 
 constexpr int kQ8Warps = 4;
-constexpr int kQ8Stages = 2;
 constexpr int kQ8TileBytes = 4096;  // K codes (or V codes) of a tile
-constexpr int kQ8RingBytes = kQ8Warps * kQ8Stages * 2 * kQ8TileBytes;
+constexpr int kQ8Stages = 2;
+constexpr int kQ8WarpBytes = kQ8Stages * 2 * kQ8TileBytes;  // a warp's ring: [stage][K | V]
+constexpr int kQ8TilesBytes = kQ8Warps * kQ8WarpBytes;
 constexpr int kQ8ScaleBytes = kQ8Warps * kQ8Stages * 2 * 64 * 4;
-constexpr int kQ8SmemBytes = kQ8RingBytes + kQ8ScaleBytes + 1024;
+constexpr int kQ8CtasPerSm = 3;
 constexpr int kQ8MaxGroup = 16;
+// tiles, scales, a chunk's folded O (group x head_dim floats), alignment slack
+__host__ __device__ constexpr int q8_smem_bytes(int hd, int nt) {
+    return kQ8TilesBytes + kQ8ScaleBytes + 8 * nt * hd * 4 + 1024;
+}
 
 __host__ __device__ constexpr int q8_tile_keys(int hd) { return kQ8TileBytes / hd; }
 
@@ -148,14 +152,14 @@ __device__ __forceinline__ uint32_t q8_smem_off(int r, int ch) {
 // clusters of max_chunks CTAs; slots count chunks from the end of the sequence, so full
 // chunks are dispatched first (as attn_decode.cuh).
 template <typename T, int kFmt, int HD, int NT>
-__global__ void __launch_bounds__(128, 3)
+__global__ void __launch_bounds__(128, kQ8CtasPerSm)
     attn_decode_q8_kernel(const __grid_constant__ CUtensorMap kmap,
                           const __grid_constant__ CUtensorMap vmap, Q8DecodeArgs a) {
     constexpr int KT = q8_tile_keys(HD);  // keys per tile
     constexpr int MT = KT / 16;           // 16-key MMA rows of S^T, k-steps of P V
     constexpr int DT = HD / 16;           // 16-dim chunks: k-steps of K Q, MMA rows of O^T
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[kQ8Warps][kQ8Stages];
+    __shared__ uint64_t bars[kQ8Warps][kQ8Stages][2];  // K tile and scales; V tile and scales
     __shared__ float w_ml[kQ8Warps][2][kQ8MaxGroup];
     __shared__ float fold_ml[2][kQ8MaxGroup];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -167,8 +171,8 @@ __global__ void __launch_bounds__(128, 3)
     const int kvh = a.fold ? (int)blockIdx.y : (int)blockIdx.x;
     const int b = a.fold ? (int)blockIdx.z : (int)blockIdx.y;
     const int G = a.group;
-    if (threadIdx.x < kQ8Warps * kQ8Stages)
-        mbar_init(&bars[0][0] + threadIdx.x, 1 + 32);  // one expect_tx, 32 scale arrivals
+    if (threadIdx.x < kQ8Warps * kQ8Stages * 2)
+        mbar_init(&bars[0][0][0] + threadIdx.x, 1 + 32);  // one expect_tx, 32 scale arrivals
     fence_mbar_init();
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -183,14 +187,15 @@ __global__ void __launch_bounds__(128, 3)
         return;
     }
     const bool active = from_end < n_chunks;
-    float* wo = reinterpret_cast<float*>(smem + warp * kQ8Stages * 2 * kQ8TileBytes);  // [16][HD]
-    float* fold_o = reinterpret_cast<float*>(smem + 2 * kQ8TileBytes);  // warp 0's second stage
+    uint8_t* ring = smem + warp * kQ8WarpBytes;
+    float* ring_scales = reinterpret_cast<float*>(smem + kQ8TilesBytes) + warp * kQ8Stages * 128;
+    // this warp's O for the merge, [8 NT][HD] over its own tiles
+    float* wo = reinterpret_cast<float*>(ring);
+    float* fold_o = reinterpret_cast<float*>(smem + kQ8TilesBytes + kQ8ScaleBytes);
     if (active) {
         const int chunk = n_chunks - 1 - from_end;
         const int key_begin = chunk * a.chunk_keys;
         const int key_end = min(len, key_begin + a.chunk_keys);
-        uint8_t* ring = smem + warp * kQ8Stages * 2 * kQ8TileBytes;
-        float* scales = reinterpret_cast<float*>(smem + kQ8RingBytes) + warp * kQ8Stages * 128;
         const int row_base = (int)(b * a.c.seq_rows + (long long)kvh * a.c.max_seq);
         const int pshift = __ffs(a.piece) - 1;
 
@@ -200,51 +205,67 @@ __global__ void __launch_bounds__(128, 3)
             if (!a.c.block_table || lane >= (KT >> pshift) || k >= key_end) return 0;
             return a.c.block_table[(size_t)b * a.c.max_blocks + k / a.c.block_size];
         };
-        int kt_issue = key_begin + warp * KT;
-        int blk = block_of(kt_issue);
-        // Requests the warp's next tile into stage st: codes by tensor copies, scales by 4-byte
-        // copies (zero past the last key), all counted on the stage's barrier.
-        auto issue = [&](int st) {
-            const int kt0 = kt_issue;
-            if (kt0 >= key_end) return;
+        int blk = block_of(key_begin + warp * KT);
+        // The tile that is requested next: its pieces, this lane's piece's row, and the rows of
+        // this lane's two keys (-1: none, their scales are zero).
+        int n_pieces = 0, row = 0, key_row[KT / 32];
+        auto place = [&](int kt0) {
             const int nk = min(KT, key_end - kt0);
-            const int n_pieces = a.c.block_table ? (nk + a.piece - 1) >> pshift : 1;
-            int row = a.total_rows;  // past the end: zeros
+            if (!a.c.block_table) {
+                n_pieces = 1;
+                row = row_base + kt0;
+#pragma unroll
+                for (int u = 0; u < KT / 32; ++u)
+                    key_row[u] = lane + 32 * u < nk ? row + lane + 32 * u : -1;
+                return;
+            }
+            n_pieces = (nk + a.piece - 1) >> pshift;
+            row = a.total_rows;  // past the end: zeros
             if (lane < n_pieces) {
-                if (!a.c.block_table) {
-                    row = row_base + kt0;
-                } else if (blk < 0 || blk >= a.c.n_blocks) {
+                if (blk < 0 || blk >= a.c.n_blocks)
                     raise_dev_error(kDevErrBadPosition);
-                } else {
+                else
                     row = (blk * a.c.n_kv + kvh) * a.c.block_size +
                           (kt0 + (lane << pshift)) % a.c.block_size;
-                }
             }
-            kt_issue += kQ8Warps * KT;
-            blk = block_of(kt_issue);
-            uint64_t* bar = &bars[warp][st];
-            uint8_t* kdst = ring + st * 2 * kQ8TileBytes;
-            if (lane == 0) mbar_expect_tx(bar, (uint32_t)(2 * n_pieces * a.piece * HD));
-            __syncwarp();
-            if (lane < n_pieces) {
-                const int off = (lane << pshift) * HD;
-                tma_load_2d(kdst + off, &kmap, bar, 0, row);
-                tma_load_2d(kdst + kQ8TileBytes + off, &vmap, bar, 0, row);
-            }
-            const uint32_t sdst = smem_u32(scales + st * 128);
+            blk = block_of(kt0 + kQ8Warps * KT);  // of the tile that is placed next
 #pragma unroll
             for (int u = 0; u < KT / 32; ++u) {
                 const int k = lane + 32 * u;
                 const int r0 = __shfl_sync(0xffffffffu, row, k >> pshift);
-                const bool ok = k < nk && r0 < a.total_rows;
-                const size_t r = ok ? (size_t)r0 + (k & (a.piece - 1)) : 0;
-                cp_async4(sdst + 4 * k, a.c.ks + r, ok ? 4 : 0);
-                cp_async4(sdst + 256 + 4 * k, a.c.vs + r, ok ? 4 : 0);
+                key_row[u] = k < nk && r0 < a.total_rows ? r0 + (k & (a.piece - 1)) : -1;
             }
+        };
+        // Requests the placed tile's K (or V) codes by tensor copies and scales by 4-byte
+        // copies, all counted on the tile's barrier.
+        auto request = [&](const CUtensorMap& map, uint8_t* tile, const float* scales, float* dst,
+                           uint64_t* bar) {
+            if (lane == 0) mbar_expect_tx(bar, (uint32_t)(n_pieces * a.piece * HD));
+            __syncwarp();
+            if (lane < n_pieces) tma_load_2d(tile + (lane << pshift) * HD, &map, bar, 0, row);
+#pragma unroll
+            for (int u = 0; u < KT / 32; ++u)
+                cp_async4(smem_u32(dst + lane + 32 * u), scales + max(key_row[u], 0),
+                          key_row[u] >= 0 ? 4 : 0);
             cp_async_arrive(bar);
         };
+        auto request_k = [&](int st) {
+            request(kmap, ring + st * 2 * kQ8TileBytes, a.c.ks, ring_scales + st * 128,
+                    &bars[warp][st][0]);
+        };
+        auto request_v = [&](int st) {
+            request(vmap, ring + (st * 2 + 1) * kQ8TileBytes, a.c.vs, ring_scales + st * 128 + 64,
+                    &bars[warp][st][1]);
+        };
 #pragma unroll
-        for (int s = 0; s < kQ8Stages; ++s) issue(s);
+        for (int i = 0; i < kQ8Stages; ++i) {
+            const int kt0 = key_begin + (warp + i * kQ8Warps) * KT;
+            if (kt0 < key_end) {
+                place(kt0);
+                request_k(i);
+                request_v(i);
+            }
+        }
 
         // Q fragments (B operand): column g = head 8 nt + g, dims 16 j + 4c .. + 3.
         uint32_t qf[DT][NT][2];
@@ -297,16 +318,26 @@ __global__ void __launch_bounds__(128, 3)
             for (int j = 0; j < DT; ++j) o[j][nt][0] = o[j][nt][1] = o[j][nt][2] = o[j][nt][3] = 0.f;
         }
         int ev = 14;  // biased exponent of the largest V scale seen; O is in units of 2^(ev - 140)
+        // Two tiles per warp in flight, K and V on barriers of their own: the K of the tile
+        // after next is requested once the scores are out of this one, its V once P V has read
+        // this V.
         bool ok = true;
         int it = 0;
+        bool k_failed = false;
         for (int kt0 = key_begin + warp * KT; kt0 < key_end; kt0 += kQ8Warps * KT, ++it) {
             const int st = it % kQ8Stages;
+            const uint32_t phase = (it / kQ8Stages) & 1;
             const int nk = min(KT, key_end - kt0);
-            ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][st], (it / kQ8Stages) & 1));
-            if (!ok) break;
+            const int kt_next = kt0 + kQ8Stages * kQ8Warps * KT;
+            const bool more = kt_next < key_end;
             const uint32_t kb = smem_u32(ring + st * 2 * kQ8TileBytes), vb = kb + kQ8TileBytes;
-            const float* ks = scales + st * 128;
+            const float* ks = ring_scales + st * 128;
             const float* vs = ks + 64;
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][st][0], phase));
+            if (!ok) {
+                k_failed = true;
+                break;
+            }
 
             // ---- S^T = K Q^T
             float s[MT][NT][4];
@@ -343,6 +374,12 @@ __global__ void __launch_bounds__(128, 3)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[t][nt][e] *= (e < 2 ? k0 : k1) * qs[nt][e & 1];
             }
+            __syncwarp();
+            fence_async_smem();  // these reads precede the next copies into the K tile
+            if (more) {
+                place(kt_next);
+                request_k(st);
+            }
             if (nk < KT) {
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
@@ -351,13 +388,6 @@ __global__ void __launch_bounds__(128, 3)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             if (16 * t + g + 8 * (e >> 1) >= nk) s[t][nt][e] = -INFINITY;
-                if (kFmt == KVB_KV_E4M3) {  // V codes past the last key may be NaN: 0 * NaN
-                    const uint32_t z = 0;
-                    for (int i = nk * HD / 16 + lane; i < KT * HD / 16; i += 32)
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vb + 16 * i), "r"(z)
-                                     : "memory");
-                    __syncwarp();
-                }
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -372,7 +402,34 @@ __global__ void __launch_bounds__(128, 3)
                     mx[nt][1] = fmaxf(mx[nt][1], __shfl_xor_sync(0xffffffffu, mx[nt][1], x));
                 }
             }
-            // ---- V scale exponent: rescale O where a larger one appears
+            float al[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float mn = fmaxf(m[nt][e], mx[nt][e]);
+                    const float ref = mn == -INFINITY ? 0.f : mn;
+                    al[nt][e] = ex2_approx(m[nt][e] - ref);
+                    m[nt][e] = mn;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        s[t][nt][e] = ex2_approx(s[t][nt][e] - ref);
+                        s[t][nt][e + 2] = ex2_approx(s[t][nt][e + 2] - ref);
+                        sum += s[t][nt][e] + s[t][nt][e + 2];
+                    }
+                    // this lane's keys; summed over lanes at the end
+                    l[nt][e] = l[nt][e] * al[nt][e] + sum;
+                }
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][st][1], phase));
+            if (!ok) break;
+            if (kFmt == KVB_KV_E4M3 && nk < KT) {  // codes past the last key may be NaN: 0 * NaN
+                for (int i = nk * HD / 16 + lane; i < KT * HD / 16; i += 32)
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vb + 16 * i), "r"(0)
+                                 : "memory");
+                __syncwarp();
+            }
+            // ---- V scale exponent: O is rescaled where a larger one appears
             uint32_t vmax = __float_as_uint(vs[lane]) & 0x7fffffffu;
             if (KT == 64) vmax = max(vmax, __float_as_uint(vs[lane + 32]) & 0x7fffffffu);
             const int en = max(ev, (int)(__reduce_max_sync(0xffffffffu, vmax) >> 23));
@@ -384,19 +441,7 @@ __global__ void __launch_bounds__(128, 3)
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float mn = fmaxf(m[nt][e], mx[nt][e]);
-                    const float ref = mn == -INFINITY ? 0.f : mn;
-                    const float al = ex2_approx(m[nt][e] - ref);
-                    m[nt][e] = mn;
-                    float sum = 0.f;
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        s[t][nt][e] = ex2_approx(s[t][nt][e] - ref);
-                        s[t][nt][e + 2] = ex2_approx(s[t][nt][e + 2] - ref);
-                        sum += s[t][nt][e] + s[t][nt][e + 2];
-                    }
-                    l[nt][e] = l[nt][e] * al + sum;  // this lane's keys; summed over lanes at the end
-                    const float ao = al * rv;
+                    const float ao = al[nt][e] * rv;
 #pragma unroll
                     for (int j = 0; j < DT; ++j) {
                         o[j][nt][e] *= ao;
@@ -430,15 +475,19 @@ __global__ void __launch_bounds__(128, 3)
                 }
             }
             __syncwarp();
-            fence_async_smem();  // these reads precede the next copies into the stage
-            issue(st);
+            fence_async_smem();  // these reads precede the next copies into the V tile
+            if (more) request_v(st);
         }
         if (!ok) {
             // A copy did not complete in time (the error word is set): wait once more, bounded,
-            // for every stage still outstanding, and contribute an empty state.
-            for (int i = it; i < it + kQ8Stages; ++i)
-                if (key_begin + (warp + i * kQ8Warps) * KT < key_end)
-                    mbar_wait(&bars[warp][i % kQ8Stages], (i / kQ8Stages) & 1);
+            // for each copy still outstanding, and contribute an empty state.
+            for (int i = it; i <= it + kQ8Stages; ++i) {
+                if (key_begin + (warp + i * kQ8Warps) * KT >= key_end) break;
+                const uint32_t ph = (i / kQ8Stages) & 1;
+                const bool k_asked = i < it + kQ8Stages || !k_failed;
+                if (k_asked && (i > it || k_failed)) mbar_wait(&bars[warp][i % kQ8Stages][0], ph);
+                if (i < it + kQ8Stages) mbar_wait(&bars[warp][i % kQ8Stages][1], ph);
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 m[nt][0] = m[nt][1] = -INFINITY;
@@ -477,25 +526,37 @@ __global__ void __launch_bounds__(128, 3)
             mlb = a.fold ? &fold_ml[0][0] : wsb + G * HD;
         }
         const int ml_step = a.fold ? kQ8MaxGroup : G;
-        for (int i = threadIdx.x; i < G * HD; i += blockDim.x) {
+        // Four neighbouring dims of one head per thread and turn; 128 threads span 512 / HD
+        // heads a turn.
+        for (int i = 4 * threadIdx.x; i < G * HD; i += 4 * kQ8Warps * 32) {
             const int r = i / HD;
             float M = -INFINITY;
 #pragma unroll
             for (int w = 0; w < kQ8Warps; ++w) M = fmaxf(M, w_ml[w][0][r]);
-            float L = 0.f, O = 0.f;
+            float L = 0.f;
+            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kQ8Warps; ++w) {
                 const float mw = w_ml[w][0][r];
-                const float f = mw == -INFINITY ? 0.f : exp2f(mw - M);
+                const float f = mw == -INFINITY ? 0.f : ex2_approx(mw - M);
                 // a warp whose scores were all NaN keeps -inf as its maximum and a NaN sum
                 const float lw = w_ml[w][1][r];
                 L += lw != lw ? lw : lw * f;
-                O += reinterpret_cast<const float*>(smem + w * kQ8Stages * 2 * kQ8TileBytes)[i] * f;
+                const float4 ow = *reinterpret_cast<const float4*>(smem + w * kQ8WarpBytes + 4 * i);
+                O.x += ow.x * f;
+                O.y += ow.y * f;
+                O.z += ow.z * f;
+                O.w += ow.w * f;
             }
             if (n_chunks == 1) {
-                outb[i] = Elem<T>::from_f(O / L);
-            } else {
-                wsb[i] = O;
+                const float inv = 1.f / L;
+                outb[i] = Elem<T>::from_f(O.x * inv);
+                outb[i + 1] = Elem<T>::from_f(O.y * inv);
+                outb[i + 2] = Elem<T>::from_f(O.z * inv);
+                outb[i + 3] = Elem<T>::from_f(O.w * inv);
+            } else {  // 8-byte stores: a part of G (HD + 2) floats starts at a multiple of 8 bytes
+                *reinterpret_cast<float2*>(wsb + i) = make_float2(O.x, O.y);
+                *reinterpret_cast<float2*>(wsb + i + 2) = make_float2(O.z, O.w);
                 if (i % HD == 0) {
                     mlb[r] = M;
                     mlb[ml_step + r] = L;

@@ -223,16 +223,24 @@ static bool q8_tensor_shape(size_t head_dim, size_t n_q, size_t n_kv) {
            n_q / n_kv <= (size_t)kQ8MaxGroup;
 }
 
-// Keys per CTA of a split call: as decode_chunk_keys (about five waves of three CTAs per SM
-// over the worst case; one tile per warp at least, four once the (sequence, KV head) pairs
-// alone fill the SMs), and at most kJoinMaxParts chunks.
+// Keys per CTA of a split call.  Long batches: about five waves of three CTAs per SM over the
+// worst case (every sequence at max_len), as decode_chunk_keys.  Below that, as few tiles as
+// fill one wave, between 4 (one per warp) and 16: shorter chunks pay more starts and a longer
+// join, longer ones leave a longer last wave.  Pairs of (sequence, KV head) that fill the SMs
+// by themselves with at most 24 tiles take one chunk each and no join.  Measured on B200,
+// tiles per CTA: 37 sequences x 2 heads U[0,5003] (head_dim 128) 8 / 16 / 32 / 48: 27.6 /
+// 25.0 / 25.6 / 31.7 us; 32 x 8 at 1000 keys 8 / 12 / 17: 19.5 / 15.7 / 15.2; 64 x 8
+// U[1,4096] 8 / 16 / 24 / 48: 40.3 / 36.7 / 36.3 / 38.7; one sequence x 8 at 513 keys 4 / 9:
+// 5.5 / 5.7.  At most kJoinMaxParts chunks.
 static int q8_chunk_keys(size_t n_seq, size_t n_kv, size_t max_len, size_t head_dim) {
     const size_t kt = (size_t)q8_tile_keys((int)head_dim);
-    const size_t tiles = (max_len + kt - 1) / kt;
-    const size_t target = (size_t)num_sms() * 3 * 5;
-    size_t per_cta = (n_seq * n_kv * tiles + target - 1) / target;
-    const size_t min_tiles = kQ8Warps * (n_seq * n_kv >= (size_t)num_sms() ? 4 : 1);
-    if (per_cta < min_tiles) per_cta = min_tiles;
+    const size_t tiles = (max_len + kt - 1) / kt, pairs = n_seq * n_kv;
+    const size_t slots = (size_t)num_sms() * kQ8CtasPerSm;
+    size_t least = pairs * tiles / slots;
+    least = least < 4 ? 4 : least > 16 ? 16 : least;
+    size_t per_cta = (pairs * tiles + 5 * slots - 1) / (5 * slots);
+    if (per_cta < least) per_cta = least;
+    if (pairs >= (size_t)num_sms() && tiles <= 24) per_cta = tiles;
     if (per_cta * kJoinMaxParts < tiles) per_cta = (tiles + kJoinMaxParts - 1) / kJoinMaxParts;
     if (per_cta > tiles) per_cta = tiles;
     if (per_cta < 1) per_cta = 1;
@@ -281,14 +289,14 @@ static int launch_q8_tensor(kvb_stream_t stream, Q8DecodeArgs& a, size_t n_seq, 
     a.ws = split ? static_cast<float*>(ws) : nullptr;
     // Small split grids fold their chunks through a cluster, as kvb_attention_decode does.
     a.fold = a.max_chunks >= 2 && a.max_chunks <= 8 &&
-             n_kv * n_seq * a.max_chunks <= (size_t)num_sms() * 3;
+             n_kv * n_seq * a.max_chunks <= (size_t)num_sms() * kQ8CtasPerSm;
     auto* kernel = attn_decode_q8_kernel<T, kFmt, HD, NT>;
-    set_max_smem(kernel, kQ8SmemBytes);
+    set_max_smem(kernel, q8_smem_bytes(HD, NT));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = a.fold ? dim3((unsigned)a.max_chunks, (unsigned)n_kv, (unsigned)n_seq)
                          : dim3((unsigned)n_kv, (unsigned)n_seq, (unsigned)a.max_chunks);
     cfg.blockDim = dim3(kQ8Warps * 32);
-    cfg.dynamicSmemBytes = kQ8SmemBytes;
+    cfg.dynamicSmemBytes = q8_smem_bytes(HD, NT);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
