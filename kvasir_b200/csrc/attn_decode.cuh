@@ -69,7 +69,7 @@ struct DecodeArgs {
     int kv_ready;
     // Partial form (kPart, kvb_attention_decode_shared): keys [key0, lens[b]), key0 a multiple
     // of 64; every chunk's state goes to the workspace as part part0 + chunk of max_parts.
-    int key0 = 0, part0 = 0, max_parts = 0;
+    int key0 = 0, part0 = 0, max_parts = 0, part_floats = 0;
 };
 
 // First row (of 64 elements) of the 64-key tile starting at key kt0 (a multiple of
@@ -410,7 +410,7 @@ __device__ __forceinline__ void decode_chunk(const CUtensorMap& kmap, const CUte
     __syncthreads();
     float* wsb = nullptr;
     if (kPart)
-        wsb = a.ws + (((size_t)b * a.n_kv + kvh) * a.max_parts + a.part0 + chunk) * (size_t)G * 66;
+        wsb = a.ws + (((size_t)b * a.n_kv + kvh) * a.max_parts + a.part0 + chunk) * (size_t)a.part_floats;
     else if (n_chunks > 1)
         wsb = fold ? fold : a.ws + (((size_t)b * a.n_kv + kvh) * a.max_chunks + chunk) * (size_t)G * 66;
     for (int i = threadIdx.x; i < G * 64; i += blockDim.x) {
@@ -457,10 +457,7 @@ __device__ __forceinline__ void decode_chunk(const CUtensorMap& kmap, const CUte
 // place of the workspace and the combine pass.  For small grids, where every
 // cluster is resident at once.  Every CTA of a cluster with keys passes both
 // cluster barriers; a cluster of an empty sequence passes none.
-// kPart: launched as a programmatic dependent of the prefix's kernel, from which it reads
-// nothing (everything before that kernel has completed when it starts); it waits for it
-// only before it ends, so that the join pass after this grid finds both kernels' parts.
-template <typename T, bool kRope, bool kPart = false>
+template <typename T, bool kRope>
 __global__ void __launch_bounds__(128, 3) attn_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                                                              const __grid_constant__ CUtensorMap vmap,
                                                              DecodeArgs a) {
@@ -469,18 +466,13 @@ __global__ void __launch_bounds__(128, 3) attn_decode_kernel(const __grid_consta
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~uintptr_t(1023));
     asm volatile("griddepcontrol.launch_dependents;");
-    if (!kPart && !a.kv_ready) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!a.kv_ready) asm volatile("griddepcontrol.wait;" ::: "memory");
     const int slot = a.fold ? (int)blockIdx.x : (int)blockIdx.z;
     const int kvh = a.fold ? (int)blockIdx.y : (int)blockIdx.x;
     const int b = a.fold ? (int)blockIdx.z : (int)blockIdx.y;
     const int from_end = a.max_chunks - 1 - slot;
     float* st = reinterpret_cast<float*>(smem + kDecWarps * 2 * kDecTileBytes);  // [G][66]
-    decode_chunk<T, kRope, kPart>(kmap, vmap, a, smem, bars, kvh, b, from_end,
-                                  !kPart && a.fold ? st : nullptr);
-    if (kPart) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        return;
-    }
+    decode_chunk<T, kRope, false>(kmap, vmap, a, smem, bars, kvh, b, from_end, a.fold ? st : nullptr);
     if (!a.fold) return;
     const int G = a.group;
     const int len = decode_len(a, b);
@@ -506,6 +498,28 @@ __global__ void __launch_bounds__(128, 3) attn_decode_kernel(const __grid_consta
         }
     }
     cluster_sync();  // no CTA leaves while the fold may still read its state
+}
+
+// The partial form (DecodeArgs::key0), grid (kv head, sequence, chunk slot): the own keys of
+// kvb_attention_decode_shared.  Launched as a programmatic dependent of the prefix's kernel,
+// from which it reads nothing (everything before that kernel has completed when it starts).
+// Only the grid's last CTA waits for it, before it ends: the grid then completes after the
+// prefix's kernel, and the join pass after it finds both kernels' parts, while the other CTAs
+// leave their slots at once and run beside the prefix's.  152 registers: beside a prefix CTA of four groups (576 threads x 80), one
+// CTA of this kernel fills the SM's register file.
+template <typename T>
+__global__ void __maxnreg__(152) attn_decode_part_kernel(const __grid_constant__ CUtensorMap kmap,
+                                                         const __grid_constant__ CUtensorMap vmap,
+                                                         DecodeArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[2 * kDecWarps];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                               ~uintptr_t(1023));
+    asm volatile("griddepcontrol.launch_dependents;");
+    decode_chunk<T, false, true>(kmap, vmap, a, smem, bars, blockIdx.x, blockIdx.y,
+                                 a.max_chunks - 1 - (int)blockIdx.z, nullptr);
+    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1)
+        asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // Folds the per-chunk partials of every (sequence, kv head) with more than one chunk.

@@ -40,6 +40,10 @@ __host__ __device__ constexpr int q8_smem_bytes(int hd, int nt) {
     return kQ8TilesBytes + kQ8ScaleBytes + 8 * nt * hd * 4 + 1024;
 }
 
+// Floats of one part of the workspace (O, m, l of a group), a multiple of four.
+__host__ __device__ constexpr int q8_part_floats(int group, int hd) {
+    return (group * (hd + 2) + 3) / 4 * 4;
+}
 __host__ __device__ constexpr int q8_tile_keys(int hd) { return kQ8TileBytes / hd; }
 
 struct Q8DecodeArgs {
@@ -50,7 +54,7 @@ struct Q8DecodeArgs {
     float scale_log2;
     uint16_t* out;
     long long out_row_stride;
-    float* ws;       // split partials: per part O[group][hd], m[group], l[group]
+    float* ws;       // split partials: per part O[group][hd], m[group], l[group], padding
     int chunk_keys;  // keys per CTA, a multiple of kQ8Warps tiles
     int max_chunks;
     int fold;        // chunks of a (sequence, KV head) folded through a cluster
@@ -522,7 +526,7 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
         if (n_chunks > 1) {
             wsb = a.fold ? fold_o
                          : a.ws + (((size_t)b * a.c.n_kv + kvh) * a.max_chunks + chunk) *
-                                      (size_t)(G * (HD + 2));
+                                      (size_t)q8_part_floats(G, HD);
             mlb = a.fold ? &fold_ml[0][0] : wsb + G * HD;
         }
         const int ml_step = a.fold ? kQ8MaxGroup : G;
@@ -554,9 +558,8 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
                 outb[i + 1] = Elem<T>::from_f(O.y * inv);
                 outb[i + 2] = Elem<T>::from_f(O.z * inv);
                 outb[i + 3] = Elem<T>::from_f(O.w * inv);
-            } else {  // 8-byte stores: a part of G (HD + 2) floats starts at a multiple of 8 bytes
-                *reinterpret_cast<float2*>(wsb + i) = make_float2(O.x, O.y);
-                *reinterpret_cast<float2*>(wsb + i + 2) = make_float2(O.z, O.w);
+            } else {
+                *reinterpret_cast<float4*>(wsb + i) = O;
                 if (i % HD == 0) {
                     mlb[r] = M;
                     mlb[ml_step + r] = L;
@@ -588,14 +591,15 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
 // Joins the partial states of every (sequence, KV head): parts 0 .. fixed - 1, which every
 // sequence has, then one for each chunk of its keys past key0.  Written rows: those with more
 // than one part (write_all: every row, zeros where a sequence has none).  A programmatic
-// dependent of the kernel that writes the partials.  The CTA first turns the parts' (m, l)
-// into weights in shared memory, then each thread sums its outputs over the parts with
-// coalesced loads: two rounds of memory latency.
+// dependent of the kernel that writes the partials.  Threads are laid out as (part, four
+// neighbouring outputs): each requests its first parts' O, 16 bytes a load, before the CTA
+// turns the parts' (m, l) into weights, so that both reads share one memory latency; the
+// threads of an output then add up through shared memory.  Parts start on 16 bytes.
 struct JoinArgs {
     const float* ws;
     const int32_t* lens;
     int max_len, key0, chunk_keys;
-    int fixed, max_parts;
+    int fixed, max_parts, part_floats;
     int n_kv, group, hd;
     int write_all;
     uint16_t* out;
@@ -603,10 +607,12 @@ struct JoinArgs {
 };
 constexpr int kJoinThreads = 256;
 constexpr int kJoinMaxParts = 512;  // weights: parts x group floats of shared memory
+constexpr int kJoinAhead = 4;       // parts whose O a thread requests ahead of the weights
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(JoinArgs a) {
     extern __shared__ float w[];  // [parts][group]
     __shared__ float inv_l[kQ8MaxGroup];
+    __shared__ float4 sums[kJoinThreads];
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int kvh = blockIdx.x, b = blockIdx.y, G = a.group, hd = a.hd;
@@ -615,8 +621,19 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(JoinArgs a) {
     const int parts = a.fixed + own;
     if (!a.write_all && parts <= 1) return;
     T* outb = reinterpret_cast<T*>(a.out) + (size_t)b * a.out_row_stride + (size_t)kvh * G * hd;
-    const size_t per = (size_t)G * (hd + 2);
+    const size_t per = (size_t)a.part_floats;
     const float* base = a.ws + ((size_t)b * a.n_kv + kvh) * a.max_parts * per;
+    const int cols = G * hd / 4;                          // groups of four outputs
+    const int lanes = max(1, kJoinThreads / cols);        // threads that share a column's parts
+    const int pl = threadIdx.x / cols;                    // this thread's (lanes > 1)
+    const bool busy = lanes == 1 || pl < lanes;
+    const int p0 = lanes == 1 ? 0 : pl, c0 = lanes == 1 ? threadIdx.x : threadIdx.x - pl * cols;
+    const float4* o4 = reinterpret_cast<const float4*>(base) + c0;
+    const size_t per4 = per / 4;
+    float4 ahead[kJoinAhead];
+#pragma unroll
+    for (int k = 0; k < kJoinAhead; ++k)
+        if (busy && c0 < cols && p0 + k * lanes < parts) ahead[k] = o4[(p0 + k * lanes) * per4];
     for (int r = threadIdx.x >> 5; r < G; r += kJoinThreads / 32) {  // a warp per head
         const int lane = threadIdx.x & 31;
         float M = -INFINITY, L = 0.f;
@@ -632,16 +649,52 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(JoinArgs a) {
         if (lane == 0) inv_l[r] = L == 0.f ? 0.f : 1.f / L;  // no keys at all: zeros
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < G * hd; i += kJoinThreads) {
-        const int r = i / hd;
-        float O = 0.f;
-#pragma unroll 8
-        for (int p = 0; p < parts; ++p) {
-            // a part without weight may hold anything (0 * NaN where every key was masked)
-            const float wp = w[p * G + r], op = base[p * per + i];
-            O += wp == 0.f ? 0.f : op * wp;
+    // a part without weight may hold anything (0 * NaN where every key was masked)
+    auto add = [](float4& x, const float4& o, float f) {
+        if (f == 0.f) return;
+        x.x += o.x * f;
+        x.y += o.y * f;
+        x.z += o.z * f;
+        x.w += o.w * f;
+    };
+    auto store = [&](int c, const float4& x) {
+        const float f = inv_l[4 * c / hd];
+        outb[4 * c] = Elem<T>::from_f(x.x * f);
+        outb[4 * c + 1] = Elem<T>::from_f(x.y * f);
+        outb[4 * c + 2] = Elem<T>::from_f(x.z * f);
+        outb[4 * c + 3] = Elem<T>::from_f(x.w * f);
+    };
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (busy && c0 < cols) {
+        const int r = 4 * c0 / hd;
+#pragma unroll
+        for (int k = 0; k < kJoinAhead; ++k)
+            if (p0 + k * lanes < parts) add(x, ahead[k], w[(p0 + k * lanes) * G + r]);
+#pragma unroll 4
+        for (int p = p0 + kJoinAhead * lanes; p < parts; p += lanes) add(x, o4[p * per4], w[p * G + r]);
+    }
+    if (lanes == 1) {
+        if (c0 < cols) store(c0, x);
+        for (int c = c0 + kJoinThreads; c < cols; c += kJoinThreads) {  // more columns than threads
+            x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (int p = 0; p < parts; ++p)
+                add(x, reinterpret_cast<const float4*>(base)[p * per4 + c], w[p * G + 4 * c / hd]);
+            store(c, x);
         }
-        outb[i] = Elem<T>::from_f(O * inv_l[r]);
+        return;
+    }
+    sums[threadIdx.x] = x;
+    __syncthreads();
+    if (pl == 0) {
+        for (int k = 1; k < lanes; ++k) {
+            const float4 y = sums[k * cols + c0];
+            x.x += y.x;
+            x.y += y.y;
+            x.z += y.z;
+            x.w += y.w;
+        }
+        store(c0, x);
     }
 }
 

@@ -251,7 +251,9 @@ static size_t q8_ws_bytes(size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
     if (!q8_tensor_shape(head_dim, n_q, n_kv) || max_len == 0) return 0;
     const size_t ck = (size_t)q8_chunk_keys(n_seq, n_kv, max_len, head_dim);
     const size_t chunks = (max_len + ck - 1) / ck;
-    return chunks <= 1 ? 0 : n_seq * chunks * n_q * (head_dim + 2) * sizeof(float);
+    return chunks <= 1 ? 0
+                       : n_seq * n_kv * chunks * q8_part_floats((int)(n_q / n_kv), (int)head_dim) *
+                             sizeof(float);
 }
 
 static int launch_join(kvb_stream_t stream, const JoinArgs& a, size_t n_seq, int dtype) {
@@ -318,6 +320,7 @@ static int launch_q8_tensor(kvb_stream_t stream, Q8DecodeArgs& a, size_t n_seq, 
     j.chunk_keys = a.chunk_keys;
     j.fixed = 0;
     j.max_parts = a.max_chunks;
+    j.part_floats = q8_part_floats(a.group, HD);
     j.n_kv = a.c.n_kv;
     j.group = a.group;
     j.hd = HD;
@@ -362,27 +365,42 @@ static int launch_q8_decode(kvb_stream_t stream, const GeneralDecodeArgs& a, con
                         : launch_q8_tensor<T, kFmt, 128, 2>(stream, d, n_seq, cache_rows, ws, ws_len);
 }
 
-// How a shared-prefix call runs on the tensor-core kernels: the prefix's 96-key tiles dealt to
-// `splits` slices, the own keys in chunks.  Slices: the number that takes the least time by
-// waves of two CTAs per SM x (tiles of the longest slice + ~4 tiles of start and end).
+// How a shared-prefix call runs on the tensor-core kernels: the prefix's 64-key tiles dealt to
+// `splits` slices, the sequences' rows to tiles of which a CTA takes `groups`, the own keys in
+// chunks.
 struct SharedPlan {
     int key0;  // keys computed for all sequences at once
-    int seqs_per_tile, row_tiles, n_tiles, splits;
-    int chunk_keys, max_chunks;
+    int seqs_per_tile, row_tiles, groups, n_tiles, splits;
+    int chunk_keys, max_chunks, part_floats;
     size_t ws_bytes;
 };
 static SharedPlan shared_plan(size_t n_seq, size_t prefix, size_t max_own, size_t n_q, size_t n_kv) {
     SharedPlan p;
     const size_t group = n_q / n_kv;
     p.key0 = (int)prefix;
-    p.seqs_per_tile = (int)(kPfRows / group);
+    p.seqs_per_tile = (int)(kSpRows / group);
     p.row_tiles = (int)((n_seq + p.seqs_per_tile - 1) / p.seqs_per_tile);
-    p.n_tiles = (int)((prefix + kPfKeys - 1) / kPfKeys);
+    p.n_tiles = (int)((prefix + kSpKeys - 1) / kSpKeys);
+    p.groups = p.row_tiles >= 3 ? 4 : p.row_tiles;
     p.splits = 0;
-    const size_t slots = (size_t)num_sms() * kPfCtasPerSm, pairs = (size_t)p.row_tiles * n_kv;
-    size_t best = ~(size_t)0;
+    // Slices: the number that takes the least time by a model fitted on B200 (us): a slice takes
+    // 1.45 per 64-key tile however many of the four groups an SM holds are busy, and about four
+    // tiles more to start and end; all slices and the own keys (half of the worst case, at 4.5
+    // TB/s) share the SMs, and a fifth of a slice's time is not covered by the own keys; a
+    // slice adds its rows' partials (264 bytes written and read, ~3
+    // TB/s) to the join.  32 sequences, 4096 keys, by slices 4 / 8 / 16 / 32: 33 / 22 / 18 / 23
+    // us; 256 sequences, 16384 keys, up to 1000 own, 4 / 6 / 12 / 24: 128 / 106 / 120 / 144.
+    const double slots = (double)num_sms() * (kSpMaxGroups / p.groups);
+    const double pairs = (double)((p.row_tiles + p.groups - 1) / p.groups) * (double)n_kv;
+    const double own_us = 0.5 * (double)n_seq * (double)max_own * (double)n_kv * 256.0 / 4.5e6;
+    const double join_us = 0.05 + (double)n_seq * (double)n_q * 264.0 * 2.0 / 3.0e6;
+    double best = 1e30;
     for (int s = 1; s <= p.n_tiles && s <= 64; ++s) {
-        const size_t cost = ((pairs * s + slots - 1) / slots) * ((size_t)(p.n_tiles + s - 1) / s + 4);
+        const double slice = 1.45 * ((p.n_tiles + s - 1) / s + 4);
+        const double waves = (double)(size_t)((pairs * s + slots - 1) / slots);
+        const double share = pairs * s * slice / slots + own_us;
+        const double cost =
+            (share > waves * slice ? share : waves * slice) + 0.2 * slice + s * join_us;
         if (cost < best) {
             best = cost;
             p.splits = s;
@@ -393,8 +411,21 @@ static SharedPlan shared_plan(size_t n_seq, size_t prefix, size_t max_own, size_
     if ((max_own + ck - 1) / ck > most) ck = ((max_own + most - 1) / most + 255) / 256 * 256;
     p.chunk_keys = (int)ck;
     p.max_chunks = (int)((max_own + ck - 1) / ck);
-    p.ws_bytes = n_seq * n_q * (size_t)(p.splits + p.max_chunks) * 66 * sizeof(float);
+    p.part_floats = q8_part_floats((int)group, 64);
+    p.ws_bytes = n_seq * n_kv * (size_t)(p.splits + p.max_chunks) * p.part_floats * sizeof(float);
     return p;
+}
+
+template <typename T, int kGroups>
+static int launch_shared_prefix(kvb_stream_t stream, const CUtensorMap& qmap, const CUtensorMap& kmap,
+                                const CUtensorMap& vmap, const SharedPrefixArgs& s) {
+    auto* kernel = attn_shared_prefix_kernel<T, kGroups>;
+    set_max_smem(kernel, sp_smem_bytes(kGroups));
+    const dim3 grid((unsigned)s.n_kv, (unsigned)s.splits,
+                    (unsigned)((s.row_tiles + kGroups - 1) / kGroups));
+    kernel<<<grid, sp_threads(kGroups), sp_smem_bytes(kGroups), stream>>>(qmap, kmap, vmap, s);
+    KVB_CHECK_LAUNCH("attention_decode_shared prefix launch");
+    return KVB_OK;
 }
 
 template <typename T>
@@ -418,13 +449,13 @@ static int launch_shared_tensor(kvb_stream_t stream, const GeneralDecodeArgs& a,
         int st;
         if (paged) {
             const uint64_t dims[2] = {64, total_rows}, strides[1] = {128};
-            const uint32_t box[2] = {64, (uint32_t)kPfPagedPiece};
+            const uint32_t box[2] = {64, (uint32_t)kSpKeys};
             st = encode_tmap(&kmap, src.kc, 2, dims, strides, box, dtype);
             if (!st) st = encode_tmap(&vmap, src.vc, 2, dims, strides, box, dtype);
         } else {
             const uint64_t dims[3] = {64, (uint64_t)p.key0, (uint64_t)a.n_kv};
             const uint64_t strides[2] = {128, (uint64_t)src.prefix_rows * 128};
-            const uint32_t box[3] = {64, (uint32_t)kPfKeys, 1};
+            const uint32_t box[3] = {64, (uint32_t)kSpKeys, 1};
             st = encode_tmap(&kmap, src.pk, 3, dims, strides, box, dtype);
             if (!st) st = encode_tmap(&vmap, src.pv, 3, dims, strides, box, dtype);
         }
@@ -434,6 +465,7 @@ static int launch_shared_tensor(kvb_stream_t stream, const GeneralDecodeArgs& a,
         s.n_kv = a.n_kv;
         s.group = group;
         s.seqs_per_tile = p.seqs_per_tile;
+        s.row_tiles = p.row_tiles;
         s.prefix = p.key0;
         s.n_tiles = p.n_tiles;
         s.splits = p.splits;
@@ -442,14 +474,14 @@ static int launch_shared_tensor(kvb_stream_t stream, const GeneralDecodeArgs& a,
         s.max_len = a.max_len;
         s.ws = ws;
         s.max_parts = max_parts;
+        s.part_floats = p.part_floats;
         s.block_table = src.block_table;
         s.block_size = src.block_size;
         s.n_blocks = src.n_blocks;
-        set_max_smem(attn_shared_prefix_kernel<T>, kPfSmemBytes);
-        attn_shared_prefix_kernel<T>
-            <<<dim3((unsigned)a.n_kv, (unsigned)p.splits, (unsigned)p.row_tiles), kPfThreads,
-               kPfSmemBytes, stream>>>(qmap, kmap, vmap, s);
-        KVB_CHECK_LAUNCH("attention_decode_shared prefix launch");
+        st = p.groups == 4   ? launch_shared_prefix<T, 4>(stream, qmap, kmap, vmap, s)
+             : p.groups == 2 ? launch_shared_prefix<T, 2>(stream, qmap, kmap, vmap, s)
+                             : launch_shared_prefix<T, 1>(stream, qmap, kmap, vmap, s);
+        if (st) return st;
     }
     if (p.max_chunks > 0) {
         CUtensorMap kmap, vmap;
@@ -478,7 +510,8 @@ static int launch_shared_tensor(kvb_stream_t stream, const GeneralDecodeArgs& a,
         d.key0 = paged ? p.key0 : 0;
         d.part0 = p.splits;
         d.max_parts = max_parts;
-        auto* kernel = attn_decode_kernel<T, false, true>;
+        d.part_floats = p.part_floats;
+        auto* kernel = attn_decode_part_kernel<T>;
         set_max_smem(kernel, kDecSmemBytes);
         const dim3 grid((unsigned)a.n_kv, (unsigned)n_seq, (unsigned)p.max_chunks);
         cudaError_t e;
@@ -498,6 +531,7 @@ static int launch_shared_tensor(kvb_stream_t stream, const GeneralDecodeArgs& a,
     j.chunk_keys = p.chunk_keys;
     j.fixed = p.splits;
     j.max_parts = max_parts > 0 ? max_parts : 1;
+    j.part_floats = p.part_floats;
     j.n_kv = a.n_kv;
     j.group = group;
     j.hd = 64;
@@ -513,7 +547,7 @@ template <typename T>
 static int launch_shared(kvb_stream_t stream, const GeneralDecodeArgs& a, const SharedSource<T>& src,
                          size_t n_seq, size_t own_rows, void* ws, size_t ws_len) {
     const bool paged = src.block_table != nullptr;
-    if (a.hd == 64 && a.n_q / a.n_kv <= kQ8MaxGroup && a.q_row_stride % 8 == 0 && aligned(a.q, 16) &&
+    if (a.hd == 64 && a.n_q / a.n_kv <= kQ8MaxGroup && a.scale_log2 >= 0.f && a.q_row_stride % 8 == 0 && aligned(a.q, 16) &&
         aligned(src.kc, 16) && aligned(src.vc, 16) && aligned(src.pk, 16) && aligned(src.pv, 16) &&
         n_seq <= 65535 && a.n_kv <= 65535 && ws != nullptr && aligned(ws, 16) &&
         (paged ? src.block_size % 64 == 0 &&
