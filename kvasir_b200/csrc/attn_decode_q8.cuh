@@ -5,15 +5,20 @@
 // tiles of 64 keys (head_dim 128: 32), 4 KB of K codes and 4 KB of V codes.  The transposed products put the keys on the MMA's 16-row
 // side and the group's heads on its 8-column side, so a group of up to 8 heads wastes no
 // rows and takes half the instructions of a 16-row query tile:
-//   S^T = K Q^T    m16n8k16, A = K codes as f16 (ldmatrix; a lane's four bytes are four
-//                  neighbouring dims, so the K side of the product runs over the dims in
-//                  the order (4c, 4c+1 | 4c+2, 4c+3), and Q's fragments are loaded so)
+//   S^T = K Q^T    A = K codes through ldmatrix (a lane's four bytes are four neighbouring
+//                  dims, so that Q's fragments are loaded in that order).  int8: m16n8k32 on the
+//                  codes as they are, Q as 16-bit integers in two signed bytes.  e4m3: m16n8k16 on
+//                  the codes turned into f16 (exact), Q in f16
 //   O^T += V^T P^T m16n8k16, A = V codes as f16 (ldmatrix.trans moves byte pairs: row g of
 //                  a tile is dim 2g and row g + 8 is dim 2g + 1), B = P through movmatrix
-// Codes are exact in f16: int8 through the bytes of 1024 + 128 + code, e4m3 by cvt.  The
+// int8 codes become f16 through the bytes of 1024 + 128 + code, e4m3 by cvt; both exact.  The
 // K scale multiplies the f32 score of its key; the V scale multiplies the key's weight.
+// The board's power limit, not HBM, sets the pace of long runs (int8 through f16 for K too:
+// 785 us a pass of 256 x 16384 keys at 1470 MHz, 669 us in a burst), so instructions count.
 //
-// Precision.  Q: f16 as it is; bf16 scaled by a power of two to a largest element in
+// Precision.  Q, int8: round(q * 32639 / max |q|) of the head, in 256 hi + lo, so each element
+// is within 1.6e-5 of the head's largest; the products are summed exactly (below 2^31 for
+// 128 dims).  Q, e4m3: f16 as it is; bf16 scaled by a power of two to a largest element in
 // [2^14, 2^15) and rounded to f16, which is exact for elements down to 2^-31 of the
 // largest.  Weights: w = p * v_scale * 2^n, n such that the largest V scale seen makes
 // w < 2^14, rounded once to f16 (half a step, 2^-11 of a weight; steps of 2^-24 below
@@ -98,17 +103,10 @@ __device__ __forceinline__ uint32_t biased_to_f16x2(uint32_t u, uint32_t sel) {
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(0x64806480u));
     return r;
 }
-// Four codes -> f16 pairs (bytes 0, 1) and (2, 3).
-template <int kFmt>
+// Four e4m3 codes -> f16 pairs (bytes 0, 1) and (2, 3).
 __device__ __forceinline__ void codes_pairs(uint32_t v, uint32_t& p01, uint32_t& p23) {
-    if (kFmt == KVB_KV_INT8) {
-        const uint32_t u = v ^ 0x80808080u;
-        p01 = biased_to_f16x2(u, 0x4140u);
-        p23 = biased_to_f16x2(u, 0x4342u);
-    } else {
-        p01 = e4m3x2_to_f16x2(v);
-        p23 = e4m3x2_hi_to_f16x2(v);
-    }
+    p01 = e4m3x2_to_f16x2(v);
+    p23 = e4m3x2_hi_to_f16x2(v);
 }
 // Four codes -> f16 pairs (bytes 0, 2) and (1, 3).
 template <int kFmt>
@@ -122,6 +120,20 @@ __device__ __forceinline__ void codes_evens_odds(uint32_t v, uint32_t& p02, uint
         p02 = e4m3x2_to_f16x2(u);
         p13 = e4m3x2_hi_to_f16x2(u);
     }
+}
+// D (s32) += A (16 x 32, s8) B (32 x 8, s8)
+__device__ __forceinline__ void mma_s8(int* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                       uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9},"
+        " {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Low bytes of four integers, in order.
+__device__ __forceinline__ uint32_t bytes4(int a, int b, int c, int d) {
+    return prmt(prmt((uint32_t)a, (uint32_t)b, 0x0040u), prmt((uint32_t)c, (uint32_t)d, 0x0040u),
+                0x5410u);
 }
 __device__ __forceinline__ uint32_t movmatrix_t(uint32_t v) {
     uint32_t r;
@@ -271,7 +283,8 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
             }
         }
 
-        // Q fragments (B operand): column g = head 8 nt + g, dims 16 j + 4c .. + 3.
+        // Q fragments (B operand): column g = head 8 nt + g, dims 16 j + 4c .. + 3.  int8: the
+        // high bytes, then the low ones; e4m3: two f16 pairs.
         uint32_t qf[DT][NT][2];
         float qs[NT][2];  // score factor of heads 8 nt + 2c, + 1
 #pragma unroll
@@ -284,7 +297,29 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
             for (int j = 0; j < DT; ++j)
                 v[j] = h < G ? *reinterpret_cast<const uint2*>(qr + 16 * j + 4 * c) : make_uint2(0u, 0u);
             float f = a.scale_log2;
-            if (Elem<T>::kDtype == KVB_BF16) {
+            if (kFmt == KVB_KV_INT8) {
+                uint32_t mx = 0;  // the head's largest magnitude, as a bit pattern
+#pragma unroll
+                for (int j = 0; j < DT; ++j) {
+                    const float2 x = Elem<T>::unpack(v[j].x), y = Elem<T>::unpack(v[j].y);
+                    mx = max(max(mx, max(abs_bits(x.x), abs_bits(x.y))),
+                             max(abs_bits(y.x), abs_bits(y.y)));
+                }
+                mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                const float big = fmaxf(__uint_as_float(mx), 0x1p-100f);
+                const float up = __fdiv_rn(32639.f, big);
+                // a NaN or an infinity among the elements: every score of the head is NaN
+                f = mx < 0x7f800000u ? f * __fdiv_rn(big, 32639.f) : __uint_as_float(0x7fc00000u);
+#pragma unroll
+                for (int j = 0; j < DT; ++j) {
+                    const float2 x = Elem<T>::unpack(v[j].x), y = Elem<T>::unpack(v[j].y);
+                    const int i0 = __float2int_rn(x.x * up), i1 = __float2int_rn(x.y * up);
+                    const int i2 = __float2int_rn(y.x * up), i3 = __float2int_rn(y.y * up);
+                    v[j].x = bytes4((i0 + 128) >> 8, (i1 + 128) >> 8, (i2 + 128) >> 8, (i3 + 128) >> 8);
+                    v[j].y = bytes4(i0, i1, i2, i3);  // i - 256 hi, in -128 .. 127
+                }
+            } else if (Elem<T>::kDtype == KVB_BF16) {
                 uint32_t mx = 0;  // largest exponent of the head's elements
 #pragma unroll
                 for (int j = 0; j < DT; ++j)
@@ -347,20 +382,42 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
             float s[MT][NT][4];
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
+                const int r = 16 * t + (lane & 15);
+                if (kFmt == KVB_KV_INT8) {
+                    int hi[NT][4], lo[NT][4];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) hi[nt][e] = lo[nt][e] = 0;
+#pragma unroll
+                    for (int j = 0; j < DT; j += 2) {
+                        uint32_t w0, w1, w2, w3;
+                        ldsm_x4(kb + q8_smem_off<HD>(r, j + (lane >> 4)), w0, w1, w2, w3);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma_s8(hi[nt], w0, w1, w2, w3, qf[j][nt][0], qf[j + 1][nt][0]);
+                            mma_s8(lo[nt], w0, w1, w2, w3, qf[j][nt][1], qf[j + 1][nt][1]);
+                        }
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[t][nt][e] = (float)(hi[nt][e] * 256 + lo[nt][e]);
+                    continue;
+                }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) s[t][nt][0] = s[t][nt][1] = s[t][nt][2] = s[t][nt][3] = 0.f;
-                const int r = 16 * t + (lane & 15);
 #pragma unroll
                 for (int j = 0; j < DT; j += 2) {
                     uint32_t w0, w1, w2, w3, af[4];
                     ldsm_x4(kb + q8_smem_off<HD>(r, j + (lane >> 4)), w0, w1, w2, w3);
-                    codes_pairs<kFmt>(w0, af[0], af[2]);
-                    codes_pairs<kFmt>(w1, af[1], af[3]);
+                    codes_pairs(w0, af[0], af[2]);
+                    codes_pairs(w1, af[1], af[3]);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
                         mma_16816<__half>(s[t][nt], af, qf[j][nt][0], qf[j][nt][1]);
-                    codes_pairs<kFmt>(w2, af[0], af[2]);
-                    codes_pairs<kFmt>(w3, af[1], af[3]);
+                    codes_pairs(w2, af[0], af[2]);
+                    codes_pairs(w3, af[1], af[3]);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
                         mma_16816<__half>(s[t][nt], af, qf[j + 1][nt][0], qf[j + 1][nt][1]);

@@ -68,24 +68,32 @@ def page(rng, x, block, spare=3, table=None):
 
 def attention(q, k, v, scale):
     """One KV head in f64: q [G, hd], k and v [n, hd] -> (out [G, hd], sum_k p_k |v_k|,
-    the largest sum_d |q_d k_d| * scale of each row).  No keys: zeros."""
+    the largest sum_d |q_d k_d| * scale of each row, the largest |q_d| sum_d |k_d| * scale).
+    No keys: zeros."""
     if k.shape[0] == 0:
         z = np.zeros(q.shape)
-        return z, z, np.zeros(q.shape[0])
+        return z, z, np.zeros(q.shape[0]), np.zeros(q.shape[0])
     s = q @ k.T * scale
     p = np.exp(s - s.max(-1, keepdims=True))
     p /= p.sum(-1, keepdims=True)
-    return p @ v, p @ np.abs(v), (np.abs(q) @ np.abs(k).T * scale).max(-1)
+    return (p @ v, p @ np.abs(v), (np.abs(q) @ np.abs(k).T * scale).max(-1),
+            np.abs(q).max(-1) * np.abs(k).sum(-1).max() * scale)
 
 
-def check_attention(got, q, kv_of, n_kv, scale, dtype, weight_eps, name=""):
+# An int8 cache's scores use Q as 16-bit integers, 32639 for a head's largest element: each
+# element is off by at most half an integer (and the f32 steps of the scaling).
+Q_EPS = {"int8": 0.5 / 32639 * (1 + 2.0 ** -6), "e4m3": 0.0}
+
+
+def check_attention(got, q, kv_of, n_kv, scale, dtype, weight_eps, name="", q_eps=0.0):
     """got [n_seq, n_q * hd] (16-bit) against f64; kv_of(b, h) -> (k, v) rows in f64.
 
     Bound per element, o the exact value and A = sum_k p_k |v_k|:
       half a step of the output type            eps / 2 * |o|  (and its smallest step)
       weights rounded to weight_eps each        weight_eps * A
       scores summed in f32 over hd terms: each off by d <= (hd + 4) 2^-24 max_k sum|q k| scale,
-        which moves a normalised weight by at most exp(2 d) - 1
+        which moves a normalised weight by at most exp(2 d) - 1; d also has q_eps max |q| sum |k|
+        scale for elements of q that are each off by q_eps of the head's largest
       exp and the sums over up to 2^11 terms in a row: 2^-13 * A
     """
     n_seq, hd = q.shape[0], q.shape[-1]
@@ -96,8 +104,8 @@ def check_attention(got, q, kv_of, n_kv, scale, dtype, weight_eps, name=""):
     for b in range(n_seq):
         for h in range(n_kv):
             k, v = kv_of(b, h)
-            o, A, s = attention(q[b, h * group:(h + 1) * group], k, v, scale)
-            d = (hd + 4) * 2.0 ** -24 * s[:, None]
+            o, A, s, s_max = attention(q[b, h * group:(h + 1) * group], k, v, scale)
+            d = (hd + 4) * 2.0 ** -24 * s[:, None] + q_eps * s_max[:, None]
             tol = fin.eps / 2 * np.abs(o) + fin.smallest_normal * fin.eps + A * (
                 weight_eps + np.expm1(2 * d) + 2.0 ** -13)
             err = np.abs(got[b, h] - o)

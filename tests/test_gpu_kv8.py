@@ -260,7 +260,7 @@ def test_decode_against_f64(g, n_q, n_kv, hd, block, fmt, dtype):
     out = _run_decode(g, q, cache, LENS, n_q, n_kv, hd, max_seq, fmt, dtype, block)
     assert g.device_error() == 0
     assert bool((out[0] == 0).all())  # no keys: zeros
-    R.check_attention(out, qf, kv_of, n_kv, R.default_scale(hd), dtype, W_EPS)
+    R.check_attention(out, qf, kv_of, n_kv, R.default_scale(hd), dtype, W_EPS, q_eps=R.Q_EPS[fmt])
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
@@ -276,7 +276,7 @@ def test_decode_splits_agree_with_f64(g, fmt, n_seq, n):
         again = _run_decode(g, q, cache, lens, n_q, n_kv, hd, max_seq, fmt, "bf16", workspace=ws)
         assert g.device_error() == 0
         assert torch.equal(out, again)
-        R.check_attention(out, qf, kv_of, n_kv, R.default_scale(hd), "bf16", W_EPS)
+        R.check_attention(out, qf, kv_of, n_kv, R.default_scale(hd), "bf16", W_EPS, q_eps=R.Q_EPS[fmt])
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
@@ -289,7 +289,7 @@ def test_decode_with_scales_of_many_magnitudes(g, fmt):
     rs = [2.0 ** rng.integers(-10, 3, shape), 2.0 ** rng.integers(-20, 5, shape)]
     q, qf, cache, kv_of, max_seq = _decode_case(rng, lens, n_q, n_kv, hd, fmt, "bf16", rs, q_std=4.0)
     out = _run_decode(g, q, cache, lens, n_q, n_kv, hd, max_seq, fmt, "bf16")
-    R.check_attention(out, qf, kv_of, n_kv, R.default_scale(hd), "bf16", W_EPS)
+    R.check_attention(out, qf, kv_of, n_kv, R.default_scale(hd), "bf16", W_EPS, q_eps=R.Q_EPS[fmt])
 
 
 @pytest.mark.parametrize("hd", [64, 128, 80])
@@ -491,5 +491,29 @@ def test_prefill_then_decode_steps_on_one_cache(g, fmt, block):
         kx, vx = exact_rows()
         qx = O.to_f32(host_bits(qkv)).astype(np.float64).reshape(n_seq, heads, hd)[:, :n_q]
         R.check_attention(step, qx, lambda b, h: (kx[b, h, :n], vx[b, h, :n]), n_kv,
-                          R.default_scale(hd), dtype, W_EPS, f"step {i}")
+                          R.default_scale(hd), dtype, W_EPS, f"step {i}", R.Q_EPS[fmt])
     assert g.device_error() == 0
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_decode_query_magnitudes(g, fmt, dtype):
+    """Heads of q from 2^-20 to 2^7 in magnitude, one of zeros, elements spread over 2^10 within
+    a head; a NaN and an infinity make their own head's row NaN and no other."""
+    rng = np.random.default_rng(31)
+    n_q, n_kv, hd, lens = 16, 2, 64, [300, 65]
+    q, qf, cache, kv_of, max_seq = _decode_case(rng, lens, n_q, n_kv, hd, fmt, dtype)
+    x = qf * 2.0 ** rng.integers(-10, 1, qf.shape) * 2.0 ** np.linspace(-20, 4, n_q)[None, :, None]
+    x[0, 5] = 0
+    q = O.from_f32(x.astype(np.float32).ravel(), dtype)
+    qf = O.to_f32(q, dtype).astype(np.float64).reshape(x.shape)
+    out = _run_decode(g, q, cache, lens, n_q, n_kv, hd, max_seq, fmt, dtype)
+    R.check_attention(out, qf, kv_of, n_kv, R.default_scale(hd), dtype, W_EPS, q_eps=R.Q_EPS[fmt])
+    x[0, 2, 7], x[1, 9, 0] = np.nan, np.inf
+    bad = _run_decode(g, O.from_f32(x.astype(np.float32).ravel(), dtype), cache, lens, n_q, n_kv, hd,
+                      max_seq, fmt, dtype).view(2, n_q, hd)
+    rows = torch.zeros(2, n_q, dtype=torch.bool)
+    rows[0, 2] = rows[1, 9] = True
+    assert torch.equal(bad.isnan().all(-1).cpu(), rows)
+    keep = ~rows.cuda()
+    assert torch.equal(bad[keep], out.view(2, n_q, hd)[keep])
