@@ -92,7 +92,7 @@ static int launch_kv8_append(kvb_stream_t stream, const Kv8AppendArgs& a, size_t
         aligned(a.sin_t, 16) && aligned(a.c.kc, 8) && aligned(a.c.vc, 8)) {
         const int cpr = a.c.hd / 16;
         const long long items = (long long)(a.n_q + 2 * a.c.n_kv) * cpr;
-        const unsigned threads = items >= 1024 ? 1024u : (unsigned)((items + 31) / 32 * 32);
+        const unsigned threads = items >= 256 ? 256u : (unsigned)((items + 31) / 32 * 32);
         if (cpr == 4) kv8_append_vec_kernel<T, kFmt, 4><<<(unsigned)rows, threads, 0, stream>>>(a);
         else kv8_append_vec_kernel<T, kFmt, 8><<<(unsigned)rows, threads, 0, stream>>>(a);
         KVB_CHECK_LAUNCH("rope_kv_append_q8 launch");

@@ -338,17 +338,15 @@ class Gpu:
         index = self.device.index
         if torch.cuda.current_device() != index:
             raise ShapeError(f"{name}: the current device is not {self.device}")
-        got = []
-        for t in tensors:
-            if t is None:
-                got.append(None)
-                continue
-            if t.get_device() != index:
-                raise ShapeError(f"{name}: a tensor is on {t.device}, not on {self.device}")
-            if not t.is_contiguous():
-                raise ShapeError(f"{name}: buffers must be contiguous")
-            got.append(t.data_ptr())
-        return got
+        return [t.data_ptr() if t is not None and t.get_device() == index and t.is_contiguous()
+                else self._no_ptr(name, t) for t in tensors]
+
+    def _no_ptr(self, name, t):
+        if t is None:
+            return None
+        if t.get_device() != self.device.index:
+            raise ShapeError(f"{name}: a tensor is on {t.device}, not on {self.device}")
+        raise ShapeError(f"{name}: buffers must be contiguous")
 
     @staticmethod
     def _check_types(name, dtype, *tensors):
