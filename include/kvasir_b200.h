@@ -565,6 +565,18 @@ int kvb_decoder_destroy(kvb_decoder_t dec);
  * the paged step; call it outside any stream capture. */
 int kvb_decoder_use_paged_cache(kvb_decoder_t dec, void* k_pools, void* v_pools, size_t pool_len,
                                 const int32_t* block_table, size_t max_blocks, size_t block_size);
+/* Switches the driver to an 8-bit KV cache (see kvb_rope_kv_append_q8): codes kc / vc
+ * [n_layers][n_seq][n_kv][max_seq][head_dim] and scales [n_layers][n_seq][n_kv]
+ * [max_seq], or pools as for kvb_decoder_use_paged_cache with scale pools [n_layers]
+ * [n_blocks][n_kv][block_size].  The caches given before are no longer used.  A step
+ * then runs kvb_rope_kv_append_q8(_paged) and kvb_attention_decode_q8(_paged) per
+ * layer; any head_dim up to 256, any block_size (multiples of 16 are fast).  The next
+ * step re-records its graph; call outside any stream capture. */
+int kvb_decoder_use_q8_cache(kvb_decoder_t dec, void* kc, void* vc, float* k_scales,
+                             float* v_scales, int kv_format);
+int kvb_decoder_use_q8_paged_cache(kvb_decoder_t dec, void* k_pools, void* v_pools, float* k_scales,
+                                   float* v_scales, size_t pool_len, const int32_t* block_table,
+                                   size_t max_blocks, size_t block_size, int kv_format);
 /* Sets the per-sequence cache fill (tokens already in the cache) from a host
  * array; the next step writes position cur_len[b]. */
 int kvb_decoder_set_lengths(kvb_decoder_t dec, kvb_stream_t stream, const int32_t* cur_len_host);

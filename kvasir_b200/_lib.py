@@ -104,6 +104,8 @@ SIGNATURES = {
                                   C.POINTER(DecoderWeights), _p, _p, _p, _p, _p, _sz]),
     "kvb_decoder_destroy": (_int, [_p]),
     "kvb_decoder_use_paged_cache": (_int, [_p, _p, _p, _sz, _p, _sz, _sz]),
+    "kvb_decoder_use_q8_cache": (_int, [_p, _p, _p, _p, _p, _int]),
+    "kvb_decoder_use_q8_paged_cache": (_int, [_p, _p, _p, _p, _p, _sz, _p, _sz, _sz, _int]),
     "kvb_decoder_set_lengths": (_int, [_p, _p, _p]),
     "kvb_decoder_ids_in": (_p, [_p]),
     "kvb_decoder_ids_out": (_p, [_p]),

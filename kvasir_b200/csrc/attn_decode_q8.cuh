@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 const int r = 16 * t + (lane & 15);
-                if (kFmt == KVB_KV_INT8) {
+                if constexpr (kFmt == KVB_KV_INT8) {
                     int hi[NT][4], lo[NT][4];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
@@ -403,24 +403,25 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[t][nt][e] = (float)(hi[nt][e] * 256 + lo[nt][e]);
-                    continue;
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) s[t][nt][0] = s[t][nt][1] = s[t][nt][2] = s[t][nt][3] = 0.f;
-#pragma unroll
-                for (int j = 0; j < DT; j += 2) {
-                    uint32_t w0, w1, w2, w3, af[4];
-                    ldsm_x4(kb + q8_smem_off<HD>(r, j + (lane >> 4)), w0, w1, w2, w3);
-                    codes_pairs(w0, af[0], af[2]);
-                    codes_pairs(w1, af[1], af[3]);
+                } else {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
-                        mma_16816<__half>(s[t][nt], af, qf[j][nt][0], qf[j][nt][1]);
-                    codes_pairs(w2, af[0], af[2]);
-                    codes_pairs(w3, af[1], af[3]);
+                        s[t][nt][0] = s[t][nt][1] = s[t][nt][2] = s[t][nt][3] = 0.f;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        mma_16816<__half>(s[t][nt], af, qf[j + 1][nt][0], qf[j + 1][nt][1]);
+                    for (int j = 0; j < DT; j += 2) {
+                        uint32_t w0, w1, w2, w3, af[4];
+                        ldsm_x4(kb + q8_smem_off<HD>(r, j + (lane >> 4)), w0, w1, w2, w3);
+                        codes_pairs(w0, af[0], af[2]);
+                        codes_pairs(w1, af[1], af[3]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma_16816<__half>(s[t][nt], af, qf[j][nt][0], qf[j][nt][1]);
+                        codes_pairs(w2, af[0], af[2]);
+                        codes_pairs(w3, af[1], af[3]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma_16816<__half>(s[t][nt], af, qf[j + 1][nt][0], qf[j + 1][nt][1]);
+                    }
                 }
             }
             // ---- scale and mask; element e: key 16 t + g + 8 (e >> 1), head 8 nt + 2c + (e & 1)

@@ -246,6 +246,8 @@ __device__ __forceinline__ uint32_t widen_bits(uint32_t h) {
 // the next row ahead (28.3).
 template <typename T, int kFmt, int CPR>
 __global__ void __launch_bounds__(256, 6) kv8_append_vec_kernel(Kv8AppendArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr int hd = 16 * CPR, half = 8 * CPR;
     const int row = blockIdx.x;
     const int seq = row / a.rows_per_seq;
@@ -349,6 +351,8 @@ __global__ void __launch_bounds__(128) kv8_read_general_kernel(Kv8ReadArgs a, lo
 // per 16 codes of a K row and the same codes of its V row.  blockIdx.y: (sequence, KV head).
 template <typename T, int kFmt>
 __global__ void __launch_bounds__(256) kv8_read_vec_kernel(Kv8ReadArgs a, int chunks_per_row) {
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int bh = blockIdx.y;
     const int b = bh / a.c.n_kv, kvh = bh - b * a.c.n_kv;
     const int it = blockIdx.x * 256 + threadIdx.x;

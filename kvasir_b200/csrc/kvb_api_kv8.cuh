@@ -93,10 +93,12 @@ static int launch_kv8_append(kvb_stream_t stream, const Kv8AppendArgs& a, size_t
         const int cpr = a.c.hd / 16;
         const long long items = (long long)(a.n_q + 2 * a.c.n_kv) * cpr;
         const unsigned threads = items >= 256 ? 256u : (unsigned)((items + 31) / 32 * 32);
-        if (cpr == 4) kv8_append_vec_kernel<T, kFmt, 4><<<(unsigned)rows, threads, 0, stream>>>(a);
-        else kv8_append_vec_kernel<T, kFmt, 8><<<(unsigned)rows, threads, 0, stream>>>(a);
-        KVB_CHECK_LAUNCH("rope_kv_append_q8 launch");
-        return KVB_OK;
+        const cudaError_t e =
+            cpr == 4 ? launch_pdl(kv8_append_vec_kernel<T, kFmt, 4>, dim3((unsigned)rows),
+                                  dim3(threads), 0, stream, a)
+                     : launch_pdl(kv8_append_vec_kernel<T, kFmt, 8>, dim3((unsigned)rows),
+                                  dim3(threads), 0, stream, a);
+        return e == cudaSuccess ? KVB_OK : cuda_fail(e, "rope_kv_append_q8 launch");
     }
     const long long items = (long long)rows * (a.n_q + 2 * a.c.n_kv);
     const long long grid = (items + 3) / 4;
@@ -142,9 +144,9 @@ static int launch_kv8_read(kvb_stream_t stream, const Kv8ReadArgs& a, size_t n_s
     if (a.c.hd % 16 == 0 && n_seq * a.c.n_kv <= 65535 && per_head <= 0x7fffff00ll &&
         aligned(a.c.kc, 16) && aligned(a.c.vc, 16) && aligned(a.k_out, 16) && aligned(a.v_out, 16)) {
         const dim3 grid((unsigned)((per_head + 255) / 256), (unsigned)(n_seq * a.c.n_kv));
-        kv8_read_vec_kernel<T, kFmt><<<grid, 256, 0, stream>>>(a, chunks);
-        KVB_CHECK_LAUNCH("kv_read_q8 launch");
-        return KVB_OK;
+        const cudaError_t e =
+            launch_pdl(kv8_read_vec_kernel<T, kFmt>, grid, dim3(256), 0, stream, a, chunks);
+        return e == cudaSuccess ? KVB_OK : cuda_fail(e, "kv_read_q8 launch");
     }
     const long long items = (long long)n_seq * a.t * a.c.n_kv * 2;
     const long long grid = (items + 3) / 4;
@@ -256,6 +258,28 @@ static size_t q8_ws_bytes(size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
                              sizeof(float);
 }
 
+// Chunks of a split call: in a workspace and joined by a pass, or (small grids, every CTA
+// resident at once, at most 8 chunks) folded through a cluster, as kvb_attention_decode does.
+struct Q8Plan {
+    int chunk_keys, max_chunks;
+    bool fold;
+};
+static Q8Plan q8_plan(size_t n_seq, size_t max_len, size_t n_q, size_t n_kv, size_t head_dim,
+                      const void* ws, size_t ws_len) {
+    const size_t need = q8_ws_bytes(n_seq, max_len, n_q, n_kv, head_dim);
+    const bool split = need > 0 && ws != nullptr && ws_len >= need && aligned(ws, 16);
+    const size_t unit = (size_t)kQ8Warps * q8_tile_keys((int)head_dim);
+    size_t ck = split ? (size_t)q8_chunk_keys(n_seq, n_kv, max_len, head_dim)
+                      : (max_len + unit - 1) / unit * unit;
+    if (ck == 0) ck = unit;
+    Q8Plan p;
+    p.chunk_keys = (int)ck;
+    p.max_chunks = max_len ? (int)((max_len + ck - 1) / ck) : 1;
+    p.fold = p.max_chunks >= 2 && p.max_chunks <= 8 &&
+             n_kv * n_seq * p.max_chunks <= (size_t)num_sms() * kQ8CtasPerSm;
+    return p;
+}
+
 static int launch_join(kvb_stream_t stream, const JoinArgs& a, size_t n_seq, int dtype) {
     const dim3 grid((unsigned)a.n_kv, (unsigned)n_seq);
     const size_t smem = (size_t)a.max_parts * a.group * sizeof(float);
@@ -280,18 +304,12 @@ static int launch_q8_tensor(kvb_stream_t stream, Q8DecodeArgs& a, size_t n_seq, 
     if (st) return st;
     st = encode_tmap_rows8(&vmap, a.c.vc, HD, cache_rows, a.piece);
     if (st) return st;
-    const size_t n_kv = (size_t)a.c.n_kv, max_len = (size_t)a.max_len;
-    const size_t need = q8_ws_bytes(n_seq, max_len, n_kv * a.group, n_kv, HD);
-    const bool split = need > 0 && ws != nullptr && ws_len >= need && aligned(ws, 16);
-    a.chunk_keys = q8_chunk_keys(n_seq, n_kv, max_len, HD);
-    if (!split) a.chunk_keys = (int)((max_len + kQ8Warps * KT - 1) / (kQ8Warps * KT) * (kQ8Warps * KT));
-    if (a.chunk_keys == 0) a.chunk_keys = kQ8Warps * KT;
-    a.max_chunks = (int)((max_len + a.chunk_keys - 1) / a.chunk_keys);
-    if (a.max_chunks < 1) a.max_chunks = 1;
-    a.ws = split ? static_cast<float*>(ws) : nullptr;
-    // Small split grids fold their chunks through a cluster, as kvb_attention_decode does.
-    a.fold = a.max_chunks >= 2 && a.max_chunks <= 8 &&
-             n_kv * n_seq * a.max_chunks <= (size_t)num_sms() * kQ8CtasPerSm;
+    const size_t n_kv = (size_t)a.c.n_kv;
+    const Q8Plan plan = q8_plan(n_seq, (size_t)a.max_len, n_kv * a.group, n_kv, HD, ws, ws_len);
+    a.chunk_keys = plan.chunk_keys;
+    a.max_chunks = plan.max_chunks;
+    a.fold = plan.fold ? 1 : 0;
+    a.ws = plan.max_chunks > 1 ? static_cast<float*>(ws) : nullptr;
     auto* kernel = attn_decode_q8_kernel<T, kFmt, HD, NT>;
     set_max_smem(kernel, q8_smem_bytes(HD, NT));
     cudaLaunchConfig_t cfg = {};
@@ -567,6 +585,13 @@ static int launch_shared(kvb_stream_t stream, const GeneralDecodeArgs& a, const 
     attn_general_src_kernel<T, SharedSource<T>><<<grid, 128, 0, stream>>>(a, src);
     KVB_CHECK_LAUNCH("attention_decode_shared launch");
     return KVB_OK;
+}
+
+int q8_join_launches(size_t n_seq, size_t max_len, size_t n_q, size_t n_kv, size_t head_dim,
+                     const void* ws, size_t ws_len) {
+    if (!q8_tensor_shape(head_dim, n_q, n_kv) || n_seq == 0) return 0;
+    const Q8Plan p = q8_plan(n_seq, max_len, n_q, n_kv, head_dim, ws, ws_len);
+    return p.max_chunks > 1 && !p.fold ? 1 : 0;
 }
 
 }  // namespace kvb

@@ -10,7 +10,8 @@
 // fused into the following rmsnorm (kvb_add_rmsnorm); RoPE, the KV append and
 // decode attention are one launch (kvb_rope_attention_decode, in the step form
 // that starts its K/V reads before the preceding kernel completes) on contiguous
-// caches at head_dim 64.  All device memory is caller-owned.
+// caches at head_dim 64.  With an 8-bit cache (kvb_decoder_use_q8_cache) they are two:
+// kvb_rope_kv_append_q8 and kvb_attention_decode_q8.  All device memory is caller-owned.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -60,6 +61,9 @@ Layout make_layout(const kvb_decoder_config& c) {
     L.lens = take(B * 4);
     L.attn_ws_len = kvb_attention_decode_workspace_bytes(B, (size_t)c.max_seq, (size_t)c.n_q,
                                                          (size_t)c.n_kv, (size_t)c.head_dim);
+    const size_t q8 = kvb_attention_decode_q8_workspace_bytes(
+        B, (size_t)c.max_seq, (size_t)c.n_q, (size_t)c.n_kv, (size_t)c.head_dim);
+    if (q8 > L.attn_ws_len) L.attn_ws_len = q8;
     L.attn_ws = take(L.attn_ws_len);
     L.lm_ws_len = B <= 32 ? kvb_lm_head_argmax_workspace_bytes(B) : 0;
     L.lm_ws = take(L.lm_ws_len);
@@ -91,6 +95,11 @@ struct kvb_decoder_s {
     uint8_t* vpool = nullptr;
     size_t pool_len = 0, max_blocks = 0, block_size = 0;
     const int32_t* block_table = nullptr;
+    // 8-bit cache (kvb_decoder_use_q8_cache / _paged; -1: 16-bit): the codes are kc / vc or
+    // the pools, one scale per head_dim codes
+    int q8_format = -1;
+    float* k_scales = nullptr;
+    float* v_scales = nullptr;
     const float* cos_t = nullptr;
     const float* sin_t = nullptr;
     kvb_blas_t blas = nullptr;
@@ -150,7 +159,38 @@ static int record_step(kvb_decoder_s* d, kvb_stream_t s) {
     for (int l = 0; l < c.n_layers; ++l) {
         st = proj(d->at(L.h), H, d->w_qkv[l], d->at(L.qkv), qkvd);
         if (st != KVB_OK) return st;
-        if (!d->block_table) {
+        if (d->q8_format >= 0) {
+            const float scale = 1.0f / sqrtf((float)hd);
+            const size_t codes = d->block_table ? d->pool_len : layer_elems;  // per layer
+            uint8_t* kl = (d->block_table ? d->kpool : d->kc) + (size_t)l * codes;
+            uint8_t* vl = (d->block_table ? d->vpool : d->vc) + (size_t)l * codes;
+            float* ksl = d->k_scales + (size_t)l * (codes / hd);
+            float* vsl = d->v_scales + (size_t)l * (codes / hd);
+            const int fmt = d->q8_format;
+            if (d->block_table) {
+                STEP(kvb_rope_kv_append_q8_paged(s, d->at(L.qkv), B * qkvd, B, 1, d->at<int32_t>(L.pos),
+                                                 d->cos_t, d->sin_t, table_len, kl, vl, ksl, vsl, codes,
+                                                 codes / hd, d->block_table, d->max_blocks,
+                                                 d->block_size, nq, nkv, hd, fmt, dt),
+                     false);
+                STEP(kvb_attention_decode_q8_paged(s, d->at(L.qkv), qkvd, kl, vl, ksl, vsl, codes,
+                                                   codes / hd, d->block_table, d->max_blocks,
+                                                   d->block_size, d->at<int32_t>(L.lens), B, max_seq,
+                                                   nq, nkv, hd, scale, d->at(L.attn), qd,
+                                                   d->at(L.attn_ws), L.attn_ws_len, fmt, dt),
+                     false);
+            } else {
+                STEP(kvb_rope_kv_append_q8(s, d->at(L.qkv), B * qkvd, B, 1, d->at<int32_t>(L.pos),
+                                           d->cos_t, d->sin_t, table_len, kl, vl, ksl, vsl, seq_stride,
+                                           codes, codes / hd, nq, nkv, hd, max_seq, fmt, dt),
+                     false);
+                STEP(kvb_attention_decode_q8(s, d->at(L.qkv), qkvd, kl, vl, ksl, vsl, seq_stride, codes,
+                                             codes / hd, d->at<int32_t>(L.lens), B, max_seq, nq, nkv, hd,
+                                             max_seq, scale, d->at(L.attn), qd, d->at(L.attn_ws),
+                                             L.attn_ws_len, fmt, dt),
+                     false);
+            }
+        } else if (!d->block_table) {
             uint8_t* kl = d->kc + (size_t)l * layer_elems * 2;
             uint8_t* vl = d->vc + (size_t)l * layer_elems * 2;
             if (hd == 64 && nq / nkv <= 16) {  // RoPE, KV append and attention: one launch
@@ -182,8 +222,11 @@ static int record_step(kvb_decoder_s* d, kvb_stream_t s) {
                      d->at(L.attn), qd, d->at(L.attn_ws), L.attn_ws_len, dt),
                  false);
         }
-        own += kvb::decode_combine_launches(B, max_seq, nq, nkv, hd, d->at(L.attn_ws),
-                                            L.attn_ws_len);  // the split-KV combine pass
+        // the split-KV combine pass
+        own += d->q8_format >= 0 ? kvb::q8_join_launches(B, max_seq, nq, nkv, hd, d->at(L.attn_ws),
+                                                         L.attn_ws_len)
+                                 : kvb::decode_combine_launches(B, max_seq, nq, nkv, hd,
+                                                                d->at(L.attn_ws), L.attn_ws_len);
         st = proj(d->at(L.attn), qd, d->w_o[l], d->at(L.o), H);
         if (st != KVB_OK) return st;
         STEP(kvb_add_rmsnorm(s, d->at(L.x), B * H, d->at(L.o), B * H, d->mlp_norm[l], H, d->at(L.h),
@@ -343,7 +386,53 @@ int kvb_decoder_use_paged_cache(kvb_decoder_t d, void* k_pools, void* v_pools, s
     d->block_table = block_table;
     d->max_blocks = max_blocks;
     d->block_size = block_size;
+    d->q8_format = -1;
     drop_graph(d);  // the next step records the paged step
+    return KVB_OK;
+}
+
+int kvb_decoder_use_q8_cache(kvb_decoder_t d, void* kc, void* vc, float* k_scales, float* v_scales,
+                             int kv_format) {
+    KVB_CHECK(d && kc && vc && k_scales && v_scales, "decoder_use_q8_cache: null argument");
+    KVB_CHECK(kv_format == KVB_KV_INT8 || kv_format == KVB_KV_E4M3,
+              "decoder_use_q8_cache: unknown KV format %d", kv_format);
+    KVB_CHECK(d->cfg.head_dim <= 256, "decoder_use_q8_cache: head_dim %d above 256", d->cfg.head_dim);
+    d->kc = static_cast<uint8_t*>(kc);
+    d->vc = static_cast<uint8_t*>(vc);
+    d->k_scales = k_scales;
+    d->v_scales = v_scales;
+    d->block_table = nullptr;
+    d->q8_format = kv_format;
+    drop_graph(d);
+    return KVB_OK;
+}
+
+int kvb_decoder_use_q8_paged_cache(kvb_decoder_t d, void* k_pools, void* v_pools, float* k_scales,
+                                   float* v_scales, size_t pool_len, const int32_t* block_table,
+                                   size_t max_blocks, size_t block_size, int kv_format) {
+    KVB_CHECK(d && k_pools && v_pools && k_scales && v_scales && block_table,
+              "decoder_use_q8_paged_cache: null argument");
+    KVB_CHECK(kv_format == KVB_KV_INT8 || kv_format == KVB_KV_E4M3,
+              "decoder_use_q8_paged_cache: unknown KV format %d", kv_format);
+    const kvb_decoder_config& c = d->cfg;
+    KVB_CHECK(c.head_dim <= 256, "decoder_use_q8_paged_cache: head_dim %d above 256", c.head_dim);
+    const size_t per_block = (size_t)c.n_kv * block_size * (size_t)c.head_dim;
+    KVB_CHECK(block_size > 0 && pool_len > 0 && pool_len % per_block == 0,
+              "decoder_use_q8_paged_cache: pool of %zu elems is not a whole number of %zu-elem blocks",
+              pool_len, per_block);
+    KVB_CHECK(max_blocks * block_size >= (size_t)c.max_seq,
+              "decoder_use_q8_paged_cache: %zu blocks of %zu hold fewer than max_seq %d positions",
+              max_blocks, block_size, c.max_seq);
+    d->kpool = static_cast<uint8_t*>(k_pools);
+    d->vpool = static_cast<uint8_t*>(v_pools);
+    d->k_scales = k_scales;
+    d->v_scales = v_scales;
+    d->pool_len = pool_len;
+    d->block_table = block_table;
+    d->max_blocks = max_blocks;
+    d->block_size = block_size;
+    d->q8_format = kv_format;
+    drop_graph(d);
     return KVB_OK;
 }
 

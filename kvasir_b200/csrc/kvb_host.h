@@ -69,6 +69,10 @@ int rope_attention_decode_paged_in_step(kvb_stream_t stream, const void* qkv, si
 int decode_combine_launches(size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
                             size_t head_dim, const void* workspace, size_t workspace_len);
 
+// The same for kvb_attention_decode_q8 (its tensor-core shapes, aligned buffers).
+int q8_join_launches(size_t n_seq, size_t max_len, size_t n_q, size_t n_kv, size_t head_dim,
+                     const void* workspace, size_t workspace_len);
+
 }  // namespace kvb
 
 #define KVB_CHECK(cond, ...)                                         \

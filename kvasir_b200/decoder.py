@@ -17,7 +17,7 @@ import torch
 
 from . import _lib as L
 from .config import LlamaConfig
-from .gpu import ShapeError, check, dtype_tag
+from .gpu import Gpu, ShapeError, check, dtype_tag, kv_format
 from .rope import cos_sin_table
 
 
@@ -58,11 +58,13 @@ class Decoder:
     ("lm_head" present for untied checkpoints).
     kc / vc: [n_layers, n_seq, n_kv, max_seq, head_dim], or with paged_block_size
     the block pools [n_layers, n_blocks, n_kv, paged_block_size, head_dim] that
-    self.block_table ([n_seq, max_blocks], one table for all layers) indexes."""
+    self.block_table ([n_seq, max_blocks], one table for all layers) indexes.
+    kv_dtype: torch.int8 or torch.float8_e4m3fn for an 8-bit cache; kc / vc then hold its codes
+    and ks / vs its f32 scales (kc / vc's shape without the last dimension)."""
 
     def __init__(self, cfg: LlamaConfig, n_seq: int, max_seq: int, device="cuda",
                  dtype=torch.bfloat16, weights: dict | None = None, seed: int = 0,
-                 paged_block_size: int | None = None):
+                 paged_block_size: int | None = None, kv_dtype: torch.dtype | None = None):
         self.cfg, self.n_seq, self.max_seq = cfg, n_seq, max_seq
         self.device = torch.device(device)
         self.dtype = dtype
@@ -77,14 +79,19 @@ class Decoder:
             shape = (cfg.num_layers, n_blocks, cfg.num_kv_heads, bs, cfg.head_dim)
             perm = np.random.default_rng(seed + 1).permutation(n_blocks).astype(np.int32)
             self.block_table = torch.from_numpy(perm.reshape(n_seq, max_blocks)).to(self.device)
-        self.kc = torch.empty(shape, dtype=dtype, device=self.device)
-        self.vc = torch.empty(shape, dtype=dtype, device=self.device)
+        self.kc = torch.empty(shape, dtype=kv_dtype or dtype, device=self.device)
+        self.vc = torch.empty(shape, dtype=kv_dtype or dtype, device=self.device)
+        self.ks = self.vs = None
+        if kv_dtype is not None:
+            kv_format(self.kc)  # refuses other types
+            self.ks = torch.zeros(shape[:-1], dtype=torch.float32, device=self.device)
+            self.vs = torch.zeros(shape[:-1], dtype=torch.float32, device=self.device)
         cos, sin = cos_sin_table(cfg, max_seq)
         self.cos = torch.from_numpy(cos).to(self.device)
         self.sin = torch.from_numpy(sin).to(self.device)
         c = L.DecoderConfig(cfg.hidden_size, cfg.intermediate_size, cfg.num_layers, cfg.num_heads,
                             cfg.num_kv_heads, cfg.head_dim, cfg.vocab_size, max_seq, n_seq,
-                            cfg.rms_norm_eps, dtype_tag(self.kc))
+                            cfg.rms_norm_eps, dtype_tag(torch.empty(0, dtype=dtype)))
         self._cfg = c
         lib = L.lib()
         nbytes = int(lib.kvb_decoder_workspace_bytes(C.byref(c)))
@@ -115,7 +122,17 @@ class Decoder:
 
         if "lm_head" in self.w:  # untied checkpoint (kvasir_b200.weights.load_weights)
             check(lib.kvb_decoder_set_lm_head(h, self.w["lm_head"].data_ptr()))
-        if paged_block_size:
+        if kv_dtype is not None:
+            tag = kv_format(self.kc)
+            k, v, ks, vs = (t.data_ptr() for t in (self.kc, self.vc, self.ks, self.vs))
+            if paged_block_size:
+                self._paged = (self.kc, self.vc, self.block_table)
+                check(lib.kvb_decoder_use_q8_paged_cache(
+                    h, k, v, ks, vs, self.kc[0].numel(), self.block_table.data_ptr(), max_blocks,
+                    paged_block_size, tag))
+            else:
+                check(lib.kvb_decoder_use_q8_cache(h, k, v, ks, vs, tag))
+        elif paged_block_size:
             self.use_paged_cache(self.kc, self.vc, self.block_table, max_blocks, paged_block_size)
         self.ids_in = view(lib.kvb_decoder_ids_in(h), n_seq, torch.int32)
         self.ids_out = view(lib.kvb_decoder_ids_out(h), n_seq, torch.int32)
@@ -143,6 +160,11 @@ class Decoder:
         split over ranks (a paged cache gets the same contents through its
         block table)."""
         g = torch.Generator(device=self.device)
+        if self.ks is not None:
+            if first_seq is None:
+                g.manual_seed(seed)
+            self._fill_q8(g, seed, std, first_seq)
+            return
         if first_seq is None:
             g.manual_seed(seed)
             for l in range(self.cfg.num_layers):
@@ -169,6 +191,27 @@ class Decoder:
                         tmp[:, :self.max_seq] = seq
                         blocks = tmp.view(nkv, mb, bs, hd).permute(1, 0, 2, 3)
                         cache[l][self.block_table[b].long()] = blocks
+
+    def _fill_q8(self, g, seed, std, first_seq) -> None:
+        """fill_kv_normal of an 8-bit cache: 16-bit rows N(0, std), quantised into it."""
+        cfg, paged = self.cfg, getattr(self, "_paged", None)
+        nkv, hd, n = cfg.num_kv_heads, cfg.head_dim, self.max_seq
+        gpu = Gpu(self.device.index or 0, torch.cuda.current_stream(self.device))
+        rows = torch.empty(n, 2 * nkv * hd, dtype=self.dtype, device=self.device)
+        pos = torch.zeros(1, dtype=torch.int32, device=self.device)
+        for l in range(cfg.num_layers):
+            for b in range(self.n_seq):
+                if first_seq is not None:
+                    g.manual_seed(((seed * 1000003 + first_seq + b) * 1024 + l) & (2 ** 63 - 1))
+                rows.normal_(0.0, std, generator=g)
+                if paged is not None:
+                    mb, bs = self.block_table.shape[1], self.kc.shape[3]
+                    gpu.rope_kv_append_q8_paged(rows, 1, n, pos, None, None, self.kc[l], self.vc[l],
+                                                self.ks[l], self.vs[l], self.block_table[b], mb, bs,
+                                                0, nkv, hd)
+                else:
+                    gpu.rope_kv_append_q8(rows, 1, n, pos, None, None, self.kc[l, b], self.vc[l, b],
+                                          self.ks[l, b], self.vs[l, b], nkv * n * hd, 0, nkv, hd, n)
 
     def use_paged_cache(self, k_pools, v_pools, block_table, max_blocks: int,
                         block_size: int) -> None:
@@ -231,4 +274,4 @@ class Decoder:
         return own.value, lib.value
 
     def weight_bytes(self) -> int:
-        return self.cfg.weight_params() * self.kc.element_size()
+        return self.cfg.weight_params() * torch.empty(0, dtype=self.dtype).element_size()

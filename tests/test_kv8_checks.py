@@ -134,6 +134,12 @@ def test_shared_refusals():
     _refused(paged(bt=None), "block table")
 
 
+def test_decoder_refusals():
+    lib = L.lib()
+    _refused(lib.kvb_decoder_use_q8_cache(None, F, F, F, F, 0), "null")
+    _refused(lib.kvb_decoder_use_q8_paged_cache(None, F, F, F, F, 64, F, 1, 16, 0), "null")
+
+
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 def test_reference_quantisation_is_within_half_a_step(fmt):
     """The tests' own reference: within half a step of the row, exact at the row's maximum."""
