@@ -64,6 +64,7 @@ struct Q8DecodeArgs {
     int max_chunks;
     int fold;        // chunks of a (sequence, KV head) folded through a cluster
     int piece;       // rows per tensor copy: a whole tile, or gcd(block_size, tile) paged
+    int bs_shift;    // paged: log2 of block_size, or -1
     int total_rows;  // rows of the code arrays (a row past the end reads as zeros)
     Kv8Place c;
 };
@@ -219,7 +220,8 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
         auto block_of = [&](int kt0) -> int {
             const int k = kt0 + (lane << pshift);
             if (!a.c.block_table || lane >= (KT >> pshift) || k >= key_end) return 0;
-            return a.c.block_table[(size_t)b * a.c.max_blocks + k / a.c.block_size];
+            const int lb = a.bs_shift >= 0 ? k >> a.bs_shift : k / a.c.block_size;
+            return a.c.block_table[(size_t)b * a.c.max_blocks + lb];
         };
         int blk = block_of(key_begin + warp * KT);
         // The tile that is requested next: its pieces, this lane's piece's row, and the rows of
@@ -240,9 +242,11 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
             if (lane < n_pieces) {
                 if (blk < 0 || blk >= a.c.n_blocks)
                     raise_dev_error(kDevErrBadPosition);
-                else
+                else {
+                    const int k = kt0 + (lane << pshift);
                     row = (blk * a.c.n_kv + kvh) * a.c.block_size +
-                          (kt0 + (lane << pshift)) % a.c.block_size;
+                          (a.bs_shift >= 0 ? k & (a.c.block_size - 1) : k % a.c.block_size);
+                }
             }
             blk = block_of(kt0 + kQ8Warps * KT);  // of the tile that is placed next
 #pragma unroll

@@ -298,6 +298,9 @@ static int launch_q8_tensor(kvb_stream_t stream, Q8DecodeArgs& a, size_t n_seq, 
     a.piece = KT;
     if (a.c.block_table)
         while (a.c.block_size % a.piece) a.piece /= 2;
+    a.bs_shift = -1;
+    for (int s = 0; a.c.block_table && s < 31; ++s)
+        if (a.c.block_size == 1 << s) a.bs_shift = s;
     a.total_rows = (int)cache_rows;
     CUtensorMap kmap, vmap;
     int st = encode_tmap_rows8(&kmap, a.c.kc, HD, cache_rows, a.piece);
