@@ -243,7 +243,9 @@ __device__ __forceinline__ uint32_t widen_bits(uint32_t h) {
 // so that 1,536 threads (48 KB of loads) are in flight on an SM -- at 62 registers 960 were,
 // and 4 x 2048 tokens of 32 + 16 heads (103 MB) took 25 us instead of 21.2.  Measured no
 // better: 48 registers with several short rows per CTA (21.2), a persistent grid that requests
-// the next row ahead (28.3).
+// the next row ahead (28.3).  What bounds it is issue (61 % of slots, 75 % of an SM's busy
+// time).  Packed f32x2 multiplies and adds would halve the arithmetic, but the assembler
+// contracts them into one rounding (x * inv = 63.5 - 2^-18 then gives code 63, not 64).
 template <typename T, int kFmt, int CPR>
 __global__ void __launch_bounds__(256, 6) kv8_append_vec_kernel(Kv8AppendArgs a) {
     asm volatile("griddepcontrol.launch_dependents;");
