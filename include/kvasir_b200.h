@@ -439,6 +439,30 @@ int kvb_attention_decode_q8_paged(kvb_stream_t stream, const void* q, size_t q_r
 size_t kvb_attention_decode_q8_workspace_bytes(size_t n_seq, size_t max_len, size_t n_q,
                                                size_t n_kv, size_t head_dim);
 
+/* Decode step of the attention block over an 8-bit cache in one launch:
+ * kvb_rope_kv_append_q8 of one row per sequence at position lens[b] - 1, then
+ * kvb_attention_decode_q8, bit for bit, as kvb_rope_attention_decode does for 16-bit
+ * caches: qkv [n_seq, (n_q + 2 n_kv) * head_dim] stays unrotated, the codes and scales of
+ * the new rows are written.  head_dim 64 or 128, n_q / n_kv <= 16, block_size a multiple
+ * of 16, 16-byte aligned buffers; otherwise KVB_ERR_UNSUPPORTED.  Workspace as for
+ * kvb_attention_decode_q8. */
+int kvb_rope_attention_decode_q8(kvb_stream_t stream, const void* qkv, size_t qkv_len,
+                                 const float* cos_t, const float* sin_t, size_t table_len, void* kc,
+                                 void* vc, float* ks, float* vs, size_t seq_stride, size_t cache_len,
+                                 size_t scale_len, const int32_t* lens, size_t n_seq, size_t max_len,
+                                 size_t n_q, size_t n_kv, size_t head_dim, size_t max_seq, float scale,
+                                 void* out, size_t out_row_stride, void* workspace,
+                                 size_t workspace_len, int kv_format, int dtype);
+int kvb_rope_attention_decode_q8_paged(kvb_stream_t stream, const void* qkv, size_t qkv_len,
+                                       const float* cos_t, const float* sin_t, size_t table_len,
+                                       void* k_pool, void* v_pool, float* k_scales, float* v_scales,
+                                       size_t pool_len, size_t scale_len, const int32_t* block_table,
+                                       size_t max_blocks, size_t block_size, const int32_t* lens,
+                                       size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
+                                       size_t head_dim, float scale, void* out, size_t out_row_stride,
+                                       void* workspace, size_t workspace_len, int kv_format,
+                                       int dtype);
+
 /* Batched single-query decode attention of sequences that share a prefix (16-bit
  * caches).  New: the reference decodes one sequence (engine/src/gpu/kernels.rs:
  * 294-371).  Contiguous: every sequence attends to the prefix's keys [0, prefix_len)
@@ -569,8 +593,8 @@ int kvb_decoder_use_paged_cache(kvb_decoder_t dec, void* k_pools, void* v_pools,
  * [n_layers][n_seq][n_kv][max_seq][head_dim] and scales [n_layers][n_seq][n_kv]
  * [max_seq], or pools as for kvb_decoder_use_paged_cache with scale pools [n_layers]
  * [n_blocks][n_kv][block_size].  The caches given before are no longer used.  A step
- * then runs kvb_rope_kv_append_q8(_paged) and kvb_attention_decode_q8(_paged) per
- * layer; any head_dim up to 256, any block_size (multiples of 16 are fast).  The next
+ * then runs kvb_rope_attention_decode_q8(_paged) per layer where it applies, else the
+ * append and the attention; any head_dim up to 256, any block_size (multiples of 16 are fast).  The next
  * step re-records its graph; call outside any stream capture. */
 int kvb_decoder_use_q8_cache(kvb_decoder_t dec, void* kc, void* vc, float* k_scales,
                              float* v_scales, int kv_format);

@@ -131,6 +131,12 @@ SIGNATURES = {
                                              _p, _sz, _sz, _sz, _sz, _sz, C.c_float, _p, _sz, _p,
                                              _sz, _int, _int]),
     "kvb_attention_decode_q8_workspace_bytes": (_sz, [_sz, _sz, _sz, _sz, _sz]),
+    "kvb_rope_attention_decode_q8": (_int, [_p, _p, _sz, _p, _p, _sz, _p, _p, _p, _p, _sz, _sz, _sz,
+                                            _p, _sz, _sz, _sz, _sz, _sz, _sz, C.c_float, _p, _sz, _p,
+                                            _sz, _int, _int]),
+    "kvb_rope_attention_decode_q8_paged": (_int, [_p, _p, _sz, _p, _p, _sz, _p, _p, _p, _p, _sz, _sz,
+                                                  _p, _sz, _sz, _p, _sz, _sz, _sz, _sz, _sz,
+                                                  C.c_float, _p, _sz, _p, _sz, _int, _int]),
     "kvb_attention_decode_shared": (_int, [_p, _p, _sz, _p, _p, _sz, _sz, _p, _p, _sz, _sz, _p, _sz,
                                            _sz, _sz, _sz, _sz, _sz, C.c_float, _p, _sz, _p, _sz,
                                            _int]),

@@ -67,7 +67,46 @@ struct Q8DecodeArgs {
     int bs_shift;    // paged: log2 of block_size, or -1
     int total_rows;  // rows of the code arrays (a row past the end reads as zeros)
     Kv8Place c;
+    // Fused RoPE + append (kRope, kvb_rope_attention_decode_q8): the new token of sequence b is
+    // key lens[b] - 1; q points at the qkv rows, unrotated.  Q is rotated in registers, and
+    // the CTA of the last chunk quantises the rotated k and the v into that cache row before
+    // its tile is requested.
+    const float* rope_cos;
+    const float* rope_sin;
+    int rope_max_pos;
 };
+
+// One warp's share of the append: a K (rotated) or V row of HD 16-bit elements, quantised to
+// codes and scale as kv8_append_vec_kernel does.
+template <typename T, int kFmt, int HD>
+__device__ __forceinline__ void q8_append_row(const T* in, const float* cos_row, const float* sin_row,
+                                              uint8_t* codes, float* scale) {
+    constexpr int half = HD / 2;
+    const int lane = threadIdx.x & 31;
+    float lo[HD / 64], hi[HD / 64];
+    uint32_t mx = 0;
+#pragma unroll
+    for (int i = 0; i < HD / 64; ++i) {
+        const int d = lane + 32 * i;
+        lo[i] = Elem<T>::to_f(in[d]);
+        hi[i] = Elem<T>::to_f(in[d + half]);
+        if (cos_row) {
+            const float r0 = rot_a(lo[i], hi[i], cos_row[d], sin_row[d]);
+            const float r1 = rot_b(lo[i], hi[i], cos_row[d], sin_row[d]);
+            lo[i] = Elem<T>::to_f(Elem<T>::from_f(r0));
+            hi[i] = Elem<T>::to_f(Elem<T>::from_f(r1));
+        }
+        mx = max(mx, max(abs_bits(lo[i]), abs_bits(hi[i])));
+    }
+    const RowScale rs = kv8_row_scale<kFmt>(__reduce_max_sync(0xffffffffu, mx));
+#pragma unroll
+    for (int i = 0; i < HD / 64; ++i) {
+        const uint32_t c2 = kv8_codes2<kFmt>(lo[i], hi[i], rs.inv);
+        codes[lane + 32 * i] = (uint8_t)c2;
+        codes[lane + 32 * i + half] = (uint8_t)(c2 >> 8);
+    }
+    if (lane == 0) *scale = rs.scale;
+}
 
 __device__ __forceinline__ int q8_len(const int32_t* lens, int max_len, int b) {
     int len = lens[b];
@@ -168,7 +207,7 @@ __device__ __forceinline__ uint32_t q8_smem_off(int r, int ch) {
 // Grid (KV head, sequence, chunk slot), or with a.fold (chunk slot, KV head, sequence) in
 // clusters of max_chunks CTAs; slots count chunks from the end of the sequence, so full
 // chunks are dispatched first (as attn_decode.cuh).
-template <typename T, int kFmt, int HD, int NT>
+template <typename T, int kFmt, int HD, int NT, bool kRope>
 __global__ void __launch_bounds__(128, kQ8CtasPerSm)
     attn_decode_q8_kernel(const __grid_constant__ CUtensorMap kmap,
                           const __grid_constant__ CUtensorMap vmap, Q8DecodeArgs a) {
@@ -215,6 +254,15 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
         const int key_end = min(len, key_begin + a.chunk_keys);
         const int row_base = (int)(b * a.c.seq_rows + (long long)kvh * a.c.max_seq);
         const int pshift = __ffs(a.piece) - 1;
+        int rope_p = -1;  // the new token's position (-1: none, or outside the tables)
+        if (kRope) {
+            rope_p = len - 1;
+            if (rope_p >= a.rope_max_pos) {
+                if (threadIdx.x == 0) raise_dev_error(kDevErrBadPosition);
+                rope_p = -1;
+            }
+        }
+        const bool appends = kRope && rope_p >= 0 && chunk == n_chunks - 1;  // CTA-uniform
 
         // Paged: this lane's piece of the next tile to be requested, read a tile ahead.
         auto block_of = [&](int kt0) -> int {
@@ -277,14 +325,37 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
             request(vmap, ring + (st * 2 + 1) * kQ8TileBytes, a.c.vs, ring_scales + st * 128 + 64,
                     &bars[warp][st][1]);
         };
+        // The first tiles; the one that holds the new key waits until that row is written (it is
+        // its warp's last).
+        auto first_tiles = [&](bool holding) {
 #pragma unroll
-        for (int i = 0; i < kQ8Stages; ++i) {
-            const int kt0 = key_begin + (warp + i * kQ8Warps) * KT;
-            if (kt0 < key_end) {
-                place(kt0);
-                request_k(i);
-                request_v(i);
+            for (int i = 0; i < kQ8Stages; ++i) {
+                const int kt0 = key_begin + (warp + i * kQ8Warps) * KT;
+                if (kt0 < key_end && (appends && rope_p < kt0 + KT) == holding) {
+                    place(kt0);
+                    request_k(i);
+                    request_v(i);
+                }
             }
+        };
+        first_tiles(false);
+        if (appends) {
+            size_t crow = 0, head_rows = 0;
+            if (warp < 2 && kv8_row(a.c, b, rope_p, crow, head_rows, threadIdx.x == 0)) {
+                crow += (size_t)kvh * head_rows;
+                const T* in = reinterpret_cast<const T*>(a.q) + (size_t)b * a.q_row_stride +
+                              (size_t)(a.c.n_kv * (G + warp) + kvh) * HD;
+                if (warp == 0)
+                    q8_append_row<T, kFmt, HD>(in, a.rope_cos + (size_t)rope_p * (HD / 2),
+                                               a.rope_sin + (size_t)rope_p * (HD / 2),
+                                               a.c.kc + crow * HD, a.c.ks + crow);
+                else
+                    q8_append_row<T, kFmt, HD>(in, nullptr, nullptr, a.c.vc + crow * HD, a.c.vs + crow);
+            }
+            // the tensor copies read these rows through the async proxy
+            asm volatile("fence.proxy.async.global;" ::: "memory");
+            __syncthreads();
+            first_tiles(true);
         }
 
         // Q fragments (B operand): column g = head 8 nt + g, dims 16 j + 4c .. + 3.  int8: the
@@ -300,6 +371,22 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
 #pragma unroll
             for (int j = 0; j < DT; ++j)
                 v[j] = h < G ? *reinterpret_cast<const uint2*>(qr + 16 * j + 4 * c) : make_uint2(0u, 0u);
+            if (kRope && rope_p >= 0) {
+                // rotate_half in registers: chunk j pairs with chunk j + DT / 2, the same lane
+#pragma unroll
+                for (int j = 0; j < DT / 2; ++j) {
+                    const size_t at = (size_t)rope_p * (HD / 2) + 16 * j + 4 * c;
+                    const float4 cs = *reinterpret_cast<const float4*>(a.rope_cos + at);
+                    const float4 sn = *reinterpret_cast<const float4*>(a.rope_sin + at);
+                    auto rotate2 = [](uint32_t& lo, uint32_t& hi, float c0, float c1, float s0, float s1) {
+                        const float2 x = Elem<T>::unpack(lo), y = Elem<T>::unpack(hi);
+                        lo = Elem<T>::pack(rot_a(x.x, y.x, c0, s0), rot_a(x.y, y.y, c1, s1));
+                        hi = Elem<T>::pack(rot_b(x.x, y.x, c0, s0), rot_b(x.y, y.y, c1, s1));
+                    };
+                    rotate2(v[j].x, v[j + DT / 2].x, cs.x, cs.y, sn.x, sn.y);
+                    rotate2(v[j].y, v[j + DT / 2].y, cs.z, cs.w, sn.z, sn.w);
+                }
+            }
             float f = a.scale_log2;
             if (kFmt == KVB_KV_INT8) {
                 uint32_t mx = 0;  // the head's largest magnitude, as a bit pattern

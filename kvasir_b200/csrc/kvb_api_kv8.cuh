@@ -313,7 +313,8 @@ static int launch_q8_tensor(kvb_stream_t stream, Q8DecodeArgs& a, size_t n_seq, 
     a.max_chunks = plan.max_chunks;
     a.fold = plan.fold ? 1 : 0;
     a.ws = plan.max_chunks > 1 ? static_cast<float*>(ws) : nullptr;
-    auto* kernel = attn_decode_q8_kernel<T, kFmt, HD, NT>;
+    auto* kernel = a.rope_cos ? attn_decode_q8_kernel<T, kFmt, HD, NT, true>
+                              : attn_decode_q8_kernel<T, kFmt, HD, NT, false>;
     set_max_smem(kernel, q8_smem_bytes(HD, NT));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = a.fold ? dim3((unsigned)a.max_chunks, (unsigned)n_kv, (unsigned)n_seq)
@@ -352,15 +353,26 @@ static int launch_q8_tensor(kvb_stream_t stream, Q8DecodeArgs& a, size_t n_seq, 
 }
 
 // The tensor-core kernel where shape and alignment allow it (cache_rows: rows of the code
-// arrays), else the general one.
+// arrays), else the general one; with RoPE tables (the fused form) else KVB_ERR_UNSUPPORTED.
+struct Q8Rope {
+    const float* cos_t = nullptr;
+    const float* sin_t = nullptr;
+    int max_pos = 0;
+};
 template <typename T, int kFmt>
 static int launch_q8_decode(kvb_stream_t stream, const GeneralDecodeArgs& a, const Kv8Place& c,
-                            size_t cache_rows, size_t n_seq, void* ws, size_t ws_len) {
+                            size_t cache_rows, size_t n_seq, void* ws, size_t ws_len,
+                            const Q8Rope& rope) {
     const bool tensor = q8_tensor_shape((size_t)a.hd, (size_t)a.n_q, (size_t)a.n_kv) &&
                         (!c.block_table || c.block_size % 16 == 0) && a.q_row_stride % 4 == 0 &&
                         aligned(a.q, 8) && aligned(c.kc, 16) && aligned(c.vc, 16) &&
                         aligned(c.ks, 4) && aligned(c.vs, 4) && n_seq <= 65535 &&
                         a.n_kv <= 65535 && fits_i32(cache_rows + 64);
+    if (rope.cos_t && !(tensor && aligned(rope.cos_t, 16) && aligned(rope.sin_t, 16)))
+        return fail(KVB_ERR_UNSUPPORTED,
+                    "rope_attention_decode_q8: needs head_dim 64 or 128, n_q/n_kv <= 16, block_size "
+                    "a multiple of 16 and 16-byte aligned caches and tables (use "
+                    "kvb_rope_kv_append_q8 + kvb_attention_decode_q8)");
     if (!tensor) {
         Q8Source<T, kFmt> src;
         src.c = c;
@@ -379,6 +391,9 @@ static int launch_q8_decode(kvb_stream_t stream, const GeneralDecodeArgs& a, con
     d.out = a.out;
     d.out_row_stride = a.out_row_stride;
     d.c = c;
+    d.rope_cos = rope.cos_t;
+    d.rope_sin = rope.sin_t;
+    d.rope_max_pos = rope.max_pos;
     if (a.hd == 64)
         return d.group <= 8 ? launch_q8_tensor<T, kFmt, 64, 1>(stream, d, n_seq, cache_rows, ws, ws_len)
                             : launch_q8_tensor<T, kFmt, 64, 2>(stream, d, n_seq, cache_rows, ws, ws_len);
@@ -671,28 +686,84 @@ size_t kvb_attention_decode_q8_workspace_bytes(size_t n_seq, size_t max_len, siz
     return q8_ws_bytes(n_seq, max_len, n_q, n_kv, head_dim);
 }
 
+static int q8_decode_contiguous(const char* name, kvb_stream_t stream, const void* q,
+                                size_t q_row_stride, const void* kc, const void* vc, const float* ks,
+                                const float* vs, size_t seq_stride, size_t cache_len,
+                                size_t scale_len, const int32_t* lens, size_t n_seq, size_t max_len,
+                                size_t n_q, size_t n_kv, size_t head_dim, size_t max_seq,
+                                float scale, void* out, size_t out_row_stride, void* workspace,
+                                size_t workspace_len, int kv_format, int dtype, const Q8Rope& rope) {
+    KVB_CHECK_DTYPE(dtype);
+    KVB_CHECK(valid_kv_format(kv_format), "unknown KV format %d", kv_format);
+    GeneralDecodeArgs a;
+    int st = decode_args(name, a, q, q_row_stride, lens, n_seq, max_len, n_q, n_kv, head_dim, scale,
+                         out, out_row_stride);
+    if (st) return st;
+    KVB_CHECK(max_len <= max_seq, "%s: max_len %zu exceeds max_seq %zu", name, max_len, max_seq);
+    Kv8Place c;
+    st = kv8_place_contiguous(name, c, kc, vc, ks, vs, seq_stride, cache_len, scale_len, n_seq, n_kv,
+                              head_dim, max_seq);
+    if (st) return st;
+    if (n_seq == 0) return KVB_OK;
+    const size_t cache_rows = scale_len;
+    return KVB_KV8_DISPATCH(launch_q8_decode, dtype, kv_format, stream, a, c, cache_rows, n_seq,
+                            workspace, workspace_len, rope);
+}
+
+static int q8_decode_paged(const char* name, kvb_stream_t stream, const void* q, size_t q_row_stride,
+                           const void* k_pool, const void* v_pool, const float* k_scales,
+                           const float* v_scales, size_t pool_len, size_t scale_len,
+                           const int32_t* block_table, size_t max_blocks, size_t block_size,
+                           const int32_t* lens, size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
+                           size_t head_dim, float scale, void* out, size_t out_row_stride,
+                           void* workspace, size_t workspace_len, int kv_format, int dtype,
+                           const Q8Rope& rope) {
+    KVB_CHECK_DTYPE(dtype);
+    KVB_CHECK(valid_kv_format(kv_format), "unknown KV format %d", kv_format);
+    GeneralDecodeArgs a;
+    int st = decode_args(name, a, q, q_row_stride, lens, n_seq, max_len, n_q, n_kv, head_dim, scale,
+                         out, out_row_stride);
+    if (st) return st;
+    Kv8Place c;
+    st = kv8_place_paged(name, c, k_pool, v_pool, k_scales, v_scales, pool_len, scale_len, block_table,
+                         max_blocks, block_size, n_seq, n_kv, head_dim);
+    if (st) return st;
+    KVB_CHECK(max_len <= max_blocks * block_size, "%s: max_len %zu exceeds %zu blocks of %zu", name,
+              max_len, max_blocks, block_size);
+    if (n_seq == 0) return KVB_OK;
+    const size_t cache_rows = scale_len;
+    return KVB_KV8_DISPATCH(launch_q8_decode, dtype, kv_format, stream, a, c, cache_rows, n_seq,
+                            workspace, workspace_len, rope);
+}
+
+// The fused forms' tables and qkv rows.
+static int q8_rope(const char* name, Q8Rope& r, const void* qkv, size_t qkv_len, const float* cos_t,
+                   const float* sin_t, size_t table_len, size_t n_seq, size_t n_q, size_t n_kv,
+                   size_t head_dim) {
+    KVB_CHECK(head_dim > 0 && head_dim % 2 == 0 && head_dim <= 256 && table_len % (head_dim / 2) == 0 &&
+                  fits_i32(table_len / (head_dim / 2)),
+              "%s: bad head_dim or cos/sin table sizes", name);
+    KVB_CHECK(cos_t != nullptr && sin_t != nullptr, "%s: null table", name);
+    KVB_CHECK(fits_i32(n_seq) && fits_i32(n_q) && fits_i32(n_kv) &&
+                  qkv_len == n_seq * (n_q + 2 * n_kv) * head_dim,
+              "%s: qkv has %zu elems, want %zux%zu", name, qkv_len, n_seq,
+              (n_q + 2 * n_kv) * head_dim);
+    r.cos_t = cos_t;
+    r.sin_t = sin_t;
+    r.max_pos = (int)(table_len / (head_dim / 2));
+    return KVB_OK;
+}
+
 int kvb_attention_decode_q8(kvb_stream_t stream, const void* q, size_t q_row_stride, const void* kc,
                             const void* vc, const float* ks, const float* vs, size_t seq_stride,
                             size_t cache_len, size_t scale_len, const int32_t* lens, size_t n_seq,
                             size_t max_len, size_t n_q, size_t n_kv, size_t head_dim,
                             size_t max_seq, float scale, void* out, size_t out_row_stride,
                             void* workspace, size_t workspace_len, int kv_format, int dtype) {
-    KVB_CHECK_DTYPE(dtype);
-    KVB_CHECK(valid_kv_format(kv_format), "unknown KV format %d", kv_format);
-    GeneralDecodeArgs a;
-    int st = decode_args("attention_decode_q8", a, q, q_row_stride, lens, n_seq, max_len, n_q, n_kv,
-                         head_dim, scale, out, out_row_stride);
-    if (st) return st;
-    KVB_CHECK(max_len <= max_seq, "attention_decode_q8: max_len %zu exceeds max_seq %zu", max_len,
-              max_seq);
-    Kv8Place c;
-    st = kv8_place_contiguous("attention_decode_q8", c, kc, vc, ks, vs, seq_stride, cache_len,
-                              scale_len, n_seq, n_kv, head_dim, max_seq);
-    if (st) return st;
-    if (n_seq == 0) return KVB_OK;
-    const size_t cache_rows = scale_len;
-    return KVB_KV8_DISPATCH(launch_q8_decode, dtype, kv_format, stream, a, c, cache_rows, n_seq,
-                            workspace, workspace_len);
+    return q8_decode_contiguous("attention_decode_q8", stream, q, q_row_stride, kc, vc, ks, vs,
+                                seq_stride, cache_len, scale_len, lens, n_seq, max_len, n_q, n_kv,
+                                head_dim, max_seq, scale, out, out_row_stride, workspace,
+                                workspace_len, kv_format, dtype, Q8Rope());
 }
 
 int kvb_attention_decode_q8_paged(kvb_stream_t stream, const void* q, size_t q_row_stride,
@@ -703,24 +774,46 @@ int kvb_attention_decode_q8_paged(kvb_stream_t stream, const void* q, size_t q_r
                                   size_t n_kv, size_t head_dim, float scale, void* out,
                                   size_t out_row_stride, void* workspace, size_t workspace_len,
                                   int kv_format, int dtype) {
-    KVB_CHECK_DTYPE(dtype);
-    KVB_CHECK(valid_kv_format(kv_format), "unknown KV format %d", kv_format);
-    GeneralDecodeArgs a;
-    int st = decode_args("attention_decode_q8_paged", a, q, q_row_stride, lens, n_seq, max_len, n_q,
-                         n_kv, head_dim, scale, out, out_row_stride);
+    return q8_decode_paged("attention_decode_q8_paged", stream, q, q_row_stride, k_pool, v_pool,
+                           k_scales, v_scales, pool_len, scale_len, block_table, max_blocks, block_size,
+                           lens, n_seq, max_len, n_q, n_kv, head_dim, scale, out, out_row_stride,
+                           workspace, workspace_len, kv_format, dtype, Q8Rope());
+}
+
+int kvb_rope_attention_decode_q8(kvb_stream_t stream, const void* qkv, size_t qkv_len,
+                                 const float* cos_t, const float* sin_t, size_t table_len, void* kc,
+                                 void* vc, float* ks, float* vs, size_t seq_stride, size_t cache_len,
+                                 size_t scale_len, const int32_t* lens, size_t n_seq, size_t max_len,
+                                 size_t n_q, size_t n_kv, size_t head_dim, size_t max_seq, float scale,
+                                 void* out, size_t out_row_stride, void* workspace,
+                                 size_t workspace_len, int kv_format, int dtype) {
+    Q8Rope r;
+    const int st = q8_rope("rope_attention_decode_q8", r, qkv, qkv_len, cos_t, sin_t, table_len, n_seq,
+                           n_q, n_kv, head_dim);
     if (st) return st;
-    Kv8Place c;
-    st = kv8_place_paged("attention_decode_q8_paged", c, k_pool, v_pool, k_scales, v_scales,
-                         pool_len, scale_len, block_table, max_blocks, block_size, n_seq, n_kv,
-                         head_dim);
+    return q8_decode_contiguous("rope_attention_decode_q8", stream, qkv, (n_q + 2 * n_kv) * head_dim,
+                                kc, vc, ks, vs, seq_stride, cache_len, scale_len, lens, n_seq, max_len,
+                                n_q, n_kv, head_dim, max_seq, scale, out, out_row_stride, workspace,
+                                workspace_len, kv_format, dtype, r);
+}
+
+int kvb_rope_attention_decode_q8_paged(kvb_stream_t stream, const void* qkv, size_t qkv_len,
+                                       const float* cos_t, const float* sin_t, size_t table_len,
+                                       void* k_pool, void* v_pool, float* k_scales, float* v_scales,
+                                       size_t pool_len, size_t scale_len, const int32_t* block_table,
+                                       size_t max_blocks, size_t block_size, const int32_t* lens,
+                                       size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
+                                       size_t head_dim, float scale, void* out, size_t out_row_stride,
+                                       void* workspace, size_t workspace_len, int kv_format,
+                                       int dtype) {
+    Q8Rope r;
+    const int st = q8_rope("rope_attention_decode_q8_paged", r, qkv, qkv_len, cos_t, sin_t, table_len,
+                           n_seq, n_q, n_kv, head_dim);
     if (st) return st;
-    KVB_CHECK(max_len <= max_blocks * block_size,
-              "attention_decode_q8_paged: max_len %zu exceeds %zu blocks of %zu", max_len,
-              max_blocks, block_size);
-    if (n_seq == 0) return KVB_OK;
-    const size_t cache_rows = scale_len;
-    return KVB_KV8_DISPATCH(launch_q8_decode, dtype, kv_format, stream, a, c, cache_rows, n_seq,
-                            workspace, workspace_len);
+    return q8_decode_paged("rope_attention_decode_q8_paged", stream, qkv, (n_q + 2 * n_kv) * head_dim,
+                           k_pool, v_pool, k_scales, v_scales, pool_len, scale_len, block_table,
+                           max_blocks, block_size, lens, n_seq, max_len, n_q, n_kv, head_dim, scale,
+                           out, out_row_stride, workspace, workspace_len, kv_format, dtype, r);
 }
 
 size_t kvb_attention_decode_shared_workspace_bytes(size_t n_seq, size_t shared_len, size_t max_own,

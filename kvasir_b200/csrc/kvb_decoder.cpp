@@ -10,8 +10,8 @@
 // fused into the following rmsnorm (kvb_add_rmsnorm); RoPE, the KV append and
 // decode attention are one launch (kvb_rope_attention_decode, in the step form
 // that starts its K/V reads before the preceding kernel completes) on contiguous
-// caches at head_dim 64.  With an 8-bit cache (kvb_decoder_use_q8_cache) they are two:
-// kvb_rope_kv_append_q8 and kvb_attention_decode_q8.  All device memory is caller-owned.
+// caches at head_dim 64, and on 8-bit caches (kvb_decoder_use_q8_cache) at head_dim 64 and
+// 128.  All device memory is caller-owned.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -167,27 +167,44 @@ static int record_step(kvb_decoder_s* d, kvb_stream_t s) {
             float* ksl = d->k_scales + (size_t)l * (codes / hd);
             float* vsl = d->v_scales + (size_t)l * (codes / hd);
             const int fmt = d->q8_format;
-            if (d->block_table) {
-                STEP(kvb_rope_kv_append_q8_paged(s, d->at(L.qkv), B * qkvd, B, 1, d->at<int32_t>(L.pos),
-                                                 d->cos_t, d->sin_t, table_len, kl, vl, ksl, vsl, codes,
-                                                 codes / hd, d->block_table, d->max_blocks,
-                                                 d->block_size, nq, nkv, hd, fmt, dt),
+            int32_t* lens = d->at<int32_t>(L.lens);
+            int32_t* pos = d->at<int32_t>(L.pos);
+            st = d->block_table
+                     ? kvb_rope_attention_decode_q8_paged(
+                           s, d->at(L.qkv), B * qkvd, d->cos_t, d->sin_t, table_len, kl, vl, ksl, vsl,
+                           codes, codes / hd, d->block_table, d->max_blocks, d->block_size, lens, B,
+                           max_seq, nq, nkv, hd, scale, d->at(L.attn), qd, d->at(L.attn_ws),
+                           L.attn_ws_len, fmt, dt)
+                     : kvb_rope_attention_decode_q8(s, d->at(L.qkv), B * qkvd, d->cos_t, d->sin_t,
+                                                    table_len, kl, vl, ksl, vsl, seq_stride, codes,
+                                                    codes / hd, lens, B, max_seq, nq, nkv, hd, max_seq,
+                                                    scale, d->at(L.attn), qd, d->at(L.attn_ws),
+                                                    L.attn_ws_len, fmt, dt);
+            if (st == KVB_OK) {
+                ++own;
+            } else if (st != KVB_ERR_UNSUPPORTED) {
+                return st;
+            } else if (d->block_table) {  // other shapes: the append, then the attention
+                STEP(kvb_rope_kv_append_q8_paged(s, d->at(L.qkv), B * qkvd, B, 1, pos, d->cos_t, d->sin_t,
+                                                 table_len, kl, vl, ksl, vsl, codes, codes / hd,
+                                                 d->block_table, d->max_blocks, d->block_size, nq, nkv,
+                                                 hd, fmt, dt),
                      false);
                 STEP(kvb_attention_decode_q8_paged(s, d->at(L.qkv), qkvd, kl, vl, ksl, vsl, codes,
                                                    codes / hd, d->block_table, d->max_blocks,
-                                                   d->block_size, d->at<int32_t>(L.lens), B, max_seq,
-                                                   nq, nkv, hd, scale, d->at(L.attn), qd,
-                                                   d->at(L.attn_ws), L.attn_ws_len, fmt, dt),
+                                                   d->block_size, lens, B, max_seq, nq, nkv, hd, scale,
+                                                   d->at(L.attn), qd, d->at(L.attn_ws), L.attn_ws_len,
+                                                   fmt, dt),
                      false);
             } else {
-                STEP(kvb_rope_kv_append_q8(s, d->at(L.qkv), B * qkvd, B, 1, d->at<int32_t>(L.pos),
-                                           d->cos_t, d->sin_t, table_len, kl, vl, ksl, vsl, seq_stride,
-                                           codes, codes / hd, nq, nkv, hd, max_seq, fmt, dt),
+                STEP(kvb_rope_kv_append_q8(s, d->at(L.qkv), B * qkvd, B, 1, pos, d->cos_t, d->sin_t,
+                                           table_len, kl, vl, ksl, vsl, seq_stride, codes, codes / hd,
+                                           nq, nkv, hd, max_seq, fmt, dt),
                      false);
                 STEP(kvb_attention_decode_q8(s, d->at(L.qkv), qkvd, kl, vl, ksl, vsl, seq_stride, codes,
-                                             codes / hd, d->at<int32_t>(L.lens), B, max_seq, nq, nkv, hd,
-                                             max_seq, scale, d->at(L.attn), qd, d->at(L.attn_ws),
-                                             L.attn_ws_len, fmt, dt),
+                                             codes / hd, lens, B, max_seq, nq, nkv, hd, max_seq, scale,
+                                             d->at(L.attn), qd, d->at(L.attn_ws), L.attn_ws_len, fmt,
+                                             dt),
                      false);
             }
         } else if (!d->block_table) {
@@ -223,8 +240,10 @@ static int record_step(kvb_decoder_s* d, kvb_stream_t s) {
                  false);
         }
         // the split-KV combine pass
-        own += d->q8_format >= 0 ? kvb::q8_join_launches(B, max_seq, nq, nkv, hd, d->at(L.attn_ws),
-                                                         L.attn_ws_len)
+        own += d->q8_format >= 0 ? (d->block_table && d->block_size % 16 != 0
+                                        ? 0  // the general kernel
+                                        : kvb::q8_join_launches(B, max_seq, nq, nkv, hd,
+                                                                d->at(L.attn_ws), L.attn_ws_len))
                                  : kvb::decode_combine_launches(B, max_seq, nq, nkv, hd,
                                                                 d->at(L.attn_ws), L.attn_ws_len);
         st = proj(d->at(L.attn), qd, d->w_o[l], d->at(L.o), H);

@@ -481,6 +481,44 @@ class Gpu:
             head_dim, scale, p[7], out_row_stride, p[8],
             workspace.nbytes if workspace is not None else 0, fmt, dtype_tag(q)))
 
+    def rope_attention_decode_q8(self, qkv, cos, sin, kc, vc, ks, vs, seq_stride, lens, max_len, n_q,
+                                 n_kv, head_dim, max_seq, out, out_row_stride, scale=None,
+                                 workspace=None):
+        """kvb_rope_attention_decode_q8: rope_kv_append_q8 of one row per sequence at positions
+        lens - 1, then attention_decode_q8, in one launch (qkv is left unrotated)."""
+        name = "rope_attention_decode_q8"
+        p = self._ptrs(name, qkv, cos, sin, kc, vc, ks, vs, lens, out, workspace)
+        fmt, table = self._check_q8(name, kc, vc, ks, vs), self._check_table(name, cos, sin)
+        n_seq = self._check_attention(name, qkv, (n_q + 2 * n_kv) * head_dim, lens, out,
+                                      out_row_stride, n_q * head_dim)
+        scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
+        check(self._lib.kvb_rope_attention_decode_q8(
+            self.stream.cuda_stream, p[0], qkv.numel(), p[1], p[2], table, p[3], p[4], p[5], p[6],
+            seq_stride, kc.numel(), ks.numel(), p[7], n_seq, max_len, n_q, n_kv, head_dim, max_seq,
+            scale, p[8], out_row_stride, p[9], workspace.nbytes if workspace is not None else 0, fmt,
+            dtype_tag(qkv)))
+
+    def rope_attention_decode_q8_paged(self, qkv, cos, sin, k_pool, v_pool, k_scales, v_scales,
+                                       block_table, max_blocks, block_size, lens, max_len, n_q, n_kv,
+                                       head_dim, out, out_row_stride, scale=None, workspace=None):
+        """kvb_rope_attention_decode_q8_paged: the same over 8-bit pools."""
+        name = "rope_attention_decode_q8_paged"
+        p = self._ptrs(name, qkv, cos, sin, k_pool, v_pool, k_scales, v_scales, block_table, lens, out,
+                       workspace)
+        fmt = self._check_q8(name, k_pool, v_pool, k_scales, v_scales)
+        table = self._check_table(name, cos, sin)
+        n_seq = self._check_attention(name, qkv, (n_q + 2 * n_kv) * head_dim, lens, out,
+                                      out_row_stride, n_q * head_dim)
+        self._check_types(name, torch.int32, block_table)
+        if block_table.numel() != n_seq * max_blocks:
+            raise ShapeError(f"{name}: one table row per sequence")
+        scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
+        check(self._lib.kvb_rope_attention_decode_q8_paged(
+            self.stream.cuda_stream, p[0], qkv.numel(), p[1], p[2], table, p[3], p[4], p[5], p[6],
+            k_pool.numel(), k_scales.numel(), p[7], max_blocks, block_size, p[8], n_seq, max_len, n_q,
+            n_kv, head_dim, scale, p[9], out_row_stride, p[10],
+            workspace.nbytes if workspace is not None else 0, fmt, dtype_tag(qkv)))
+
     # ------------------------------------------------ shared-prefix decode attention
     def attention_decode_shared_workspace_bytes(self, n_seq, shared_len, max_own, n_q, n_kv,
                                                 head_dim) -> int:

@@ -517,3 +517,98 @@ def test_decode_query_magnitudes(g, fmt, dtype):
     assert torch.equal(bad.isnan().all(-1).cpu(), rows)
     keep = ~rows.cuda()
     assert torch.equal(bad[keep], out.view(2, n_q, hd)[keep])
+
+
+@pytest.mark.parametrize("n_q,n_kv,hd,block", [
+    (32, 8, 64, 0), (32, 8, 64, 16), (6, 2, 64, 48), (16, 1, 64, 64), (8, 2, 128, 0), (16, 1, 128, 32),
+    (3, 3, 128, 16)])
+@pytest.mark.parametrize("fmt,dtype", [("int8", "bf16"), ("e4m3", "bf16"), ("int8", "f16"),
+                                       ("e4m3", "f16")])
+@pytest.mark.parametrize("workspace", [True, False])
+def test_fused_step_equals_append_then_decode(g, n_q, n_kv, hd, block, fmt, dtype, workspace):
+    """rope_attention_decode_q8: out, codes and scales bit for bit, at lengths around tiles and
+    chunks; qkv stays as it was.  The last sequence's position lies outside the RoPE tables."""
+    rng = np.random.default_rng(hd + block + n_q)
+    lens = [1, 2, 32, 33, 64, 65, 128, 129, 256, 257, 512, 513, 900, 1301, 1400]
+    n_seq, max_seq = len(lens), 1408
+    heads = n_q + 2 * n_kv
+    qkv = dev(normal16(rng, n_seq * heads * hd, dtype=dtype), dtype).view(n_seq, -1)
+    cos, sin = _tables(hd, 1399)
+    dcos, dsin = torch.from_numpy(cos).cuda(), torch.from_numpy(sin).cuda()
+    kc, ks = R.cache(rng, (n_seq, n_kv), max_seq, hd, fmt)
+    vc, vs = R.cache(rng, (n_seq, n_kv), max_seq, hd, fmt)
+    table = None
+    arrays = [kc, vc, ks, vs]
+    if block:
+        pools = []
+        for x in arrays:
+            pool, table = R.page(np.random.default_rng(3), x, block, table=table)
+            pools.append(pool)
+        arrays = pools
+        dt = torch.from_numpy(table).cuda()
+
+    def caches():
+        return [R.to_dev(arrays[0], fmt), R.to_dev(arrays[1], fmt), torch.from_numpy(arrays[2]).cuda(),
+                torch.from_numpy(arrays[3]).cuda()]
+    ld = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ws = torch.empty(max(16, g.attention_decode_q8_workspace_bytes(n_seq, max_seq, n_q, n_kv, hd)),
+                     dtype=torch.uint8, device="cuda") if workspace else None
+    want = torch.empty(n_seq, n_q * hd, dtype=R.TDT[dtype], device="cuda")
+    got = torch.empty_like(want)
+    a, b = caches(), caches()
+    rot = qkv.clone()
+    stride = n_kv * max_seq * hd
+    if block:
+        g.rope_kv_append_q8_paged(rot, n_seq, 1, ld - 1, dcos, dsin, *a, dt, dt.shape[1], block, n_q, n_kv,
+                                  hd)
+        assert g.device_error() == 4
+        g.attention_decode_q8_paged(rot, heads * hd, *a, dt, dt.shape[1], block, ld, max_seq, n_q, n_kv, hd,
+                                    want, n_q * hd, workspace=ws)
+        before = qkv.clone()
+        g.rope_attention_decode_q8_paged(qkv, dcos, dsin, *b, dt, dt.shape[1], block, ld, max_seq, n_q,
+                                         n_kv, hd, got, n_q * hd, workspace=ws)
+    else:
+        g.rope_kv_append_q8(rot, n_seq, 1, ld - 1, dcos, dsin, *a, stride, n_q, n_kv, hd, max_seq)
+        assert g.device_error() == 4
+        g.attention_decode_q8(rot, heads * hd, *a, stride, ld, max_seq, n_q, n_kv, hd, max_seq, want,
+                              n_q * hd, workspace=ws)
+        before = qkv.clone()
+        g.rope_attention_decode_q8(qkv, dcos, dsin, *b, stride, ld, max_seq, n_q, n_kv, hd, max_seq, got,
+                                   n_q * hd, workspace=ws)
+    assert g.device_error() == 4
+    assert torch.equal(qkv, before)
+    assert torch.equal(got, want)
+    for x, y in zip(a, b):
+        if x.dtype == torch.float32:
+            assert torch.equal(x.view(torch.int32), y.view(torch.int32))
+        else:
+            assert torch.equal(x.view(torch.int8), y.view(torch.int8))
+
+
+def test_fused_step_reports_bad_blocks_and_refuses_other_shapes(g):
+    from kvasir_b200.gpu import ShapeError, UnsupportedError
+    n_q, n_kv, hd = 4, 2, 64
+    rng = np.random.default_rng(2)
+    qkv = dev(normal16(rng, 2 * 8 * hd)).view(2, -1)
+    cos, sin = (torch.from_numpy(x).cuda() for x in _tables(hd, 64))
+    kp = torch.full((4, n_kv, 16, hd), 9, dtype=torch.int8, device="cuda")
+    vp, sk = kp.clone(), torch.full((4, n_kv, 16), 1.0, device="cuda")
+    sv = sk.clone()
+    table = torch.tensor([[0, -1], [1, 9]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([20, 17], dtype=torch.int32, device="cuda")
+    out = torch.empty(2, n_q * hd, dtype=torch.bfloat16, device="cuda")
+    g.rope_attention_decode_q8_paged(qkv, cos, sin, kp, vp, sk, sv, table, 2, 16, lens, 32, n_q, n_kv, hd,
+                                     out, n_q * hd)
+    assert g.device_error() == 4
+    assert bool((kp == 9).all()) and bool((vp == 9).all()) and bool((sk == 1).all())
+    # 16 keys of value 9 with scale 1, then keys that read as zeros: between 0 and 9
+    assert bool(((out >= 0) & (out <= 9)).all())
+    with pytest.raises(UnsupportedError):
+        g.rope_attention_decode_q8_paged(qkv, cos, sin, kp, vp, sk, sv, table.view(2, 2), 2, 8, lens, 16,
+                                         n_q, n_kv, hd, out, n_q * hd)
+    with pytest.raises(ShapeError):
+        g.rope_attention_decode_q8_paged(qkv[:, :-1].contiguous(), cos, sin, kp, vp, sk, sv, table, 2, 16,
+                                         lens, 32, n_q, n_kv, hd, out, n_q * hd)
+    with pytest.raises(ShapeError):
+        g.attention_decode_q8_paged(qkv.float(), n_q * hd, kp, vp, sk, sv, table, 2, 16, lens, 32, n_q,
+                                    n_kv, hd, out, n_q * hd)
