@@ -505,12 +505,11 @@ __global__ void __launch_bounds__(128, 3) attn_decode_kernel(const __grid_consta
 // from which it reads nothing (everything before that kernel has completed when it starts).
 // Only the grid's last CTA waits for it, before it ends: the grid then completes after the
 // prefix's kernel, and the join pass after it finds both kernels' parts, while the other CTAs
-// leave their slots at once and run beside the prefix's.  152 registers: beside a prefix CTA of four groups (576 threads x 80), one
-// CTA of this kernel fills the SM's register file.
+// leave their slots at once and run on the SMs that the prefix's grid leaves free.
 template <typename T>
-__global__ void __maxnreg__(152) attn_decode_part_kernel(const __grid_constant__ CUtensorMap kmap,
-                                                         const __grid_constant__ CUtensorMap vmap,
-                                                         DecodeArgs a) {
+__global__ void __launch_bounds__(128, 3)
+    attn_decode_part_kernel(const __grid_constant__ CUtensorMap kmap,
+                            const __grid_constant__ CUtensorMap vmap, DecodeArgs a) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2 * kDecWarps];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &

@@ -12,19 +12,21 @@
 //
 // A CTA takes kGroups row tiles against the same keys: 64-key K/V tiles come through a ring
 // once for all of them (TMA producer warp).  Each group has four warps, one row per thread,
-// which turn S (TMEM) into P (over it).  One warp issues every group's O += P V and next
-// S = Q K^T, taking whichever group's P is ready: in a fixed order the groups queue for it,
+// which turn S (TMEM) into P (over it).  An MMA warp for every two groups issues their
+// O += P V and next S = Q K^T, taking whichever group's P is ready: in a fixed order the
+// groups queue for it, one warp for four groups is busy 830 cycles of every group's tile,
 // and a softmax warp that issues for its own group takes ~1000 cycles a tile to do so.
-// What bounds the kernel is the exponentials (16 per SM and clock: the 134 M of 1024 rows x
-// 8 heads x 16384 keys are 30 us), so the layout is for independent streams: a group has one
-// S buffer and O, 128 TMEM columns, four groups fill an SM's 512, and the others compute
-// while one waits for its tensor work.  The groups of a CTA stay within the ring's depth of
-// each other; four CTAs of one group each do not -- the SM's schedulers favour the oldest,
-// whose slices end early and leave the youngest alone (measured 41 to 71 us for equal
-// slices).  A thread reads its scores from TMEM 32 at a time (maximum, then exponentials),
-// which keeps it near 80 registers, so that a CTA of the own keys' kernel fits beside four
-// groups.  There is no causal mask; a row's keys end at the prefix's end, or earlier for a
-// paged sequence shorter than the prefix.
+// What bounds the kernel is the softmax: 16 exponentials per SM and clock (the 134 M of 1024
+// rows x 8 heads x 16384 keys are 30 us; that pipe is 63 % busy) and the ~1000 cycles from a
+// tile's P to its next S.  So the layout is for independent streams: a group has one S buffer
+// and O, 128 TMEM columns, four groups fill an SM's 512, and the others compute while one
+// waits.  The groups of a CTA stay within the ring's depth of each other; four CTAs of one
+// group each do not -- the SM's schedulers favour the oldest, whose slices end early and leave
+// the youngest alone (measured 41 to 71 us for equal slices).  A thread reads its scores from
+// TMEM 32 at a time (maximum, then exponentials).  There is no causal mask; a row's keys end
+// at the prefix's end, or earlier for a paged sequence shorter than the prefix.
+// Measured on B200 with the own keys and the join: 256 sequences of 32 + 8 heads on 16384 keys
+// with up to 1000 own, 105 us (f16) and 111 us (bf16, P in two halves).
 #pragma once
 
 #include "attn_decode_q8.cuh"
@@ -39,7 +41,11 @@ __host__ __device__ constexpr int sp_stages(int groups) { return groups == 1 ? 2
 __host__ __device__ constexpr int sp_smem_bytes(int groups) {
     return groups * kSpQBytes + sp_stages(groups) * 2 * kSpKVBytes + 1024;
 }
-__host__ __device__ constexpr int sp_threads(int groups) { return groups * 128 + 64; }
+// one TMA warp, and an MMA warp for every two groups
+__host__ __device__ constexpr int sp_mma_warps(int groups) { return (groups + 1) / 2; }
+__host__ __device__ constexpr int sp_threads(int groups) {
+    return groups * 128 + 32 + 32 * sp_mma_warps(groups);
+}
 
 struct SharedBars {
     uint64_t q_full;
@@ -128,7 +134,7 @@ __device__ __forceinline__ void umma_pv_64(uint32_t d, uint32_t p, uint64_t v, u
 }
 
 template <typename T, int kGroups>
-__global__ void __maxnreg__(80)
+__global__ void __launch_bounds__(sp_threads(kGroups), kSpMaxGroups / kGroups)
     attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap qmap,
                               const __grid_constant__ CUtensorMap kmap,
                               const __grid_constant__ CUtensorMap vmap, SharedPrefixArgs a) {
@@ -140,7 +146,8 @@ __global__ void __maxnreg__(80)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~uintptr_t(1023));
     constexpr int kStages = sp_stages(kGroups);
-    constexpr int kMma = 0, kTma = 1;  // warps; the softmax warps come after them
+    // warps: the MMA issuers, the TMA producer, the softmax warps
+    constexpr int kMmas = sp_mma_warps(kGroups), kTma = kMmas, kSoftmax = kMmas + 1;
     constexpr uint32_t kTmemCols = kGroups * kSpTmemGroup;
     uint8_t* sq = smem;                       // Q of each group
     uint8_t* skv = sq + kGroups * kSpQBytes;  // [stage][K | V]
@@ -165,7 +172,7 @@ __global__ void __maxnreg__(80)
             mbar_init(&bars.s_full[g], 1);
             mbar_init(&bars.p_full[g], kSpRows);
         }
-        mbar_init(&bars.mma_done, 1);
+        mbar_init(&bars.mma_done, kMmas);
         s_err = 0;
         fence_mbar_init();
     }
@@ -174,7 +181,7 @@ __global__ void __maxnreg__(80)
         for (int i = rows * 8 + tid; i < kSpRows * 8; i += sp_threads(kGroups))
             reinterpret_cast<uint4*>(sq + g * kSpQBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
     fence_async_smem();
-    if (warp == kMma) tmem_alloc(&tmem_slot, kTmemCols);
+    if (warp == 0) tmem_alloc(&tmem_slot, kTmemCols);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -227,7 +234,7 @@ __global__ void __maxnreg__(80)
                 mbar_wait(&bars.q_full, 0);
             }
         }
-    } else if (warp == kMma) {
+    } else if (warp < kMmas) {
         // ------------------------------------------------------------ MMA issuer
         // The whole warp stays converged; one elected lane issues.  Per group P_j V_j, then
         // S_{j+1} into the columns that P_j was read from: one thread's MMAs execute in order.
@@ -242,20 +249,26 @@ __global__ void __maxnreg__(80)
                       dk0 + kStage * (j % kStages), idesc_s, &bars.s_full[g]);
         };
         bool ok = warp_all(mbar_wait(&bars.q_full, 0) && mbar_wait(&bars.kv_full[0], 0));
-        int next[kGroups];  // each group's tile whose P is awaited
-        int left = ok ? n_groups : 0;
+        // this warp's groups: warp, warp + kMmas; next: the tile whose P is awaited
+        constexpr int kMine = (kGroups + kMmas - 1) / kMmas;
+        int next[kMine];
+        int left = 0;
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-            next[g] = g < n_groups ? 0 : nt;
-            if (ok && g < n_groups) issue_s(g, 0);
+        for (int i = 0; i < kMine; ++i) {
+            const int g = warp + i * kMmas;
+            next[i] = g < n_groups ? 0 : nt;
+            if (ok && g < n_groups) {
+                issue_s(g, 0);
+                ++left;
+            }
         }
         uint64_t last = globaltimer_ns();
         int idle = 0;
         while (left > 0) {
             bool any = false;
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
-                const int j = next[g];
+            for (int i = 0; i < kMine; ++i) {
+                const int j = next[i], g = warp + i * kMmas;
                 if (j >= nt || !warp_all(mbar_test_wait(&bars.p_full[g], j & 1))) continue;
                 const bool more = j + 1 < nt;
                 if (more && !warp_all(mbar_test_wait(&bars.kv_full[(j + 1) % kStages],
@@ -269,7 +282,7 @@ __global__ void __maxnreg__(80)
                 if (more) issue_s(g, j + 1);
                 else umma_commit(&bars.s_full[g]);  // O is final
                 umma_commit(&bars.kv_empty[j % kStages]);
-                next[g] = j + 1;
+                next[i] = j + 1;
                 left -= more ? 0 : 1;
             }
             // a bounded wait: no group has moved for kWaitLimitNs, or another role has failed
@@ -290,9 +303,9 @@ __global__ void __maxnreg__(80)
         umma_commit(&bars.mma_done);
         mbar_wait(&bars.mma_done, 0);  // no MMA may still be running when TMEM is released
         __syncwarp();
-    } else if ((warp - 2) / 4 < n_groups) {
+    } else if ((warp - kSoftmax) / 4 < n_groups) {
         // ------------------------------------------------------------ softmax warps
-        const int grp = (warp - 2) / 4, quarter = warp % 4;  // a warp's TMEM lanes: 32 quarter ..
+        const int grp = (warp - kSoftmax) / 4, quarter = warp % 4;  // a warp's TMEM lanes: 32 quarter ..
         const int row = quarter * 32 + lane;
         const uint32_t t_s = tmem + grp * kSpTmemGroup + ((uint32_t)(quarter * 32) << 16);
         const uint32_t t_o = t_s + kSpTmemO;  // S, then P, at t_s
@@ -423,7 +436,7 @@ __global__ void __maxnreg__(80)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kMma) {
+    if (warp == 0) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
     }
