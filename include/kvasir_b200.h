@@ -421,7 +421,12 @@ int kvb_kv_read_q8_paged(kvb_stream_t stream, const void* k_pool, const void* v_
 /* Batched single-query decode attention over an 8-bit cache: kvb_attention_decode's
  * arguments and result (f32 scores, sums and accumulation) on the values that the
  * rows stand for.  Any head_dim up to 256, any group size; a block entry outside the
- * pool sets kvb_device_error code 4 and those keys read as zeros. */
+ * pool sets kvb_device_error code 4 and those keys read as zeros.  The tensor-core kernel
+ * takes head_dim 64 and 128 with n_q / n_kv <= 16, block_size a multiple of 16, codes 16-byte
+ * and q 8-byte aligned with q_row_stride a multiple of 4; a general kernel, several times
+ * slower, takes the rest.  The workspace (kvb_attention_decode_q8_workspace_bytes; NULL: no
+ * KV split) needs no initialisation and belongs to one call at a time: calls that may overlap
+ * on the GPU, replayed graphs among them, need one each. */
 int kvb_attention_decode_q8(kvb_stream_t stream, const void* q, size_t q_row_stride, const void* kc,
                             const void* vc, const float* ks, const float* vs, size_t seq_stride,
                             size_t cache_len, size_t scale_len, const int32_t* lens, size_t n_seq,
@@ -473,9 +478,15 @@ int kvb_rope_attention_decode_q8_paged(kvb_stream_t stream, const void* qkv, siz
  * the caches of kvb_attention_decode_paged; the first shared_len keys of every
  * sequence are the same, and are read through row 0 of the block table (whole blocks
  * of a prefix appear in every row, a block that the prefix ends in may be copied for
- * each sequence); lens[b] counts them, and a length below shared_len attends to
- * that many of them.  Both equal kvb_attention_decode(_paged) over the same keys up
- * to the order of the f32 sums.  Any head_dim up to 256, any group size. */
+ * each sequence); row 0 holds them whatever lens[0] is; lens[b] counts them, and a length
+ * below shared_len attends to that many of them (V rows of the prefix that hold a NaN or
+ * an infinity may then reach that sequence all the same).  Both equal
+ * kvb_attention_decode(_paged) over the same keys up to the order of the f32 sums.  Any
+ * head_dim up to 256, any group size.  The tensor-core kernels take head_dim 64 with
+ * n_q / n_kv <= 16, scale > 0, block_size a multiple of 64, 16-byte aligned q and caches,
+ * q_row_stride a multiple of 8, and a workspace of
+ * kvb_attention_decode_shared_workspace_bytes (no initialisation; one call at a time, as
+ * above); a general kernel, many times slower, takes the rest, NULL workspaces too. */
 int kvb_attention_decode_shared(kvb_stream_t stream, const void* q, size_t q_row_stride,
                                 const void* pk, const void* pv, size_t prefix_len,
                                 size_t prefix_rows, const void* kc, const void* vc,

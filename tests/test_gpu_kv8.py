@@ -43,6 +43,7 @@ def _rotated(bits, cos, sin, pos, t, n_q, n_kv, hd, dtype):
 SHAPES = [  # n_seq, t, n_q, n_kv, hd
     (1, 1, 32, 8, 64), (32, 1, 32, 8, 64), (3, 517, 32, 8, 64), (2, 5, 6, 2, 128),
     (2, 700, 4, 4, 128), (3, 4, 2, 1, 80), (2, 3, 3, 3, 256), (2, 3, 0, 2, 6), (1, 2, 16, 1, 2),
+    (2, 3, 64, 8, 128), (1, 5, 32, 33, 64),  # more chunks in a row than a CTA has threads
 ]
 
 
@@ -612,3 +613,88 @@ def test_fused_step_reports_bad_blocks_and_refuses_other_shapes(g):
     with pytest.raises(ShapeError):
         g.attention_decode_q8_paged(qkv.float(), n_q * hd, kp, vp, sk, sv, table, 2, 16, lens, 32, n_q,
                                     n_kv, hd, out, n_q * hd)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_unaligned_buffers_take_the_general_kernels(g, hd):
+    """Views that start one element (or one code) past an aligned address: the append gives the
+    same bits, the attention the f64 result."""
+    rng = np.random.default_rng(17)
+    n_q, n_kv, fmt, dtype, t, max_seq = 4, 2, "int8", "bf16", 3, 40
+    heads = n_q + 2 * n_kv
+    bits = normal16(rng, t * heads * hd)
+    cos, sin = (torch.from_numpy(x).cuda() for x in _tables(hd, max_seq))
+    pos = torch.tensor([30], dtype=torch.int32, device="cuda")
+    got = []
+    for shift in (0, 1):
+        q = torch.empty(t * heads * hd + 1, dtype=torch.bfloat16, device="cuda")[shift:shift + bits.size]
+        q.copy_(dev(bits))
+        cs = [torch.zeros(n_kv * max_seq * hd + 1, dtype=torch.int8, device="cuda")[shift:][
+            :n_kv * max_seq * hd] for _ in range(2)]
+        sc = [torch.zeros(n_kv * max_seq, device="cuda") for _ in range(2)]
+        g.rope_kv_append_q8(q, 1, t, pos, cos, sin, *cs, *sc, n_kv * max_seq * hd, n_q, n_kv, hd, max_seq)
+        ko = torch.empty(2 * n_kv * t * hd + 1, dtype=torch.bfloat16, device="cuda")[shift:]
+        kv = ko[:n_kv * t * hd], ko[n_kv * t * hd:2 * n_kv * t * hd]
+        g.kv_read_q8(*cs, *sc, n_kv * max_seq * hd, pos, 1, t, n_kv, hd, max_seq, *kv, t)
+        got.append([q.clone(), *[x.clone() for x in cs], *sc, *[x.clone() for x in kv]])
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+    lens = [33, 7]
+    q, qf, cache, kv_of, max_seq = _decode_case(rng, lens, n_q, n_kv, hd, fmt, dtype)
+    kc, vc, ks, vs = cache
+    shifted = []
+    for x in (kc, vc):
+        y = torch.empty(x.size + 1, dtype=torch.int8, device="cuda")[1:]
+        y.copy_(torch.from_numpy(x.ravel()))
+        shifted.append(y)
+    qs = torch.empty(q.size + 1, dtype=torch.bfloat16, device="cuda")[1:]
+    qs.copy_(dev(q))
+    out = torch.empty(2, n_q * hd, dtype=torch.bfloat16, device="cuda")
+    g.attention_decode_q8(qs, n_q * hd, *shifted, torch.from_numpy(ks).cuda(), torch.from_numpy(vs).cuda(),
+                          n_kv * max_seq * hd, torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                          max(lens), n_q, n_kv, hd, max_seq, out, n_q * hd)
+    R.check_attention(out, qf, kv_of, n_kv, R.default_scale(hd), dtype, W_EPS, q_eps=R.Q_EPS[fmt])
+    assert g.device_error() == 0
+
+
+def test_calls_on_two_streams_at_once(g):
+    """Two handles on two streams, each with a workspace of its own, many calls in flight."""
+    from kvasir_b200 import Gpu
+    rng = np.random.default_rng(41)
+    n_q, n_kv, hd, fmt = 32, 8, 64, "e4m3"
+    jobs = []
+    for lens in ([700, 1301, 64], [5, 2000, 900]):
+        q, qf, cache, kv_of, max_seq = _decode_case(rng, lens, n_q, n_kv, hd, fmt, "bf16")
+        want = _run_decode(g, q, cache, lens, n_q, n_kv, hd, max_seq, fmt, "bf16")
+        h = Gpu(0, stream=torch.cuda.Stream())
+        ws = torch.empty(max(16, h.attention_decode_q8_workspace_bytes(3, max(lens), n_q, n_kv, hd)),
+                         dtype=torch.uint8, device="cuda")
+        args = (dev(q), n_q * hd, R.to_dev(cache[0], fmt), R.to_dev(cache[1], fmt),
+                torch.from_numpy(cache[2]).cuda(), torch.from_numpy(cache[3]).cuda(), n_kv * max_seq * hd,
+                torch.tensor(lens, dtype=torch.int32, device="cuda"), max(lens), n_q, n_kv, hd, max_seq)
+        jobs.append((h, args, want, ws))
+    torch.cuda.synchronize()
+    outs = [[torch.empty_like(want) for _ in range(20)] for _, _, want, _ in jobs]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for (h, args, _, ws), o in zip(jobs, outs):
+            h.attention_decode_q8(*args, o[i], n_q * hd, workspace=ws)
+    torch.cuda.synchronize()
+    for (_, _, want, _), o in zip(jobs, outs):
+        assert all(torch.equal(x, want) for x in o)
+    assert g.device_error() == 0
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("scale", [0.0, -0.125])
+def test_decode_scale_of_either_sign(g, fmt, scale):
+    rng = np.random.default_rng(3)
+    n_q, n_kv, hd, lens = 8, 2, 64, [70, 300]
+    q, qf, cache, kv_of, max_seq = _decode_case(rng, lens, n_q, n_kv, hd, fmt, "bf16")
+    kc, vc, ks, vs = cache
+    out = torch.empty(2, n_q * hd, dtype=torch.bfloat16, device="cuda")
+    g.attention_decode_q8(dev(q), n_q * hd, R.to_dev(kc, fmt), R.to_dev(vc, fmt),
+                          torch.from_numpy(ks).cuda(), torch.from_numpy(vs).cuda(), n_kv * max_seq * hd,
+                          torch.tensor(lens, dtype=torch.int32, device="cuda"), max(lens), n_q, n_kv, hd,
+                          max_seq, out, n_q * hd, scale=scale)
+    R.check_attention(out, qf * (-1 if scale < 0 else 1), kv_of, n_kv, abs(scale), "bf16", W_EPS,
+                      q_eps=R.Q_EPS[fmt])

@@ -251,3 +251,42 @@ def test_strides_graph_and_stream(g, hd):
         torch.cuda.synchronize()
         assert torch.equal(out[:, :n_q * hd], want) and bool((out[:, n_q * hd:] == 1.0).all())
     assert g.device_error() == 0
+
+
+def test_two_streams_at_once_and_negative_scale(g):
+    from kvasir_b200 import Gpu
+    jobs = []
+    for seed, prefix, lens in ((1, 900, [70, 3, 640]), (2, 2000, [1, 0, 200])):
+        c = Case(np.random.default_rng(seed), prefix, lens, 32, 8, 64, "bf16")
+        want = c.contiguous(g)
+        h = Gpu(0, stream=torch.cuda.Stream())
+        t = [dev(x) for x in (c.q, c.pk, c.pv, c.kc, c.vc)]
+        jobs.append((c, h, t, want, c.ws(g, max(lens))))
+    outs = [[torch.empty_like(j[3]) for _ in range(10)] for j in jobs]
+    torch.cuda.synchronize()
+    for i in range(10):
+        for (c, h, (q, pk, pv, kc, vc), _, ws), o in zip(jobs, outs):
+            h.attention_decode_shared(q, 2048, pk, pv, c.prefix, c.rows, kc, vc, 8 * c.max_seq * 64, c.ld,
+                                      max(c.lens), 32, 8, 64, c.max_seq, o[i], 2048, workspace=ws)
+    torch.cuda.synchronize()
+    for (c, *_, want, _), o in zip(jobs, outs):
+        assert all(torch.equal(x, want) for x in o)
+    c, _, (q, pk, pv, kc, vc), _, ws = jobs[0]
+    for scale in (-0.125, 0.0):
+        out = c.out()
+        g.attention_decode_shared(q, 2048, pk, pv, c.prefix, c.rows, kc, vc, 8 * c.max_seq * 64, c.ld,
+                                  max(c.lens), 32, 8, 64, c.max_seq, out, 2048, scale=scale, workspace=ws)
+        # scores of -scale against -q are those of scale against q
+        R.check_attention(out, c.qf * (-1 if scale < 0 else 1), c.kv_of, 8, abs(scale), "bf16",
+                          W_EPS["bf16"])
+    assert g.device_error() == 0
+
+
+@pytest.mark.parametrize("n_q,n_kv", [(8, 8), (21, 3), (26, 2), (16, 1)])
+def test_groups_that_do_not_fill_a_tile(g, n_q, n_kv):
+    """Group sizes 1, 7, 13 and 16 over enough sequences for several CTAs of row tiles."""
+    rng = np.random.default_rng(n_q)
+    c = Case(rng, 200, [int(x) for x in rng.integers(0, 70, 300)], n_q, n_kv, 64, "bf16")
+    c.check(c.contiguous(g))
+    c.check(c.paged(g, 64))
+    assert g.device_error() == 0
