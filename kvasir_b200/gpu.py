@@ -361,13 +361,13 @@ class Gpu:
         f32 scales ks / vs, one per position and KV head).  cos = sin = None: no rotation."""
         name = "rope_kv_append_q8"
         p = self._ptrs(name, qkv, pos, cos, sin, kc, vc, ks, vs)
-        fmt, table = self._check_q8(name, kc, vc, ks, vs), self._check_table(name, cos, sin)
-        self._check_types(name, torch.int32, pos)
-        if pos.numel() != n_seq:
-            raise ShapeError(f"{name}: one position per sequence")
+        fmt, n, n_scales = self._check_q8(name, kc, vc, ks, vs)
+        table = self._check_table(name, cos, sin)
+        if pos.numel() != n_seq or pos.dtype is not torch.int32:
+            raise ShapeError(f"{name}: one int32 position per sequence")
         check(self._lib.kvb_rope_kv_append_q8(
             self.stream.cuda_stream, p[0], qkv.numel(), n_seq, t, p[1], p[2], p[3], table, p[4],
-            p[5], p[6], p[7], seq_stride, kc.numel(), ks.numel(), n_q, n_kv, head_dim, max_seq, fmt,
+            p[5], p[6], p[7], seq_stride, n, n_scales, n_q, n_kv, head_dim, max_seq, fmt,
             dtype_tag(qkv)))
 
     def rope_kv_append_q8_paged(self, qkv, n_seq, t, pos, cos, sin, k_pool, v_pool, k_scales,
@@ -377,15 +377,15 @@ class Gpu:
         head_dim] of codes and [n_blocks, n_kv, block_size] of scales."""
         name = "rope_kv_append_q8_paged"
         p = self._ptrs(name, qkv, pos, cos, sin, k_pool, v_pool, k_scales, v_scales, block_table)
-        fmt = self._check_q8(name, k_pool, v_pool, k_scales, v_scales)
+        fmt, n, n_scales = self._check_q8(name, k_pool, v_pool, k_scales, v_scales)
         table = self._check_table(name, cos, sin)
         self._check_types(name, torch.int32, pos, block_table)
         if pos.numel() != n_seq or block_table.numel() != n_seq * max_blocks:
             raise ShapeError(f"{name}: one position and one table row per sequence")
         check(self._lib.kvb_rope_kv_append_q8_paged(
             self.stream.cuda_stream, p[0], qkv.numel(), n_seq, t, p[1], p[2], p[3], table, p[4],
-            p[5], p[6], p[7], k_pool.numel(), k_scales.numel(), p[8], max_blocks, block_size, n_q,
-            n_kv, head_dim, fmt, dtype_tag(qkv)))
+            p[5], p[6], p[7], n, n_scales, p[8], max_blocks, block_size, n_q, n_kv, head_dim, fmt,
+            dtype_tag(qkv)))
 
     def kv_read_q8(self, kc, vc, ks, vs, seq_stride, pos, n_seq, t, n_kv, head_dim, max_seq, k_out,
                    v_out, out_rows):
@@ -393,53 +393,68 @@ class Gpu:
         0 .. t-1 of k_out / v_out [n_seq, n_kv, out_rows, head_dim]."""
         name = "kv_read_q8"
         p = self._ptrs(name, kc, vc, ks, vs, pos, k_out, v_out)
-        fmt = self._check_q8(name, kc, vc, ks, vs)
-        self._check_types(name, torch.int32, pos)
-        if pos.numel() != n_seq or k_out.dtype != v_out.dtype or k_out.numel() != v_out.numel():
-            raise ShapeError(f"{name}: one position per sequence, k_out and v_out alike")
+        fmt, n, n_scales = self._check_q8(name, kc, vc, ks, vs)
+        n_out = k_out.numel()
+        if (pos.numel() != n_seq or pos.dtype is not torch.int32 or v_out.dtype is not k_out.dtype
+                or v_out.numel() != n_out):
+            raise ShapeError(f"{name}: one int32 position per sequence, k_out and v_out alike")
         check(self._lib.kvb_kv_read_q8(
-            self.stream.cuda_stream, p[0], p[1], p[2], p[3], seq_stride, kc.numel(), ks.numel(),
-            p[4], n_seq, t, n_kv, head_dim, max_seq, p[5], p[6], k_out.numel(), out_rows, fmt,
-            dtype_tag(k_out)))
+            self.stream.cuda_stream, p[0], p[1], p[2], p[3], seq_stride, n, n_scales, p[4], n_seq, t,
+            n_kv, head_dim, max_seq, p[5], p[6], n_out, out_rows, fmt, dtype_tag(k_out)))
 
     def kv_read_q8_paged(self, k_pool, v_pool, k_scales, v_scales, block_table, max_blocks,
                          block_size, pos, n_seq, t, n_kv, head_dim, k_out, v_out, out_rows):
         """kvb_kv_read_q8_paged: kv_read_q8 through a block table."""
         name = "kv_read_q8_paged"
         p = self._ptrs(name, k_pool, v_pool, k_scales, v_scales, block_table, pos, k_out, v_out)
-        fmt = self._check_q8(name, k_pool, v_pool, k_scales, v_scales)
+        fmt, n, n_scales = self._check_q8(name, k_pool, v_pool, k_scales, v_scales)
         self._check_types(name, torch.int32, pos, block_table)
         if (pos.numel() != n_seq or block_table.numel() != n_seq * max_blocks
                 or k_out.dtype != v_out.dtype or k_out.numel() != v_out.numel()):
             raise ShapeError(f"{name}: one position and one table row per sequence, k_out and "
                              "v_out alike")
         check(self._lib.kvb_kv_read_q8_paged(
-            self.stream.cuda_stream, p[0], p[1], p[2], p[3], k_pool.numel(), k_scales.numel(), p[4],
-            max_blocks, block_size, p[5], n_seq, t, n_kv, head_dim, p[6], p[7], k_out.numel(),
-            out_rows, fmt, dtype_tag(k_out)))
+            self.stream.cuda_stream, p[0], p[1], p[2], p[3], n, n_scales, p[4], max_blocks,
+            block_size, p[5], n_seq, t, n_kv, head_dim, p[6], p[7], k_out.numel(), out_rows, fmt,
+            dtype_tag(k_out)))
 
     def attention_decode_q8_workspace_bytes(self, n_seq, max_len, n_q, n_kv, head_dim) -> int:
         return int(self._lib.kvb_attention_decode_q8_workspace_bytes(n_seq, max_len, n_q, n_kv,
                                                                      head_dim))
 
-    def _check_q8(self, name, kc, vc, ks, vs):
-        if kc.dtype is not vc.dtype or kc.numel() != vc.numel() or ks.numel() != vs.numel():
+    @staticmethod
+    def _check_q8(name, kc, vc, ks, vs):
+        """Format, codes and scales of an 8-bit cache (of K, and of V alike)."""
+        n, n_scales, kind = kc.numel(), ks.numel(), kc.dtype
+        if vc.dtype is not kind or vc.numel() != n or vs.numel() != n_scales:
             raise ShapeError(f"{name}: K and V caches (or their scales) differ")
-        self._check_types(name, torch.float32, ks, vs)
-        return kv_format(kc)
+        if ks.dtype is not torch.float32 or vs.dtype is not torch.float32:
+            raise ShapeError(f"{name}: scales must be float32")
+        if kind is torch.int8:
+            return L.KVB_KV_INT8, n, n_scales
+        return kv_format(kc), n, n_scales
 
     def _check_table(self, name, cos, sin):
         """Elements of the cos / sin tables (0 without)."""
+        if cos is None and sin is None:
+            return 0
         self._check_types(name, torch.float32, cos, sin)
-        if (cos is None) != (sin is None) or (cos is not None and cos.numel() != sin.numel()):
+        n = cos.numel() if cos is not None and sin is not None else -1
+        if n < 0 or sin.numel() != n:
             raise ShapeError(f"{name}: bad cos/sin table sizes")
-        return cos.numel() if cos is not None else 0
+        return n
 
     def _check_attention(self, name, q, q_row_stride, lens, out, out_row_stride, row, *caches):
         """lens is int32; q and out hold rows of `row` elements, their strides apart; one
         16-bit type."""
-        self._check_types(name, torch.int32, lens)
-        self._check_types(name, q.dtype, out, *caches)
+        kind = q.dtype
+        if lens.dtype is not torch.int32:
+            raise ShapeError(f"{name}: lengths must be int32")
+        if out.dtype is not kind:
+            raise ShapeError(f"{name}: out is {out.dtype}, q {kind}")
+        for t in caches:
+            if t.dtype is not kind:
+                raise ShapeError(f"{name}: a cache is {t.dtype}, q {kind}")
         n = lens.numel()
         if n and (q.numel() < (n - 1) * q_row_stride + row
                   or out.numel() < (n - 1) * out_row_stride + row):
@@ -452,13 +467,13 @@ class Gpu:
         """kvb_attention_decode_q8: attention_decode over an 8-bit cache."""
         name = "attention_decode_q8"
         p = self._ptrs(name, q, kc, vc, ks, vs, lens, out, workspace)
-        fmt = self._check_q8(name, kc, vc, ks, vs)
+        fmt, n, n_scales = self._check_q8(name, kc, vc, ks, vs)
         n_seq = self._check_attention(name, q, q_row_stride, lens, out, out_row_stride,
                                       n_q * head_dim)
         scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
         check(self._lib.kvb_attention_decode_q8(
-            self.stream.cuda_stream, p[0], q_row_stride, p[1], p[2], p[3], p[4], seq_stride,
-            kc.numel(), ks.numel(), p[5], n_seq, max_len, n_q, n_kv, head_dim, max_seq, scale, p[6],
+            self.stream.cuda_stream, p[0], q_row_stride, p[1], p[2], p[3], p[4], seq_stride, n,
+            n_scales, p[5], n_seq, max_len, n_q, n_kv, head_dim, max_seq, scale, p[6],
             out_row_stride, p[7], workspace.nbytes if workspace is not None else 0, fmt,
             dtype_tag(q)))
 
@@ -468,7 +483,7 @@ class Gpu:
         """kvb_attention_decode_q8_paged: attention_decode_paged over 8-bit pools."""
         name = "attention_decode_q8_paged"
         p = self._ptrs(name, q, k_pool, v_pool, k_scales, v_scales, block_table, lens, out, workspace)
-        fmt = self._check_q8(name, k_pool, v_pool, k_scales, v_scales)
+        fmt, n, n_scales = self._check_q8(name, k_pool, v_pool, k_scales, v_scales)
         n_seq = self._check_attention(name, q, q_row_stride, lens, out, out_row_stride,
                                       n_q * head_dim)
         self._check_types(name, torch.int32, block_table)
@@ -476,8 +491,8 @@ class Gpu:
             raise ShapeError(f"{name}: one table row per sequence")
         scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
         check(self._lib.kvb_attention_decode_q8_paged(
-            self.stream.cuda_stream, p[0], q_row_stride, p[1], p[2], p[3], p[4], k_pool.numel(),
-            k_scales.numel(), p[5], max_blocks, block_size, p[6], n_seq, max_len, n_q, n_kv,
+            self.stream.cuda_stream, p[0], q_row_stride, p[1], p[2], p[3], p[4], n, n_scales, p[5],
+            max_blocks, block_size, p[6], n_seq, max_len, n_q, n_kv,
             head_dim, scale, p[7], out_row_stride, p[8],
             workspace.nbytes if workspace is not None else 0, fmt, dtype_tag(q)))
 
@@ -488,13 +503,14 @@ class Gpu:
         lens - 1, then attention_decode_q8, in one launch (qkv is left unrotated)."""
         name = "rope_attention_decode_q8"
         p = self._ptrs(name, qkv, cos, sin, kc, vc, ks, vs, lens, out, workspace)
-        fmt, table = self._check_q8(name, kc, vc, ks, vs), self._check_table(name, cos, sin)
+        fmt, n, n_scales = self._check_q8(name, kc, vc, ks, vs)
+        table = self._check_table(name, cos, sin)
         n_seq = self._check_attention(name, qkv, (n_q + 2 * n_kv) * head_dim, lens, out,
                                       out_row_stride, n_q * head_dim)
         scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
         check(self._lib.kvb_rope_attention_decode_q8(
             self.stream.cuda_stream, p[0], qkv.numel(), p[1], p[2], table, p[3], p[4], p[5], p[6],
-            seq_stride, kc.numel(), ks.numel(), p[7], n_seq, max_len, n_q, n_kv, head_dim, max_seq,
+            seq_stride, n, n_scales, p[7], n_seq, max_len, n_q, n_kv, head_dim, max_seq,
             scale, p[8], out_row_stride, p[9], workspace.nbytes if workspace is not None else 0, fmt,
             dtype_tag(qkv)))
 
@@ -505,7 +521,7 @@ class Gpu:
         name = "rope_attention_decode_q8_paged"
         p = self._ptrs(name, qkv, cos, sin, k_pool, v_pool, k_scales, v_scales, block_table, lens, out,
                        workspace)
-        fmt = self._check_q8(name, k_pool, v_pool, k_scales, v_scales)
+        fmt, n, n_scales = self._check_q8(name, k_pool, v_pool, k_scales, v_scales)
         table = self._check_table(name, cos, sin)
         n_seq = self._check_attention(name, qkv, (n_q + 2 * n_kv) * head_dim, lens, out,
                                       out_row_stride, n_q * head_dim)
@@ -515,7 +531,7 @@ class Gpu:
         scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
         check(self._lib.kvb_rope_attention_decode_q8_paged(
             self.stream.cuda_stream, p[0], qkv.numel(), p[1], p[2], table, p[3], p[4], p[5], p[6],
-            k_pool.numel(), k_scales.numel(), p[7], max_blocks, block_size, p[8], n_seq, max_len, n_q,
+            n, n_scales, p[7], max_blocks, block_size, p[8], n_seq, max_len, n_q,
             n_kv, head_dim, scale, p[9], out_row_stride, p[10],
             workspace.nbytes if workspace is not None else 0, fmt, dtype_tag(qkv)))
 
