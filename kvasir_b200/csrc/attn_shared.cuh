@@ -152,7 +152,6 @@ __global__ void __launch_bounds__(sp_threads(kGroups), kSpMaxGroups / kGroups)
     uint8_t* sq = smem;                       // Q of each group
     uint8_t* skv = sq + kGroups * kSpQBytes;  // [stage][K | V]
 
-    asm volatile("griddepcontrol.launch_dependents;");
     const int kvh = blockIdx.x, split = blockIdx.y;
     const int tile0 = blockIdx.z * kGroups;  // this CTA's row tiles
     const int n_groups = min(kGroups, a.row_tiles - tile0);
@@ -186,6 +185,9 @@ __global__ void __launch_bounds__(sp_threads(kGroups), kSpMaxGroups / kGroups)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    // Only now may the chain behind this grid start: a later kernel of it that allocates TMEM
+    // ahead of its own wait then finds every CTA of this one with its columns.
+    asm volatile("griddepcontrol.launch_dependents;");
     const uint32_t fmt = Elem<T>::kDtype == KVB_BF16 ? 1u : 0u;
 
     if (warp == kTma) {
