@@ -698,3 +698,79 @@ def test_decode_scale_of_either_sign(g, fmt, scale):
                           max_seq, out, n_q * hd, scale=scale)
     R.check_attention(out, qf * (-1 if scale < 0 else 1), kv_of, n_kv, abs(scale), "bf16", W_EPS,
                       q_eps=R.Q_EPS[fmt])
+
+
+@pytest.mark.parametrize("hd", [64, 80])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_rows_past_32_bit_offsets(g, fmt, hd):
+    """The second sequence's rows lie more than 2^32 codes behind the first's, contiguous and in
+    blocks of a pool: append, read back, decode and the one-launch step as on a small cache, bit
+    for bit (hd 80: the general kernels)."""
+    n_q, n_kv, rows, t, block = 8, 2, 80, 70, 16
+    heads = n_q + 2 * n_kv
+    rng = np.random.default_rng(51)
+    cos, sin = (torch.from_numpy(x).cuda() for x in _tables(hd, rows))
+    qkv0 = dev(normal16(rng, 2 * t * heads * hd)).view(2 * t, -1)
+    step0 = dev(normal16(rng, 2 * heads * hd)).view(2, -1)
+    zero = torch.zeros(2, dtype=torch.int32, device="cuda")
+    lens = torch.full((2,), t + 1, dtype=torch.int32, device="cuda")
+    per = n_kv * rows * hd
+    per_block = n_kv * block * hd
+    blocks = rows // block
+
+    def run(stride, n, table=None):
+        kc, vc = (torch.empty(n, dtype=torch.int8, device="cuda").view(R.CODE[fmt]) for _ in range(2))
+        ks, vs = (torch.empty(n // hd, device="cuda") for _ in range(2))
+        qkv, step = qkv0.clone(), step0.clone()
+        ko, vo = (torch.empty(2, n_kv, t, hd, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        out, out2 = (torch.empty(2, n_q * hd, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        if table is None:
+            g.rope_kv_append_q8(qkv, 2, t, zero, cos, sin, kc, vc, ks, vs, stride, n_q, n_kv, hd, rows)
+            g.kv_read_q8(kc, vc, ks, vs, stride, zero, 2, t, n_kv, hd, rows, ko, vo, t)
+            g.attention_decode_q8(step, heads * hd, kc, vc, ks, vs, stride, lens - 1, t, n_q, n_kv, hd,
+                                  rows, out, n_q * hd)
+            if hd == 64:
+                g.rope_attention_decode_q8(step, cos, sin, kc, vc, ks, vs, stride, lens, t + 1, n_q, n_kv,
+                                           hd, rows, out2, n_q * hd)
+        else:
+            tab = (table, table.shape[1], block)
+            g.rope_kv_append_q8_paged(qkv, 2, t, zero, cos, sin, kc, vc, ks, vs, *tab, n_q, n_kv, hd)
+            g.kv_read_q8_paged(kc, vc, ks, vs, *tab, zero, 2, t, n_kv, hd, ko, vo, t)
+            g.attention_decode_q8_paged(step, heads * hd, kc, vc, ks, vs, *tab, lens - 1, t, n_q, n_kv, hd,
+                                        out, n_q * hd)
+            if hd == 64:
+                g.rope_attention_decode_q8_paged(step, cos, sin, kc, vc, ks, vs, *tab, lens, t + 1, n_q,
+                                                 n_kv, hd, out2, n_q * hd)
+        assert g.device_error() == 0
+        return (ko, vo, out) + ((out2,) if hd == 64 else ())
+
+    far = (2 ** 32 // hd + 5) * hd
+    want = run(per, 2 * per)
+    for x, y in zip(run(far, far + per), want):
+        assert torch.equal(x, y)
+    n_blocks = 2 ** 32 // per_block + 9
+    table = torch.arange(2 * blocks, dtype=torch.int32, device="cuda").view(2, blocks)
+    table[1] += n_blocks - 2 * blocks
+    for x, y in zip(run(0, n_blocks * per_block, table), want):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 80])
+def test_int8_codes_of_minus_128(g, hd):
+    """A cache written by something else may hold -128, which the append never does."""
+    rng = np.random.default_rng(52)
+    n_q, n_kv, lens = 8, 2, [100, 37]
+    q, qf, cache, kv_of, max_seq = _decode_case(rng, lens, n_q, n_kv, hd, "int8", "bf16")
+    kc, vc, ks, vs = cache
+    for x in (kc, vc):
+        x[rng.random(x.shape) < 0.3] = -128
+    out = _run_decode(g, q, cache, lens, n_q, n_kv, hd, max_seq, "int8", "bf16")
+    R.check_attention(out, qf, kv_of, n_kv, R.default_scale(hd), "bf16", W_EPS, q_eps=R.Q_EPS["int8"])
+    ko, vo = (torch.empty(2, n_kv, 30, hd, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    g.kv_read_q8(R.to_dev(kc, "int8"), R.to_dev(vc, "int8"), torch.from_numpy(ks).cuda(),
+                 torch.from_numpy(vs).cuda(), n_kv * max_seq * hd,
+                 torch.zeros(2, dtype=torch.int32, device="cuda"), 2, 30, n_kv, hd, max_seq, ko, vo, 30)
+    for got, c, s in ((ko, kc, ks), (vo, vc, vs)):
+        want = torch.from_numpy(c[:, :, :30].astype(np.float32) * s[:, :, :30, None]).to(torch.bfloat16)
+        assert torch.equal(got.cpu(), want)
+    assert g.device_error() == 0

@@ -290,3 +290,48 @@ def test_groups_that_do_not_fill_a_tile(g, n_q, n_kv):
     c.check(c.contiguous(g))
     c.check(c.paged(g, 64))
     assert g.device_error() == 0
+
+
+@pytest.mark.parametrize("hd", [64, 80])
+def test_rows_past_32_bit_offsets(g, hd):
+    """Own keys more than 2^32 elements apart, contiguous and in blocks of a pool: as on a small
+    cache, bit for bit."""
+    n_q, n_kv, prefix, own, block = 8, 2, 128, 128, 64
+    rng = np.random.default_rng(61)
+    q = dev(normal16(rng, 2 * n_q * hd)).view(2, -1)
+    rows = [dev(normal16(rng, n_kv * n * hd)).view(n_kv, n, hd) for n in (prefix, prefix, own, own, own, own)]
+    pk, pv, own_kv = rows[0], rows[1], (rows[2:4], rows[4:6])
+    lens = torch.tensor([100, 77], dtype=torch.int32, device="cuda")
+    ws = torch.empty(max(16, g.attention_decode_shared_workspace_bytes(2, prefix, own, n_q, n_kv, hd)),
+                     dtype=torch.uint8, device="cuda")
+    per, per_block = n_kv * own * hd, n_kv * block * hd
+
+    def contiguous(stride):
+        out = torch.empty(2, n_q * hd, dtype=torch.bfloat16, device="cuda")
+        kc, vc = (torch.empty(stride + per, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        for b in (0, 1):
+            for x, r in zip((kc, vc), own_kv[b]):
+                x[b * stride:b * stride + per].view(n_kv, own, hd).copy_(r)
+        g.attention_decode_shared(q, n_q * hd, pk, pv, prefix, prefix, kc, vc, stride, lens, 100, n_q, n_kv,
+                                  hd, own, out, n_q * hd, workspace=ws)
+        assert g.device_error() == 0
+        return out
+
+    def paged(n_blocks):
+        out = torch.empty(2, n_q * hd, dtype=torch.bfloat16, device="cuda")
+        kp, vp = (torch.empty(n_blocks, n_kv, block, hd, dtype=torch.bfloat16, device="cuda")
+                  for _ in range(2))
+        last = n_blocks - 1  # the prefix: the first and the last block; own keys: near both ends
+        table = torch.tensor([[0, last, 1, last - 1], [0, last, 2, last - 2]], dtype=torch.int32)
+        for x, p, i in ((kp, pk, 0), (vp, pv, 1)):
+            for j in (0, 1):
+                x[table[0, j]] = p[:, j * block:(j + 1) * block]
+                for b in (0, 1):
+                    x[table[b, 2 + j]] = own_kv[b][i][:, j * block:(j + 1) * block]
+        g.attention_decode_shared_paged(q, n_q * hd, kp, vp, table.cuda(), 4, block, prefix, lens + prefix,
+                                        prefix + 100, n_q, n_kv, hd, out, n_q * hd, workspace=ws)
+        assert g.device_error() == 0
+        return out
+
+    assert torch.equal(contiguous((2 ** 32 // hd + 3) * hd), contiguous(per))
+    assert torch.equal(paged(2 ** 32 // per_block + 9), paged(8))
