@@ -737,113 +737,149 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
     cluster_sync();  // no CTA leaves while its state may still be read
 }
 
-// Joins the partial states of every (sequence, KV head): parts 0 .. fixed - 1, which every
+// Joins the partial states of every (sequence, head): parts 0 .. fixed - 1, which every
 // sequence has, then one for each chunk of its keys past key0.  Written rows: those with more
 // than one part (write_all: every row, zeros where a sequence has none).  A programmatic
-// dependent of the kernel that writes the partials.  Threads are laid out as (part, four
-// neighbouring outputs): each requests its first parts' O, 16 bytes a load, before the CTA
-// turns the parts' (m, l) into weights, so that both reads share one memory latency; the
-// threads of an output then add up through shared memory.  Parts start on 16 bytes.
+// dependent of the kernel that writes the partials.  Latency bounds it, so a row is one warp's (or
+// W of its CTA's eight, parts w, w + W, ..., where there are more than 32): the lanes are laid
+// out as (part, four neighbouring outputs), each requests its first kAhead parts' O, 16 bytes
+// a load, beside the parts' (m, l), a part a lane, so that all reads share one latency and
+// nothing goes through shared memory.  Parts start on 16 bytes.  Measured in the calls that end
+// with it: 256 sequences x 32 heads of 9 parts 59.6 us, where a CTA per (sequence, KV head) with
+// the weights in shared memory took 64.5; 37 x 16 heads of 128 dims, 18.0 against 19.7.  16 loads
+// ahead instead of 8 where 8 reach all parts cost the many rows residency (62.1 us); where they
+// do not, 2048 rows of 18 parts: 22.0 us, two warps of 8 ahead 23.8, one of 8 ahead 23.7.
 struct JoinArgs {
     const float* ws;
     const int32_t* lens;
     int max_len, key0, chunk_keys;
     int fixed, max_parts, part_floats;
-    int n_kv, group, hd;
+    int n_kv, group;
     int write_all;
     uint16_t* out;
     long long out_row_stride;
 };
-constexpr int kJoinThreads = 256;
-constexpr int kJoinMaxParts = 512;  // weights: parts x group floats of shared memory
-constexpr int kJoinAhead = 4;       // parts whose O a thread requests ahead of the weights
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(JoinArgs a) {
-    extern __shared__ float w[];  // [parts][group]
-    __shared__ float inv_l[kQ8MaxGroup];
-    __shared__ float4 sums[kJoinThreads];
+constexpr int kJoinWarps = 8;
+constexpr int kJoinMaxParts = 512;
+// Grid (groups of kJoinWarps / W heads, sequence).
+template <typename T, int HD, int W, int kAhead>
+__global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) {
+    constexpr int kCols = HD / 4, kLanes = 32 / kCols;  // lanes of a row, parts side by side
+    __shared__ float ml[kJoinWarps][2];
+    __shared__ float4 sums[W > 1 ? kJoinWarps : 1][kCols];
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int kvh = blockIdx.x, b = blockIdx.y, G = a.group, hd = a.hd;
-    const int len = q8_len(a.lens, a.max_len, b);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int G = a.group, b = blockIdx.y, n_q = a.n_kv * G;
+    const int w = warp % W;
+    const int head = blockIdx.x * (kJoinWarps / W) + warp / W;
+    const bool have = head < n_q;
+    const int kvh = min(head, n_q - 1) / G, r = min(head, n_q - 1) - kvh * G;
+    const int per4 = a.part_floats / 4;
+    const float* base = a.ws + ((size_t)b * a.n_kv + kvh) * a.max_parts * (size_t)a.part_floats;
+    const float4* o4 = reinterpret_cast<const float4*>(base + r * HD) + lane % kCols;
+    const int side = lane / kCols;
+    // this warp's parts: w + W q
+    auto part = [&](int q) { return w + W * q; };
+    int len = a.lens[b];
+    float4 ahead[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+        const int p = part(kLanes * k + side);
+        ahead[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p < a.fixed) ahead[k] = o4[(size_t)p * per4];
+    }
+    if (len < 0 || len > a.max_len) {
+        if (threadIdx.x == 0) raise_dev_error(kDevErrBadLength);
+        len = len < 0 ? 0 : a.max_len;
+    }
     const int own = len > a.key0 ? (len - a.key0 + a.chunk_keys - 1) / a.chunk_keys : 0;
     const int parts = a.fixed + own;
-    if (!a.write_all && parts <= 1) return;
-    T* outb = reinterpret_cast<T*>(a.out) + (size_t)b * a.out_row_stride + (size_t)kvh * G * hd;
-    const size_t per = (size_t)a.part_floats;
-    const float* base = a.ws + ((size_t)b * a.n_kv + kvh) * a.max_parts * per;
-    const int cols = G * hd / 4;                          // groups of four outputs
-    const int lanes = max(1, kJoinThreads / cols);        // threads that share a column's parts
-    const int pl = threadIdx.x / cols;                    // this thread's (lanes > 1)
-    const bool busy = lanes == 1 || pl < lanes;
-    const int p0 = lanes == 1 ? 0 : pl, c0 = lanes == 1 ? threadIdx.x : threadIdx.x - pl * cols;
-    const float4* o4 = reinterpret_cast<const float4*>(base) + c0;
-    const size_t per4 = per / 4;
-    float4 ahead[kJoinAhead];
+    if (!a.write_all && parts <= 1) return;  // the same for the whole CTA
 #pragma unroll
-    for (int k = 0; k < kJoinAhead; ++k)
-        if (busy && c0 < cols && p0 + k * lanes < parts) ahead[k] = o4[(p0 + k * lanes) * per4];
-    for (int r = threadIdx.x >> 5; r < G; r += kJoinThreads / 32) {  // a warp per head
-        const int lane = threadIdx.x & 31;
-        float M = -INFINITY, L = 0.f;
-        for (int p = lane; p < parts; p += 32) M = fmaxf(M, base[p * per + G * hd + r]);
-        M = warp_max(M);
-        for (int p = lane; p < parts; p += 32) {
-            const float mp = base[p * per + G * hd + r], lp = base[p * per + G * hd + G + r];
-            const float f = mp == -INFINITY ? 0.f : exp2f(mp - M);
-            w[p * G + r] = f;
-            L += lp != lp ? lp : lp * f;
-        }
-        L = warp_sum(L);
-        if (lane == 0) inv_l[r] = L == 0.f ? 0.f : 1.f / L;  // no keys at all: zeros
+    for (int k = 0; k < kAhead; ++k) {
+        const int p = part(kLanes * k + side);
+        if (p >= a.fixed && p < parts) ahead[k] = o4[(size_t)p * per4];
     }
-    __syncthreads();
+    float M = -INFINITY, L = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     // a part without weight may hold anything (0 * NaN where every key was masked)
-    auto add = [](float4& x, const float4& o, float f) {
+    auto add = [&](const float4& o, float f) {
         if (f == 0.f) return;
         x.x += o.x * f;
         x.y += o.y * f;
         x.z += o.z * f;
         x.w += o.w * f;
     };
-    auto store = [&](int c, const float4& x) {
-        const float f = inv_l[4 * c / hd];
-        outb[4 * c] = Elem<T>::from_f(x.x * f);
-        outb[4 * c + 1] = Elem<T>::from_f(x.y * f);
-        outb[4 * c + 2] = Elem<T>::from_f(x.z * f);
-        outb[4 * c + 3] = Elem<T>::from_f(x.w * f);
+    auto rescale = [&](float f) {
+        x.x *= f;
+        x.y *= f;
+        x.z *= f;
+        x.w *= f;
     };
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (busy && c0 < cols) {
-        const int r = 4 * c0 / hd;
+    for (int q0 = 0; part(q0) < parts; q0 += 32) {  // 32 parts at a time, one per lane
+        const int p = part(q0 + lane);
+        float mp = -INFINITY, lp = 0.f;
+        if (p < parts) {
+            mp = base[(size_t)p * a.part_floats + G * HD + r];
+            lp = base[(size_t)p * a.part_floats + G * HD + G + r];
+        }
+        const float Mn = fmaxf(M, warp_max(mp));
+        const float f = mp == -INFINITY ? 0.f : exp2f(mp - Mn);
+        const float down = M == -INFINITY ? 0.f : exp2f(M - Mn);
+        if (q0 > 0) {
+            L *= down;
+            if (M != Mn) rescale(down);
+        }
+        M = Mn;
+        L += warp_sum(lp != lp ? lp : lp * f);
 #pragma unroll
-        for (int k = 0; k < kJoinAhead; ++k)
-            if (p0 + k * lanes < parts) add(x, ahead[k], w[(p0 + k * lanes) * G + r]);
-#pragma unroll 4
-        for (int p = p0 + kJoinAhead * lanes; p < parts; p += lanes) add(x, o4[p * per4], w[p * G + r]);
-    }
-    if (lanes == 1) {
-        if (c0 < cols) store(c0, x);
-        for (int c = c0 + kJoinThreads; c < cols; c += kJoinThreads) {  // more columns than threads
-            x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (int p = 0; p < parts; ++p)
-                add(x, reinterpret_cast<const float4*>(base)[p * per4 + c], w[p * G + 4 * c / hd]);
-            store(c, x);
+        for (int k = 0; k < 32 / kLanes; ++k) {
+            const int q = kLanes * k + side;
+            const float fq = __shfl_sync(0xffffffffu, f, q);
+            if (part(q0 + kLanes * k) >= parts) break;
+            if (k < kAhead && q0 == 0) add(ahead[k < kAhead ? k : 0], fq);
+            else if (part(q0 + q) < parts) add(o4[(size_t)part(q0 + q) * per4], fq);
         }
-        return;
     }
-    sums[threadIdx.x] = x;
-    __syncthreads();
-    if (pl == 0) {
-        for (int k = 1; k < lanes; ++k) {
-            const float4 y = sums[k * cols + c0];
-            x.x += y.x;
-            x.y += y.y;
-            x.z += y.z;
-            x.w += y.w;
+    if (kLanes == 2) {  // the two sides' parts
+        x.x += __shfl_xor_sync(0xffffffffu, x.x, 16);
+        x.y += __shfl_xor_sync(0xffffffffu, x.y, 16);
+        x.z += __shfl_xor_sync(0xffffffffu, x.z, 16);
+        x.w += __shfl_xor_sync(0xffffffffu, x.w, 16);
+    }
+    if constexpr (W > 1) {
+        if (lane == 0) {
+            ml[warp][0] = M;
+            ml[warp][1] = L;
         }
-        store(c0, x);
+        if (lane < kCols) sums[warp][lane] = x;
+        __syncthreads();
+        if (w != 0) return;
+        float Mr = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < W; ++i) Mr = fmaxf(Mr, ml[warp + i][0]);
+        L = 0.f;
+        x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const float f = ml[warp + i][0] == -INFINITY ? 0.f : exp2f(ml[warp + i][0] - Mr);
+            const float li = ml[warp + i][1];
+            L += li != li ? li : li * f;
+            add(sums[warp + i][lane % kCols], f);
+        }
+    }
+    if (!have || lane >= kCols) return;
+    const float inv = L == 0.f ? 0.f : 1.f / L;  // no keys at all: zeros
+    T* out = reinterpret_cast<T*>(a.out) + (size_t)b * a.out_row_stride + (size_t)head * HD + 4 * lane;
+    if ((reinterpret_cast<uintptr_t>(out) & 7) == 0) {
+        *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack(x.x * inv, x.y * inv),
+                                                    Elem<T>::pack(x.z * inv, x.w * inv));
+    } else {
+        out[0] = Elem<T>::from_f(x.x * inv);
+        out[1] = Elem<T>::from_f(x.y * inv);
+        out[2] = Elem<T>::from_f(x.z * inv);
+        out[3] = Elem<T>::from_f(x.w * inv);
     }
 }
 

@@ -180,13 +180,16 @@ __global__ void __launch_bounds__(sp_threads(kGroups), kSpMaxGroups / kGroups)
         for (int i = rows * 8 + tid; i < kSpRows * 8; i += sp_threads(kGroups))
             reinterpret_cast<uint4*>(sq + g * kSpQBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
     fence_async_smem();
+    // Nothing global is read or written, and no TMEM is taken, while the kernel before may run.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp == 0) tmem_alloc(&tmem_slot, kTmemCols);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    // Only now may the chain behind this grid start: a later kernel of it that allocates TMEM
-    // ahead of its own wait then finds every CTA of this one with its columns.
+    // Only now may the chain behind this grid start: its first kernel relies on everything before
+    // this one, and a later one that allocates TMEM ahead of its own wait then finds every CTA of
+    // this one with its columns.
     asm volatile("griddepcontrol.launch_dependents;");
     const uint32_t fmt = Elem<T>::kDtype == KVB_BF16 ? 1u : 0u;
 

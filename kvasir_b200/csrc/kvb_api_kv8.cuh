@@ -280,15 +280,21 @@ static Q8Plan q8_plan(size_t n_seq, size_t max_len, size_t n_q, size_t n_kv, siz
     return p;
 }
 
-static int launch_join(kvb_stream_t stream, const JoinArgs& a, size_t n_seq, int dtype) {
-    const dim3 grid((unsigned)a.n_kv, (unsigned)n_seq);
-    const size_t smem = (size_t)a.max_parts * a.group * sizeof(float);
-    const cudaError_t e =
-        dtype == KVB_BF16
-            ? launch_pdl(attn_join_kernel<__nv_bfloat16>, grid, dim3(kJoinThreads), smem, stream, a)
-            : launch_pdl(attn_join_kernel<__half>, grid, dim3(kJoinThreads), smem, stream, a);
-    if (e != cudaSuccess) return cuda_fail(e, "attention join launch");
-    return KVB_OK;
+template <typename T, int HD>
+static int launch_join(kvb_stream_t stream, const JoinArgs& a, size_t n_seq) {
+    // parts that one load a lane reaches, and the warps of 16 loads that reach all of them
+    const int side = 128 / HD;
+    const int w = a.max_parts <= 16 * side ? 1 : a.max_parts <= 32 * side ? 2
+                  : a.max_parts <= 64 * side ? 4 : 8;
+    const int rows = kJoinWarps / w;
+    const dim3 grid((unsigned)((a.n_kv * a.group + rows - 1) / rows), (unsigned)n_seq);
+    auto* kernel = a.max_parts <= 8 * side ? attn_join_kernel<T, HD, 1, 8>
+                   : w == 1                ? attn_join_kernel<T, HD, 1, 16>
+                   : w == 2                ? attn_join_kernel<T, HD, 2, 16>
+                   : w == 4                ? attn_join_kernel<T, HD, 4, 16>
+                                           : attn_join_kernel<T, HD, 8, 16>;
+    const cudaError_t e = launch_pdl(kernel, grid, dim3(32 * kJoinWarps), 0, stream, a);
+    return e == cudaSuccess ? KVB_OK : cuda_fail(e, "attention join launch");
 }
 
 template <typename T, int kFmt, int HD, int NT>
@@ -345,11 +351,10 @@ static int launch_q8_tensor(kvb_stream_t stream, Q8DecodeArgs& a, size_t n_seq, 
     j.part_floats = q8_part_floats(a.group, HD);
     j.n_kv = a.c.n_kv;
     j.group = a.group;
-    j.hd = HD;
     j.write_all = 0;
     j.out = a.out;
     j.out_row_stride = a.out_row_stride;
-    return launch_join(stream, j, n_seq, Elem<T>::kDtype);
+    return launch_join<T, HD>(stream, j, n_seq);
 }
 
 // The tensor-core kernel where shape and alignment allow it (cache_rows: rows of the code
@@ -459,9 +464,9 @@ static int launch_shared_prefix(kvb_stream_t stream, const CUtensorMap& qmap, co
     set_max_smem(kernel, sp_smem_bytes(kGroups));
     const dim3 grid((unsigned)s.n_kv, (unsigned)s.splits,
                     (unsigned)((s.row_tiles + kGroups - 1) / kGroups));
-    kernel<<<grid, sp_threads(kGroups), sp_smem_bytes(kGroups), stream>>>(qmap, kmap, vmap, s);
-    KVB_CHECK_LAUNCH("attention_decode_shared prefix launch");
-    return KVB_OK;
+    const cudaError_t e = launch_pdl(kernel, grid, dim3(sp_threads(kGroups)),
+                                     (size_t)sp_smem_bytes(kGroups), stream, qmap, kmap, vmap, s);
+    return e == cudaSuccess ? KVB_OK : cuda_fail(e, "attention_decode_shared prefix launch");
 }
 
 template <typename T>
@@ -553,7 +558,7 @@ static int launch_shared_tensor(kvb_stream_t stream, const GeneralDecodeArgs& a,
         cudaError_t e;
         if (p.splits > 0) {
             e = launch_pdl(kernel, grid, dim3(128), kDecSmemBytes, stream, kmap, vmap, d);
-        } else {  // nothing before it in this call: an ordinary launch
+        } else {  // no kernel before it that has waited for the ones before: an ordinary launch
             kernel<<<grid, 128, kDecSmemBytes, stream>>>(kmap, vmap, d);
             e = cudaGetLastError();
         }
@@ -570,11 +575,10 @@ static int launch_shared_tensor(kvb_stream_t stream, const GeneralDecodeArgs& a,
     j.part_floats = p.part_floats;
     j.n_kv = a.n_kv;
     j.group = group;
-    j.hd = 64;
     j.write_all = 1;
     j.out = a.out;
     j.out_row_stride = a.out_row_stride;
-    return launch_join(stream, j, n_seq, dtype);
+    return launch_join<T, 64>(stream, j, n_seq);
 }
 
 // The tensor-core kernels where shape, alignment and workspace allow them (own_rows: rows of 64
