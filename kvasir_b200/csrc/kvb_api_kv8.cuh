@@ -424,24 +424,28 @@ static SharedPlan shared_plan(size_t n_seq, size_t prefix, size_t max_own, size_
     p.n_tiles = (int)((prefix + kSpKeys - 1) / kSpKeys);
     p.groups = p.row_tiles >= 3 ? 4 : p.row_tiles;
     p.splits = 0;
-    // Slices: the number that takes the least time by a model fitted on B200 (us): a slice takes
-    // 1.45 per 64-key tile however many of the four groups an SM holds are busy, and about four
-    // tiles more to start and end; all slices and the own keys (half of the worst case, at 4.5
-    // TB/s) share the SMs, and a fifth of a slice's time is not covered by the own keys; a
-    // slice adds its rows' partials (264 bytes written and read, ~3
-    // TB/s) to the join.  32 sequences, 4096 keys, by slices 4 / 8 / 16 / 32: 33 / 22 / 18 / 23
-    // us; 256 sequences, 16384 keys, up to 1000 own, 4 / 6 / 12 / 24: 128 / 106 / 120 / 144.
-    const double slots = (double)num_sms() * (kSpMaxGroups / p.groups);
-    const double pairs = (double)((p.row_tiles + p.groups - 1) / p.groups) * (double)n_kv;
-    const double own_us = 0.5 * (double)n_seq * (double)max_own * (double)n_kv * 256.0 / 4.5e6;
-    const double join_us = 0.05 + (double)n_seq * (double)n_q * 264.0 * 2.0 / 3.0e6;
+    // Slices: the number that takes the least time by a model fitted on B200 (us; 28 shapes x 1 to
+    // 64 slices, n_kv 1 to 8, both types: the choice is 1.8 % slower than the best on average,
+    // 12 % at worst).  A slice takes 0.77 + 0.19 per row tile that shares its SM for each 64-key
+    // tile, and 3.6 to start and end.  All slices and the own keys (half of the worst case, at
+    // 5.75 TB/s) share the SMs, and a seventh of a slice's time is not covered by the own keys.
+    // A slice adds its rows' partials (264 bytes written and read, 3.1 TB/s) to the join.  32
+    // sequences, 4096 keys, 128 own, by slices 4 / 8 / 16 / 32: 22.0 / 15.8 / 12.7 / 13.7 us; 256
+    // sequences, 16384 keys, up to 1000 own, 4 / 6 / 12 / 24: 124 / 97 / 107 / 133.
+    const size_t pairs = (size_t)((p.row_tiles + p.groups - 1) / p.groups) * n_kv;
+    const size_t sms = (size_t)num_sms(), most_ctas = (size_t)(kSpMaxGroups / p.groups);
+    const double own_us = 0.5 * (double)n_seq * (double)max_own * (double)n_kv * 256.0 / 5.75e6;
+    const double join_us = 0.007 + (double)n_seq * (double)n_q * 264.0 * 2.0 / 3.1e6;
     double best = 1e30;
     for (int s = 1; s <= p.n_tiles && s <= 64; ++s) {
-        const double slice = 1.45 * ((p.n_tiles + s - 1) / s + 4);
-        const double waves = (double)(size_t)((pairs * s + slots - 1) / slots);
-        const double share = pairs * s * slice / slots + own_us;
+        const size_t ctas = pairs * s;
+        const size_t per_sm = ctas >= most_ctas * sms ? most_ctas : (ctas + sms - 1) / sms;
+        const double slice =
+            (0.77 + 0.19 * (double)(p.groups * per_sm)) * ((p.n_tiles + s - 1) / s) + 3.6;
+        const double waves = (double)((ctas + per_sm * sms - 1) / (per_sm * sms));
+        const double share = (double)ctas * slice / (double)(per_sm * sms) + own_us;
         const double cost =
-            (share > waves * slice ? share : waves * slice) + 0.2 * slice + s * join_us;
+            (share > waves * slice ? share : waves * slice) + 0.15 * slice + s * join_us;
         if (cost < best) {
             best = cost;
             p.splits = s;
