@@ -40,10 +40,7 @@ constexpr int kQ8TilesBytes = kQ8Warps * kQ8WarpBytes;
 constexpr int kQ8ScaleBytes = kQ8Warps * kQ8Stages * 2 * 64 * 4;
 constexpr int kQ8CtasPerSm = 3;
 constexpr int kQ8MaxGroup = 16;
-// tiles, scales, a chunk's folded O (group x head_dim floats), alignment slack
-__host__ __device__ constexpr int q8_smem_bytes(int hd, int nt) {
-    return kQ8TilesBytes + kQ8ScaleBytes + 8 * nt * hd * 4 + 1024;
-}
+constexpr int kQ8SmemBytes = kQ8TilesBytes + kQ8ScaleBytes + 1024;  // with alignment slack
 
 // Floats of one part of the workspace (O, m, l of a group), a multiple of four.
 __host__ __device__ constexpr int q8_part_floats(int group, int hd) {
@@ -62,7 +59,6 @@ struct Q8DecodeArgs {
     float* ws;       // split partials: per part O[group][hd], m[group], l[group], padding
     int chunk_keys;  // keys per CTA, a multiple of kQ8Warps tiles
     int max_chunks;
-    int fold;        // chunks of a (sequence, KV head) folded through a cluster
     int piece;       // rows per tensor copy: a whole tile, or gcd(block_size, tile) paged
     int bs_shift;    // paged: log2 of block_size, or -1
     int total_rows;  // rows of the code arrays (a row past the end reads as zeros)
@@ -204,8 +200,7 @@ __device__ __forceinline__ uint32_t q8_smem_off(int r, int ch) {
                     : (uint32_t)(r * 128 + ((ch ^ (r & 7)) << 4));
 }
 
-// Grid (KV head, sequence, chunk slot), or with a.fold (chunk slot, KV head, sequence) in
-// clusters of max_chunks CTAs; slots count chunks from the end of the sequence, so full
+// Grid (KV head, sequence, chunk slot); slots count chunks from the end of the sequence, so full
 // chunks are dispatched first (as attn_decode.cuh).
 template <typename T, int kFmt, int HD, int NT, bool kRope>
 __global__ void __launch_bounds__(128, kQ8CtasPerSm)
@@ -217,15 +212,12 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[kQ8Warps][kQ8Stages][2];  // K tile and scales; V tile and scales
     __shared__ float w_ml[kQ8Warps][2][kQ8MaxGroup];
-    __shared__ float fold_ml[2][kQ8MaxGroup];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~uintptr_t(1023));
     asm volatile("griddepcontrol.launch_dependents;");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, c = lane & 3;
-    const int slot = a.fold ? (int)blockIdx.x : (int)blockIdx.z;
-    const int kvh = a.fold ? (int)blockIdx.y : (int)blockIdx.x;
-    const int b = a.fold ? (int)blockIdx.z : (int)blockIdx.y;
+    const int kvh = blockIdx.x, b = blockIdx.y;
     const int G = a.group;
     if (threadIdx.x < kQ8Warps * kQ8Stages * 2)
         mbar_init(&bars[0][0][0] + threadIdx.x, 1 + 32);  // one expect_tx, 32 scale arrivals
@@ -235,211 +227,410 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
 
     const int len = q8_len(a.lens, a.max_len, b);
     const int n_chunks = (len + a.chunk_keys - 1) / a.chunk_keys;
-    const int from_end = a.max_chunks - 1 - slot;
+    const int from_end = a.max_chunks - 1 - (int)blockIdx.z;
     T* outb = reinterpret_cast<T*>(a.out) + (size_t)b * a.out_row_stride + (size_t)kvh * G * HD;
-    if (len == 0) {  // no keys: a zero row (the whole cluster returns here)
+    if (len == 0) {  // no keys: a zero row
         if (from_end == 0)
             for (int i = threadIdx.x; i < G * HD; i += blockDim.x) outb[i] = Elem<T>::from_f(0.f);
         return;
     }
-    const bool active = from_end < n_chunks;
+    if (from_end >= n_chunks) return;
     uint8_t* ring = smem + warp * kQ8WarpBytes;
     float* ring_scales = reinterpret_cast<float*>(smem + kQ8TilesBytes) + warp * kQ8Stages * 128;
     // this warp's O for the merge, [8 NT][HD] over its own tiles
     float* wo = reinterpret_cast<float*>(ring);
-    float* fold_o = reinterpret_cast<float*>(smem + kQ8TilesBytes + kQ8ScaleBytes);
-    if (active) {
-        const int chunk = n_chunks - 1 - from_end;
-        const int key_begin = chunk * a.chunk_keys;
-        const int key_end = min(len, key_begin + a.chunk_keys);
-        const int row_base = (int)(b * a.c.seq_rows + (long long)kvh * a.c.max_seq);
-        const int pshift = __ffs(a.piece) - 1;
-        int rope_p = -1;  // the new token's position (-1: none, or outside the tables)
-        if (kRope) {
-            rope_p = len - 1;
-            if (rope_p >= a.rope_max_pos) {
-                if (threadIdx.x == 0) raise_dev_error(kDevErrBadPosition);
-                rope_p = -1;
-            }
+    const int chunk = n_chunks - 1 - from_end;
+    const int key_begin = chunk * a.chunk_keys;
+    const int key_end = min(len, key_begin + a.chunk_keys);
+    const int row_base = (int)(b * a.c.seq_rows + (long long)kvh * a.c.max_seq);
+    const int pshift = __ffs(a.piece) - 1;
+    int rope_p = -1;  // the new token's position (-1: none, or outside the tables)
+    if (kRope) {
+        rope_p = len - 1;
+        if (rope_p >= a.rope_max_pos) {
+            if (threadIdx.x == 0) raise_dev_error(kDevErrBadPosition);
+            rope_p = -1;
         }
-        const bool appends = kRope && rope_p >= 0 && chunk == n_chunks - 1;  // CTA-uniform
+    }
+    const bool appends = kRope && rope_p >= 0 && chunk == n_chunks - 1;  // CTA-uniform
 
-        // Paged: this lane's piece of the next tile to be requested, read a tile ahead.
-        auto block_of = [&](int kt0) -> int {
-            const int k = kt0 + (lane << pshift);
-            if (!a.c.block_table || lane >= (KT >> pshift) || k >= key_end) return 0;
-            const int lb = a.bs_shift >= 0 ? k >> a.bs_shift : k / a.c.block_size;
-            return a.c.block_table[(size_t)b * a.c.max_blocks + lb];
-        };
-        int blk = block_of(key_begin + warp * KT);
-        // The tile that is requested next: its pieces, this lane's piece's row, and the rows of
-        // this lane's two keys (-1: none, their scales are zero).
-        int n_pieces = 0, row = 0, key_row[KT / 32];
-        auto place = [&](int kt0) {
-            const int nk = min(KT, key_end - kt0);
-            if (!a.c.block_table) {
-                n_pieces = 1;
-                row = row_base + kt0;
-#pragma unroll
-                for (int u = 0; u < KT / 32; ++u)
-                    key_row[u] = lane + 32 * u < nk ? row + lane + 32 * u : -1;
-                return;
-            }
-            n_pieces = (nk + a.piece - 1) >> pshift;
-            row = a.total_rows;  // past the end: zeros
-            if (lane < n_pieces) {
-                if (blk < 0 || blk >= a.c.n_blocks)
-                    raise_dev_error(kDevErrBadPosition);
-                else {
-                    const int k = kt0 + (lane << pshift);
-                    row = (blk * a.c.n_kv + kvh) * a.c.block_size +
-                          (a.bs_shift >= 0 ? k & (a.c.block_size - 1) : k % a.c.block_size);
-                }
-            }
-            blk = block_of(kt0 + kQ8Warps * KT);  // of the tile that is placed next
-#pragma unroll
-            for (int u = 0; u < KT / 32; ++u) {
-                const int k = lane + 32 * u;
-                const int r0 = __shfl_sync(0xffffffffu, row, k >> pshift);
-                key_row[u] = k < nk && r0 < a.total_rows ? r0 + (k & (a.piece - 1)) : -1;
-            }
-        };
-        // Requests the placed tile's K (or V) codes by tensor copies and scales by 4-byte
-        // copies, all counted on the tile's barrier.
-        auto request = [&](const CUtensorMap& map, uint8_t* tile, const float* scales, float* dst,
-                           uint64_t* bar) {
-            if (lane == 0) mbar_expect_tx(bar, (uint32_t)(n_pieces * a.piece * HD));
-            __syncwarp();
-            if (lane < n_pieces) tma_load_2d(tile + (lane << pshift) * HD, &map, bar, 0, row);
+    // Paged: this lane's piece of the next tile to be requested, read a tile ahead.
+    auto block_of = [&](int kt0) -> int {
+        const int k = kt0 + (lane << pshift);
+        if (!a.c.block_table || lane >= (KT >> pshift) || k >= key_end) return 0;
+        const int lb = a.bs_shift >= 0 ? k >> a.bs_shift : k / a.c.block_size;
+        return a.c.block_table[(size_t)b * a.c.max_blocks + lb];
+    };
+    int blk = block_of(key_begin + warp * KT);
+    // The tile that is requested next: its pieces, this lane's piece's row, and the rows of
+    // this lane's two keys (-1: none, their scales are zero).
+    int n_pieces = 0, row = 0, key_row[KT / 32];
+    auto place = [&](int kt0) {
+        const int nk = min(KT, key_end - kt0);
+        if (!a.c.block_table) {
+            n_pieces = 1;
+            row = row_base + kt0;
 #pragma unroll
             for (int u = 0; u < KT / 32; ++u)
-                cp_async4(smem_u32(dst + lane + 32 * u), scales + max(key_row[u], 0),
-                          key_row[u] >= 0 ? 4 : 0);
-            cp_async_arrive(bar);
-        };
-        auto request_k = [&](int st) {
-            request(kmap, ring + st * 2 * kQ8TileBytes, a.c.ks, ring_scales + st * 128,
-                    &bars[warp][st][0]);
-        };
-        auto request_v = [&](int st) {
-            request(vmap, ring + (st * 2 + 1) * kQ8TileBytes, a.c.vs, ring_scales + st * 128 + 64,
-                    &bars[warp][st][1]);
-        };
-        // The first tiles; the one that holds the new key waits until that row is written (it is
-        // its warp's last).
-        auto first_tiles = [&](bool holding) {
-#pragma unroll
-            for (int i = 0; i < kQ8Stages; ++i) {
-                const int kt0 = key_begin + (warp + i * kQ8Warps) * KT;
-                if (kt0 < key_end && (appends && rope_p < kt0 + KT) == holding) {
-                    place(kt0);
-                    request_k(i);
-                    request_v(i);
-                }
-            }
-        };
-        first_tiles(false);
-        if (appends) {
-            size_t crow = 0, head_rows = 0;
-            if (warp < 2 && kv8_row(a.c, b, rope_p, crow, head_rows, threadIdx.x == 0)) {
-                crow += (size_t)kvh * head_rows;
-                const T* in = reinterpret_cast<const T*>(a.q) + (size_t)b * a.q_row_stride +
-                              (size_t)(a.c.n_kv * (G + warp) + kvh) * HD;
-                if (warp == 0)
-                    q8_append_row<T, kFmt, HD>(in, a.rope_cos + (size_t)rope_p * (HD / 2),
-                                               a.rope_sin + (size_t)rope_p * (HD / 2),
-                                               a.c.kc + crow * HD, a.c.ks + crow);
-                else
-                    q8_append_row<T, kFmt, HD>(in, nullptr, nullptr, a.c.vc + crow * HD, a.c.vs + crow);
-            }
-            // the tensor copies read these rows through the async proxy
-            asm volatile("fence.proxy.async.global;" ::: "memory");
-            __syncthreads();
-            first_tiles(true);
+                key_row[u] = lane + 32 * u < nk ? row + lane + 32 * u : -1;
+            return;
         }
+        n_pieces = (nk + a.piece - 1) >> pshift;
+        row = a.total_rows;  // past the end: zeros
+        if (lane < n_pieces) {
+            if (blk < 0 || blk >= a.c.n_blocks)
+                raise_dev_error(kDevErrBadPosition);
+            else {
+                const int k = kt0 + (lane << pshift);
+                row = (blk * a.c.n_kv + kvh) * a.c.block_size +
+                      (a.bs_shift >= 0 ? k & (a.c.block_size - 1) : k % a.c.block_size);
+            }
+        }
+        blk = block_of(kt0 + kQ8Warps * KT);  // of the tile that is placed next
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u) {
+            const int k = lane + 32 * u;
+            const int r0 = __shfl_sync(0xffffffffu, row, k >> pshift);
+            key_row[u] = k < nk && r0 < a.total_rows ? r0 + (k & (a.piece - 1)) : -1;
+        }
+    };
+    // Requests the placed tile's K (or V) codes by tensor copies and scales by 4-byte
+    // copies, all counted on the tile's barrier.
+    auto request = [&](const CUtensorMap& map, uint8_t* tile, const float* scales, float* dst,
+                       uint64_t* bar) {
+        if (lane == 0) mbar_expect_tx(bar, (uint32_t)(n_pieces * a.piece * HD));
+        __syncwarp();
+        if (lane < n_pieces) tma_load_2d(tile + (lane << pshift) * HD, &map, bar, 0, row);
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u)
+            cp_async4(smem_u32(dst + lane + 32 * u), scales + max(key_row[u], 0),
+                      key_row[u] >= 0 ? 4 : 0);
+        cp_async_arrive(bar);
+    };
+    auto request_k = [&](int st) {
+        request(kmap, ring + st * 2 * kQ8TileBytes, a.c.ks, ring_scales + st * 128,
+                &bars[warp][st][0]);
+    };
+    auto request_v = [&](int st) {
+        request(vmap, ring + (st * 2 + 1) * kQ8TileBytes, a.c.vs, ring_scales + st * 128 + 64,
+                &bars[warp][st][1]);
+    };
+    // The first tiles; the one that holds the new key waits until that row is written (it is
+    // its warp's last).
+    auto first_tiles = [&](bool holding) {
+#pragma unroll
+        for (int i = 0; i < kQ8Stages; ++i) {
+            const int kt0 = key_begin + (warp + i * kQ8Warps) * KT;
+            if (kt0 < key_end && (appends && rope_p < kt0 + KT) == holding) {
+                place(kt0);
+                request_k(i);
+                request_v(i);
+            }
+        }
+    };
+    first_tiles(false);
+    if (appends) {
+        size_t crow = 0, head_rows = 0;
+        if (warp < 2 && kv8_row(a.c, b, rope_p, crow, head_rows, threadIdx.x == 0)) {
+            crow += (size_t)kvh * head_rows;
+            const T* in = reinterpret_cast<const T*>(a.q) + (size_t)b * a.q_row_stride +
+                          (size_t)(a.c.n_kv * (G + warp) + kvh) * HD;
+            if (warp == 0)
+                q8_append_row<T, kFmt, HD>(in, a.rope_cos + (size_t)rope_p * (HD / 2),
+                                           a.rope_sin + (size_t)rope_p * (HD / 2),
+                                           a.c.kc + crow * HD, a.c.ks + crow);
+            else
+                q8_append_row<T, kFmt, HD>(in, nullptr, nullptr, a.c.vc + crow * HD, a.c.vs + crow);
+        }
+        // the tensor copies read these rows through the async proxy
+        asm volatile("fence.proxy.async.global;" ::: "memory");
+        __syncthreads();
+        first_tiles(true);
+    }
 
-        // Q fragments (B operand): column g = head 8 nt + g, dims 16 j + 4c .. + 3.  int8: the
-        // high bytes, then the low ones; e4m3: two f16 pairs.
-        uint32_t qf[DT][NT][2];
-        float qs[NT][2];  // score factor of heads 8 nt + 2c, + 1
+    // Q fragments (B operand): column g = head 8 nt + g, dims 16 j + 4c .. + 3.  int8: the
+    // high bytes, then the low ones; e4m3: two f16 pairs.
+    uint32_t qf[DT][NT][2];
+    float qs[NT][2];  // score factor of heads 8 nt + 2c, + 1
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int h = 8 * nt + g;
-            const T* qr = reinterpret_cast<const T*>(a.q) + (size_t)b * a.q_row_stride +
-                          (size_t)(kvh * G + min(h, G - 1)) * HD;
-            uint2 v[DT];
+    for (int nt = 0; nt < NT; ++nt) {
+        const int h = 8 * nt + g;
+        const T* qr = reinterpret_cast<const T*>(a.q) + (size_t)b * a.q_row_stride +
+                      (size_t)(kvh * G + min(h, G - 1)) * HD;
+        uint2 v[DT];
 #pragma unroll
-            for (int j = 0; j < DT; ++j)
-                v[j] = h < G ? *reinterpret_cast<const uint2*>(qr + 16 * j + 4 * c) : make_uint2(0u, 0u);
-            if (kRope && rope_p >= 0) {
-                // rotate_half in registers: chunk j pairs with chunk j + DT / 2, the same lane
+        for (int j = 0; j < DT; ++j)
+            v[j] = h < G ? *reinterpret_cast<const uint2*>(qr + 16 * j + 4 * c) : make_uint2(0u, 0u);
+        if (kRope && rope_p >= 0) {
+            // rotate_half in registers: chunk j pairs with chunk j + DT / 2, the same lane
 #pragma unroll
-                for (int j = 0; j < DT / 2; ++j) {
-                    const size_t at = (size_t)rope_p * (HD / 2) + 16 * j + 4 * c;
-                    const float4 cs = *reinterpret_cast<const float4*>(a.rope_cos + at);
-                    const float4 sn = *reinterpret_cast<const float4*>(a.rope_sin + at);
-                    auto rotate2 = [](uint32_t& lo, uint32_t& hi, float c0, float c1, float s0, float s1) {
-                        const float2 x = Elem<T>::unpack(lo), y = Elem<T>::unpack(hi);
-                        lo = Elem<T>::pack(rot_a(x.x, y.x, c0, s0), rot_a(x.y, y.y, c1, s1));
-                        hi = Elem<T>::pack(rot_b(x.x, y.x, c0, s0), rot_b(x.y, y.y, c1, s1));
-                    };
-                    rotate2(v[j].x, v[j + DT / 2].x, cs.x, cs.y, sn.x, sn.y);
-                    rotate2(v[j].y, v[j + DT / 2].y, cs.z, cs.w, sn.z, sn.w);
-                }
+            for (int j = 0; j < DT / 2; ++j) {
+                const size_t at = (size_t)rope_p * (HD / 2) + 16 * j + 4 * c;
+                const float4 cs = *reinterpret_cast<const float4*>(a.rope_cos + at);
+                const float4 sn = *reinterpret_cast<const float4*>(a.rope_sin + at);
+                auto rotate2 = [](uint32_t& lo, uint32_t& hi, float c0, float c1, float s0, float s1) {
+                    const float2 x = Elem<T>::unpack(lo), y = Elem<T>::unpack(hi);
+                    lo = Elem<T>::pack(rot_a(x.x, y.x, c0, s0), rot_a(x.y, y.y, c1, s1));
+                    hi = Elem<T>::pack(rot_b(x.x, y.x, c0, s0), rot_b(x.y, y.y, c1, s1));
+                };
+                rotate2(v[j].x, v[j + DT / 2].x, cs.x, cs.y, sn.x, sn.y);
+                rotate2(v[j].y, v[j + DT / 2].y, cs.z, cs.w, sn.z, sn.w);
             }
-            float f = a.scale_log2;
-            if (kFmt == KVB_KV_INT8) {
-                uint32_t mx = 0;  // the head's largest magnitude, as a bit pattern
-#pragma unroll
-                for (int j = 0; j < DT; ++j) {
-                    const float2 x = Elem<T>::unpack(v[j].x), y = Elem<T>::unpack(v[j].y);
-                    mx = max(max(mx, max(abs_bits(x.x), abs_bits(x.y))),
-                             max(abs_bits(y.x), abs_bits(y.y)));
-                }
-                mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float big = fmaxf(__uint_as_float(mx), 0x1p-100f);
-                const float up = __fdiv_rn(32639.f, big);
-                // a NaN or an infinity among the elements: every score of the head is NaN
-                f = mx < 0x7f800000u ? f * __fdiv_rn(big, 32639.f) : __uint_as_float(0x7fc00000u);
-#pragma unroll
-                for (int j = 0; j < DT; ++j) {
-                    const float2 x = Elem<T>::unpack(v[j].x), y = Elem<T>::unpack(v[j].y);
-                    const int i0 = __float2int_rn(x.x * up), i1 = __float2int_rn(x.y * up);
-                    const int i2 = __float2int_rn(y.x * up), i3 = __float2int_rn(y.y * up);
-                    v[j].x = bytes4((i0 + 128) >> 8, (i1 + 128) >> 8, (i2 + 128) >> 8, (i3 + 128) >> 8);
-                    v[j].y = bytes4(i0, i1, i2, i3);  // i - 256 hi, in -128 .. 127
-                }
-            } else if (Elem<T>::kDtype == KVB_BF16) {
-                uint32_t mx = 0;  // largest exponent of the head's elements
-#pragma unroll
-                for (int j = 0; j < DT; ++j)
-                    mx = max(max(mx, max(v[j].x & 0x7fffu, (v[j].x >> 16) & 0x7fffu)),
-                             max(v[j].y & 0x7fffu, (v[j].y >> 16) & 0x7fffu));
-                mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                // biased exponent, kept where 2^(14 - e) and its inverse are normal numbers
-                const int e = min(max((int)(mx >> 7), 16), 254);
-                const float up = __uint_as_float((uint32_t)(268 - e) << 23);  // 2^(141 - e)
-                f *= __uint_as_float((uint32_t)(e - 14) << 23);               // 2^(e - 141)
-#pragma unroll
-                for (int j = 0; j < DT; ++j) {
-                    const float2 x = Elem<T>::unpack(v[j].x), y = Elem<T>::unpack(v[j].y);
-                    v[j].x = f16x2(x.x * up, x.y * up);
-                    v[j].y = f16x2(y.x * up, y.y * up);
-                }
-            }
+        }
+        float f = a.scale_log2;
+        if (kFmt == KVB_KV_INT8) {
+            uint32_t mx = 0;  // the head's largest magnitude, as a bit pattern
 #pragma unroll
             for (int j = 0; j < DT; ++j) {
-                qf[j][nt][0] = v[j].x;
-                qf[j][nt][1] = v[j].y;
+                const float2 x = Elem<T>::unpack(v[j].x), y = Elem<T>::unpack(v[j].y);
+                mx = max(max(mx, max(abs_bits(x.x), abs_bits(x.y))),
+                         max(abs_bits(y.x), abs_bits(y.y)));
             }
-            qs[nt][0] = __shfl_sync(0xffffffffu, f, 8 * c);
-            qs[nt][1] = __shfl_sync(0xffffffffu, f, 8 * c + 4);
+            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float big = fmaxf(__uint_as_float(mx), 0x1p-100f);
+            const float up = __fdiv_rn(32639.f, big);
+            // a NaN or an infinity among the elements: every score of the head is NaN
+            f = mx < 0x7f800000u ? f * __fdiv_rn(big, 32639.f) : __uint_as_float(0x7fc00000u);
+#pragma unroll
+            for (int j = 0; j < DT; ++j) {
+                const float2 x = Elem<T>::unpack(v[j].x), y = Elem<T>::unpack(v[j].y);
+                const int i0 = __float2int_rn(x.x * up), i1 = __float2int_rn(x.y * up);
+                const int i2 = __float2int_rn(y.x * up), i3 = __float2int_rn(y.y * up);
+                v[j].x = bytes4((i0 + 128) >> 8, (i1 + 128) >> 8, (i2 + 128) >> 8, (i3 + 128) >> 8);
+                v[j].y = bytes4(i0, i1, i2, i3);  // i - 256 hi, in -128 .. 127
+            }
+        } else if (Elem<T>::kDtype == KVB_BF16) {
+            uint32_t mx = 0;  // largest exponent of the head's elements
+#pragma unroll
+            for (int j = 0; j < DT; ++j)
+                mx = max(max(mx, max(v[j].x & 0x7fffu, (v[j].x >> 16) & 0x7fffu)),
+                         max(v[j].y & 0x7fffu, (v[j].y >> 16) & 0x7fffu));
+            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            // biased exponent, kept where 2^(14 - e) and its inverse are normal numbers
+            const int e = min(max((int)(mx >> 7), 16), 254);
+            const float up = __uint_as_float((uint32_t)(268 - e) << 23);  // 2^(141 - e)
+            f *= __uint_as_float((uint32_t)(e - 14) << 23);               // 2^(e - 141)
+#pragma unroll
+            for (int j = 0; j < DT; ++j) {
+                const float2 x = Elem<T>::unpack(v[j].x), y = Elem<T>::unpack(v[j].y);
+                v[j].x = f16x2(x.x * up, x.y * up);
+                v[j].y = f16x2(y.x * up, y.y * up);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < DT; ++j) {
+            qf[j][nt][0] = v[j].x;
+            qf[j][nt][1] = v[j].y;
+        }
+        qs[nt][0] = __shfl_sync(0xffffffffu, f, 8 * c);
+        qs[nt][1] = __shfl_sync(0xffffffffu, f, 8 * c + 4);
+    }
+
+    float o[DT][NT][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        m[nt][0] = m[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < DT; ++j) o[j][nt][0] = o[j][nt][1] = o[j][nt][2] = o[j][nt][3] = 0.f;
+    }
+    int ev = 14;  // biased exponent of the largest V scale seen; O is in units of 2^(ev - 140)
+    // Two tiles per warp in flight, K and V on barriers of their own: the K of the tile
+    // after next is requested once the scores are out of this one, its V once P V has read
+    // this V.
+    bool ok = true;
+    int it = 0;
+    bool k_failed = false;
+    for (int kt0 = key_begin + warp * KT; kt0 < key_end; kt0 += kQ8Warps * KT, ++it) {
+        const int st = it % kQ8Stages;
+        const uint32_t phase = (it / kQ8Stages) & 1;
+        const int nk = min(KT, key_end - kt0);
+        const int kt_next = kt0 + kQ8Stages * kQ8Warps * KT;
+        const bool more = kt_next < key_end;
+        const uint32_t kb = smem_u32(ring + st * 2 * kQ8TileBytes), vb = kb + kQ8TileBytes;
+        const float* ks = ring_scales + st * 128;
+        const float* vs = ks + 64;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][st][0], phase));
+        if (!ok) {
+            k_failed = true;
+            break;
         }
 
-        float o[DT][NT][4];
-        float m[NT][2], l[NT][2];
+        // ---- S^T = K Q^T
+        float s[MT][NT][4];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int r = 16 * t + (lane & 15);
+            if constexpr (kFmt == KVB_KV_INT8) {
+                int hi[NT][4], lo[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) hi[nt][e] = lo[nt][e] = 0;
+#pragma unroll
+                for (int j = 0; j < DT; j += 2) {
+                    uint32_t w0, w1, w2, w3;
+                    ldsm_x4(kb + q8_smem_off<HD>(r, j + (lane >> 4)), w0, w1, w2, w3);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_s8(hi[nt], w0, w1, w2, w3, qf[j][nt][0], qf[j + 1][nt][0]);
+                        mma_s8(lo[nt], w0, w1, w2, w3, qf[j][nt][1], qf[j + 1][nt][1]);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[t][nt][e] = (float)(hi[nt][e] * 256 + lo[nt][e]);
+            } else {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    s[t][nt][0] = s[t][nt][1] = s[t][nt][2] = s[t][nt][3] = 0.f;
+#pragma unroll
+                for (int j = 0; j < DT; j += 2) {
+                    uint32_t w0, w1, w2, w3, af[4];
+                    ldsm_x4(kb + q8_smem_off<HD>(r, j + (lane >> 4)), w0, w1, w2, w3);
+                    codes_pairs(w0, af[0], af[2]);
+                    codes_pairs(w1, af[1], af[3]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        mma_16816<__half>(s[t][nt], af, qf[j][nt][0], qf[j][nt][1]);
+                    codes_pairs(w2, af[0], af[2]);
+                    codes_pairs(w3, af[1], af[3]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        mma_16816<__half>(s[t][nt], af, qf[j + 1][nt][0], qf[j + 1][nt][1]);
+                }
+            }
+        }
+        // ---- scale and mask; element e: key 16 t + g + 8 (e >> 1), head 8 nt + 2c + (e & 1)
+        float mx[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const float k0 = ks[16 * t + g], k1 = ks[16 * t + g + 8];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[t][nt][e] *= (e < 2 ? k0 : k1) * qs[nt][e & 1];
+        }
+        __syncwarp();
+        fence_async_smem();  // these reads precede the next copies into the K tile
+        if (more) {
+            place(kt_next);
+            request_k(st);
+        }
+        if (nk < KT) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (16 * t + g + 8 * (e >> 1) >= nk) s[t][nt][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                mx[nt][0] = fmaxf(mx[nt][0], fmaxf(s[t][nt][0], s[t][nt][2]));
+                mx[nt][1] = fmaxf(mx[nt][1], fmaxf(s[t][nt][1], s[t][nt][3]));
+            }
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+                mx[nt][0] = fmaxf(mx[nt][0], __shfl_xor_sync(0xffffffffu, mx[nt][0], x));
+                mx[nt][1] = fmaxf(mx[nt][1], __shfl_xor_sync(0xffffffffu, mx[nt][1], x));
+            }
+        }
+        float al[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float mn = fmaxf(m[nt][e], mx[nt][e]);
+                const float ref = mn == -INFINITY ? 0.f : mn;
+                al[nt][e] = ex2_approx(m[nt][e] - ref);
+                m[nt][e] = mn;
+                float sum = 0.f;
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    s[t][nt][e] = ex2_approx(s[t][nt][e] - ref);
+                    s[t][nt][e + 2] = ex2_approx(s[t][nt][e + 2] - ref);
+                    sum += s[t][nt][e] + s[t][nt][e + 2];
+                }
+                // this lane's keys; summed over lanes at the end
+                l[nt][e] = l[nt][e] * al[nt][e] + sum;
+            }
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][st][1], phase));
+        if (!ok) break;
+        if (kFmt == KVB_KV_E4M3 && nk < KT) {  // codes past the last key may be NaN: 0 * NaN
+            for (int i = nk * HD / 16 + lane; i < KT * HD / 16; i += 32)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vb + 16 * i), "r"(0)
+                             : "memory");
+            __syncwarp();
+        }
+        // ---- V scale exponent: O is rescaled where a larger one appears
+        uint32_t vmax = __float_as_uint(vs[lane]) & 0x7fffffffu;
+        if (KT == 64) vmax = max(vmax, __float_as_uint(vs[lane + 32]) & 0x7fffffffu);
+        const int en = max(ev, (int)(__reduce_max_sync(0xffffffffu, vmax) >> 23));
+        const float vf = __uint_as_float((uint32_t)(267 - en) << 23);  // 2^(140 - en)
+        const int down = 127 + ev - en;  // exponent field of 2^(ev - en)
+        const float rv = down > 0 ? __uint_as_float((uint32_t)down << 23) : 0.f;
+        ev = en;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float ao = al[nt][e] * rv;
+#pragma unroll
+                for (int j = 0; j < DT; ++j) {
+                    o[j][nt][e] *= ao;
+                    o[j][nt][e + 2] *= ao;
+                }
+            }
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const float v0 = vs[16 * t + g] * vf, v1 = vs[16 * t + g + 8] * vf;
+            uint32_t pf[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                pf[nt][0] = movmatrix_t(f16x2(s[t][nt][0] * v0, s[t][nt][1] * v0));
+                pf[nt][1] = movmatrix_t(f16x2(s[t][nt][2] * v1, s[t][nt][3] * v1));
+            }
+            const int r = 16 * t + (lane & 15);
+#pragma unroll
+            for (int j = 0; j < DT; j += 2) {
+                uint32_t w0, w1, w2, w3, af[4];
+                ldsm_x4_t(vb + q8_smem_off<HD>(r, j + (lane >> 4)), w0, w1, w2, w3);
+                codes_evens_odds<kFmt>(w0, af[0], af[1]);
+                codes_evens_odds<kFmt>(w1, af[2], af[3]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_16816<__half>(o[j][nt], af, pf[nt][0], pf[nt][1]);
+                codes_evens_odds<kFmt>(w2, af[0], af[1]);
+                codes_evens_odds<kFmt>(w3, af[2], af[3]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    mma_16816<__half>(o[j + 1][nt], af, pf[nt][0], pf[nt][1]);
+            }
+        }
+        __syncwarp();
+        fence_async_smem();  // these reads precede the next copies into the V tile
+        if (more) request_v(st);
+    }
+    if (!ok) {
+        // A copy did not complete in time (the error word is set): wait once more, bounded,
+        // for each copy still outstanding, and contribute an empty state.
+        for (int i = it; i <= it + kQ8Stages; ++i) {
+            if (key_begin + (warp + i * kQ8Warps) * KT >= key_end) break;
+            const uint32_t ph = (i / kQ8Stages) & 1;
+            const bool k_asked = i < it + kQ8Stages || !k_failed;
+            if (k_asked && (i > it || k_failed)) mbar_wait(&bars[warp][i % kQ8Stages][0], ph);
+            if (i < it + kQ8Stages) mbar_wait(&bars[warp][i % kQ8Stages][1], ph);
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             m[nt][0] = m[nt][1] = -INFINITY;
@@ -447,294 +638,68 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
 #pragma unroll
             for (int j = 0; j < DT; ++j) o[j][nt][0] = o[j][nt][1] = o[j][nt][2] = o[j][nt][3] = 0.f;
         }
-        int ev = 14;  // biased exponent of the largest V scale seen; O is in units of 2^(ev - 140)
-        // Two tiles per warp in flight, K and V on barriers of their own: the K of the tile
-        // after next is requested once the scores are out of this one, its V once P V has read
-        // this V.
-        bool ok = true;
-        int it = 0;
-        bool k_failed = false;
-        for (int kt0 = key_begin + warp * KT; kt0 < key_end; kt0 += kQ8Warps * KT, ++it) {
-            const int st = it % kQ8Stages;
-            const uint32_t phase = (it / kQ8Stages) & 1;
-            const int nk = min(KT, key_end - kt0);
-            const int kt_next = kt0 + kQ8Stages * kQ8Warps * KT;
-            const bool more = kt_next < key_end;
-            const uint32_t kb = smem_u32(ring + st * 2 * kQ8TileBytes), vb = kb + kQ8TileBytes;
-            const float* ks = ring_scales + st * 128;
-            const float* vs = ks + 64;
-            ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][st][0], phase));
-            if (!ok) {
-                k_failed = true;
-                break;
-            }
-
-            // ---- S^T = K Q^T
-            float s[MT][NT][4];
+        __syncwarp();
+    }
+    // ---- merge the four warps' states through shared memory
+    const float unit = __uint_as_float((uint32_t)(ev - 13) << 23);  // 2^(ev - 140)
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const int r = 16 * t + (lane & 15);
-                if constexpr (kFmt == KVB_KV_INT8) {
-                    int hi[NT][4], lo[NT][4];
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+        for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) hi[nt][e] = lo[nt][e] = 0;
-#pragma unroll
-                    for (int j = 0; j < DT; j += 2) {
-                        uint32_t w0, w1, w2, w3;
-                        ldsm_x4(kb + q8_smem_off<HD>(r, j + (lane >> 4)), w0, w1, w2, w3);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            mma_s8(hi[nt], w0, w1, w2, w3, qf[j][nt][0], qf[j + 1][nt][0]);
-                            mma_s8(lo[nt], w0, w1, w2, w3, qf[j][nt][1], qf[j + 1][nt][1]);
-                        }
-                    }
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[t][nt][e] = (float)(hi[nt][e] * 256 + lo[nt][e]);
-                } else {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        s[t][nt][0] = s[t][nt][1] = s[t][nt][2] = s[t][nt][3] = 0.f;
-#pragma unroll
-                    for (int j = 0; j < DT; j += 2) {
-                        uint32_t w0, w1, w2, w3, af[4];
-                        ldsm_x4(kb + q8_smem_off<HD>(r, j + (lane >> 4)), w0, w1, w2, w3);
-                        codes_pairs(w0, af[0], af[2]);
-                        codes_pairs(w1, af[1], af[3]);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-                            mma_16816<__half>(s[t][nt], af, qf[j][nt][0], qf[j][nt][1]);
-                        codes_pairs(w2, af[0], af[2]);
-                        codes_pairs(w3, af[1], af[3]);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-                            mma_16816<__half>(s[t][nt], af, qf[j + 1][nt][0], qf[j + 1][nt][1]);
-                    }
-                }
-            }
-            // ---- scale and mask; element e: key 16 t + g + 8 (e >> 1), head 8 nt + 2c + (e & 1)
-            float mx[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const float k0 = ks[16 * t + g], k1 = ks[16 * t + g + 8];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[t][nt][e] *= (e < 2 ? k0 : k1) * qs[nt][e & 1];
-            }
-            __syncwarp();
-            fence_async_smem();  // these reads precede the next copies into the K tile
-            if (more) {
-                place(kt_next);
-                request_k(st);
-            }
-            if (nk < KT) {
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (16 * t + g + 8 * (e >> 1) >= nk) s[t][nt][e] = -INFINITY;
+            for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
+            const int h = 8 * nt + 2 * c + e;
+            if (g == 0) {
+                w_ml[warp][0][h] = m[nt][e];
+                w_ml[warp][1][h] = l[nt][e];
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    mx[nt][0] = fmaxf(mx[nt][0], fmaxf(s[t][nt][0], s[t][nt][2]));
-                    mx[nt][1] = fmaxf(mx[nt][1], fmaxf(s[t][nt][1], s[t][nt][3]));
-                }
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) {
-                    mx[nt][0] = fmaxf(mx[nt][0], __shfl_xor_sync(0xffffffffu, mx[nt][0], x));
-                    mx[nt][1] = fmaxf(mx[nt][1], __shfl_xor_sync(0xffffffffu, mx[nt][1], x));
-                }
-            }
-            float al[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float mn = fmaxf(m[nt][e], mx[nt][e]);
-                    const float ref = mn == -INFINITY ? 0.f : mn;
-                    al[nt][e] = ex2_approx(m[nt][e] - ref);
-                    m[nt][e] = mn;
-                    float sum = 0.f;
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        s[t][nt][e] = ex2_approx(s[t][nt][e] - ref);
-                        s[t][nt][e + 2] = ex2_approx(s[t][nt][e + 2] - ref);
-                        sum += s[t][nt][e] + s[t][nt][e + 2];
-                    }
-                    // this lane's keys; summed over lanes at the end
-                    l[nt][e] = l[nt][e] * al[nt][e] + sum;
-                }
-            ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][st][1], phase));
-            if (!ok) break;
-            if (kFmt == KVB_KV_E4M3 && nk < KT) {  // codes past the last key may be NaN: 0 * NaN
-                for (int i = nk * HD / 16 + lane; i < KT * HD / 16; i += 32)
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vb + 16 * i), "r"(0)
-                                 : "memory");
-                __syncwarp();
-            }
-            // ---- V scale exponent: O is rescaled where a larger one appears
-            uint32_t vmax = __float_as_uint(vs[lane]) & 0x7fffffffu;
-            if (KT == 64) vmax = max(vmax, __float_as_uint(vs[lane + 32]) & 0x7fffffffu);
-            const int en = max(ev, (int)(__reduce_max_sync(0xffffffffu, vmax) >> 23));
-            const float vf = __uint_as_float((uint32_t)(267 - en) << 23);  // 2^(140 - en)
-            const int down = 127 + ev - en;  // exponent field of 2^(ev - en)
-            const float rv = down > 0 ? __uint_as_float((uint32_t)down << 23) : 0.f;
-            ev = en;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float ao = al[nt][e] * rv;
-#pragma unroll
-                    for (int j = 0; j < DT; ++j) {
-                        o[j][nt][e] *= ao;
-                        o[j][nt][e + 2] *= ao;
-                    }
-                }
-            // ---- O^T += V^T P^T
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const float v0 = vs[16 * t + g] * vf, v1 = vs[16 * t + g + 8] * vf;
-                uint32_t pf[NT][2];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    pf[nt][0] = movmatrix_t(f16x2(s[t][nt][0] * v0, s[t][nt][1] * v0));
-                    pf[nt][1] = movmatrix_t(f16x2(s[t][nt][2] * v1, s[t][nt][3] * v1));
-                }
-                const int r = 16 * t + (lane & 15);
-#pragma unroll
-                for (int j = 0; j < DT; j += 2) {
-                    uint32_t w0, w1, w2, w3, af[4];
-                    ldsm_x4_t(vb + q8_smem_off<HD>(r, j + (lane >> 4)), w0, w1, w2, w3);
-                    codes_evens_odds<kFmt>(w0, af[0], af[1]);
-                    codes_evens_odds<kFmt>(w1, af[2], af[3]);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma_16816<__half>(o[j][nt], af, pf[nt][0], pf[nt][1]);
-                    codes_evens_odds<kFmt>(w2, af[0], af[1]);
-                    codes_evens_odds<kFmt>(w3, af[2], af[3]);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        mma_16816<__half>(o[j + 1][nt], af, pf[nt][0], pf[nt][1]);
-                }
-            }
-            __syncwarp();
-            fence_async_smem();  // these reads precede the next copies into the V tile
-            if (more) request_v(st);
+            for (int j = 0; j < DT; ++j)
+                *reinterpret_cast<float2*>(wo + h * HD + 16 * j + 2 * g) =
+                    make_float2(o[j][nt][e] * unit, o[j][nt][e + 2] * unit);
         }
-        if (!ok) {
-            // A copy did not complete in time (the error word is set): wait once more, bounded,
-            // for each copy still outstanding, and contribute an empty state.
-            for (int i = it; i <= it + kQ8Stages; ++i) {
-                if (key_begin + (warp + i * kQ8Warps) * KT >= key_end) break;
-                const uint32_t ph = (i / kQ8Stages) & 1;
-                const bool k_asked = i < it + kQ8Stages || !k_failed;
-                if (k_asked && (i > it || k_failed)) mbar_wait(&bars[warp][i % kQ8Stages][0], ph);
-                if (i < it + kQ8Stages) mbar_wait(&bars[warp][i % kQ8Stages][1], ph);
-            }
+    }
+    __syncthreads();
+    float* wsb = nullptr;
+    if (n_chunks > 1)
+        wsb = a.ws + (((size_t)b * a.c.n_kv + kvh) * a.max_chunks + chunk) *
+                         (size_t)q8_part_floats(G, HD);
+    // Four neighbouring dims of one head per thread and turn; 128 threads span 512 / HD
+    // heads a turn.
+    for (int i = 4 * threadIdx.x; i < G * HD; i += 4 * kQ8Warps * 32) {
+        const int r = i / HD;
+        float M = -INFINITY;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                m[nt][0] = m[nt][1] = -INFINITY;
-                l[nt][0] = l[nt][1] = 0.f;
+        for (int w = 0; w < kQ8Warps; ++w) M = fmaxf(M, w_ml[w][0][r]);
+        float L = 0.f;
+        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int j = 0; j < DT; ++j) o[j][nt][0] = o[j][nt][1] = o[j][nt][2] = o[j][nt][3] = 0.f;
-            }
-            __syncwarp();
+        for (int w = 0; w < kQ8Warps; ++w) {
+            const float mw = w_ml[w][0][r];
+            const float f = mw == -INFINITY ? 0.f : ex2_approx(mw - M);
+            // a warp whose scores were all NaN keeps -inf as its maximum and a NaN sum
+            const float lw = w_ml[w][1][r];
+            L += lw != lw ? lw : lw * f;
+            const float4 ow = *reinterpret_cast<const float4*>(smem + w * kQ8WarpBytes + 4 * i);
+            O.x += ow.x * f;
+            O.y += ow.y * f;
+            O.z += ow.z * f;
+            O.w += ow.w * f;
         }
-        // ---- merge the four warps' states through shared memory
-        const float unit = __uint_as_float((uint32_t)(ev - 13) << 23);  // 2^(ev - 140)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
-                const int h = 8 * nt + 2 * c + e;
-                if (g == 0) {
-                    w_ml[warp][0][h] = m[nt][e];
-                    w_ml[warp][1][h] = l[nt][e];
-                }
-#pragma unroll
-                for (int j = 0; j < DT; ++j)
-                    *reinterpret_cast<float2*>(wo + h * HD + 16 * j + 2 * g) =
-                        make_float2(o[j][nt][e] * unit, o[j][nt][e + 2] * unit);
-            }
-        }
-        __syncthreads();
-        float* wsb = nullptr;
-        float* mlb = nullptr;
-        if (n_chunks > 1) {
-            wsb = a.fold ? fold_o
-                         : a.ws + (((size_t)b * a.c.n_kv + kvh) * a.max_chunks + chunk) *
-                                      (size_t)q8_part_floats(G, HD);
-            mlb = a.fold ? &fold_ml[0][0] : wsb + G * HD;
-        }
-        const int ml_step = a.fold ? kQ8MaxGroup : G;
-        // Four neighbouring dims of one head per thread and turn; 128 threads span 512 / HD
-        // heads a turn.
-        for (int i = 4 * threadIdx.x; i < G * HD; i += 4 * kQ8Warps * 32) {
-            const int r = i / HD;
-            float M = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kQ8Warps; ++w) M = fmaxf(M, w_ml[w][0][r]);
-            float L = 0.f;
-            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < kQ8Warps; ++w) {
-                const float mw = w_ml[w][0][r];
-                const float f = mw == -INFINITY ? 0.f : ex2_approx(mw - M);
-                // a warp whose scores were all NaN keeps -inf as its maximum and a NaN sum
-                const float lw = w_ml[w][1][r];
-                L += lw != lw ? lw : lw * f;
-                const float4 ow = *reinterpret_cast<const float4*>(smem + w * kQ8WarpBytes + 4 * i);
-                O.x += ow.x * f;
-                O.y += ow.y * f;
-                O.z += ow.z * f;
-                O.w += ow.w * f;
-            }
-            if (n_chunks == 1) {
-                const float inv = 1.f / L;
-                outb[i] = Elem<T>::from_f(O.x * inv);
-                outb[i + 1] = Elem<T>::from_f(O.y * inv);
-                outb[i + 2] = Elem<T>::from_f(O.z * inv);
-                outb[i + 3] = Elem<T>::from_f(O.w * inv);
-            } else {
-                *reinterpret_cast<float4*>(wsb + i) = O;
-                if (i % HD == 0) {
-                    mlb[r] = M;
-                    mlb[ml_step + r] = L;
-                }
+        if (n_chunks == 1) {
+            const float inv = 1.f / L;
+            outb[i] = Elem<T>::from_f(O.x * inv);
+            outb[i + 1] = Elem<T>::from_f(O.y * inv);
+            outb[i + 2] = Elem<T>::from_f(O.z * inv);
+            outb[i + 3] = Elem<T>::from_f(O.w * inv);
+        } else {
+            *reinterpret_cast<float4*>(wsb + i) = O;
+            if (i % HD == 0) {
+                wsb[G * HD + r] = M;
+                wsb[G * HD + G + r] = L;
             }
         }
     }
-    if (!a.fold) return;
-    cluster_sync();  // every chunk's state is in its CTA's shared memory
-    if (n_chunks > 1 && slot == a.max_chunks - 1) {
-        const uint32_t r0 = (uint32_t)(a.max_chunks - n_chunks);
-        for (int i = threadIdx.x; i < G * HD; i += blockDim.x) {
-            const int r = i / HD;
-            float M = -INFINITY;
-            for (int k = 0; k < n_chunks; ++k) M = fmaxf(M, dsmem_ld(&fold_ml[0][r], r0 + k));
-            float L = 0.f, O = 0.f;
-            for (int k = 0; k < n_chunks; ++k) {
-                const float mk = dsmem_ld(&fold_ml[0][r], r0 + k), lk = dsmem_ld(&fold_ml[1][r], r0 + k);
-                const float f = mk == -INFINITY ? 0.f : exp2f(mk - M);
-                L += lk != lk ? lk : lk * f;
-                O += dsmem_ld(fold_o + i, r0 + k) * f;
-            }
-            outb[i] = Elem<T>::from_f(O / L);
-        }
-    }
-    cluster_sync();  // no CTA leaves while its state may still be read
 }
 
 // Joins the partial states of every (sequence, head): parts 0 .. fixed - 1, which every
