@@ -225,24 +225,27 @@ static bool q8_tensor_shape(size_t head_dim, size_t n_q, size_t n_kv) {
            n_q / n_kv <= (size_t)kQ8MaxGroup;
 }
 
-// Keys per CTA of a split call.  Long batches: about five waves of three CTAs per SM over the
-// worst case (every sequence at max_len), as decode_chunk_keys.  Below that, as few tiles as
-// fill one wave, between 4 (one per warp) and 16: shorter chunks pay more starts and a longer
-// join, longer ones leave a longer last wave.  Pairs of (sequence, KV head) that fill the SMs
-// by themselves with at most 24 tiles take one chunk each and no join.  Measured on B200,
-// tiles per CTA: 37 sequences x 2 heads U[0,5003] (head_dim 128) 8 / 16 / 32 / 48: 27.6 /
-// 25.0 / 25.6 / 31.7 us; 32 x 8 at 1000 keys 8 / 12 / 17: 19.5 / 15.7 / 15.2; 64 x 8
-// U[1,4096] 8 / 16 / 24 / 48: 40.3 / 36.7 / 36.3 / 38.7; one sequence x 8 at 513 keys 4 / 9:
-// 5.5 / 5.7.  At most kJoinMaxParts chunks.
+// Keys per CTA of a split call.  The fewest tiles, up to 20, with which one wave of three CTAs
+// per SM holds the worst case (every sequence at max_len); beyond that about five waves, of
+// at least 20 tiles: shorter chunks pay more starts and a longer join, longer ones leave a
+// longer last wave.  Pairs of (sequence, KV head) that fill the SMs by themselves with at most
+// 32 tiles take one chunk each and no join.  Against the best of 4 to 128 tiles over 140 shapes
+// (full and ragged batches, n_kv 1 to 8, both head_dims) 3.9 % slower on average, 24 % at worst.
+// Measured on B200, tiles per CTA: one sequence x 8 heads at 65536 keys 12 / 16 / 20 / 32:
+// 23.5 / 25.0 / 19.5 / 22.2 us (16 is a wave and a bit); 16 x 8 at 4096 8 / 16 / 20 / 32: 22.3 /
+// 23.3 / 18.1 / 20.9; 64 x 8 U[1,4096] 8 / 16 / 20 / 48: 37.4 / 33.8 / 35.1 / 34.9; 32 x 8 at 1000
+// keys 8 / 12 / 16: 16.4 / 13.7 / 12.3.  At most kJoinMaxParts chunks.
 static int q8_chunk_keys(size_t n_seq, size_t n_kv, size_t max_len, size_t head_dim) {
     const size_t kt = (size_t)q8_tile_keys((int)head_dim);
     const size_t tiles = (max_len + kt - 1) / kt, pairs = n_seq * n_kv;
     const size_t slots = (size_t)num_sms() * kQ8CtasPerSm;
-    size_t least = pairs * tiles / slots;
-    least = least < 4 ? 4 : least > 16 ? 16 : least;
-    size_t per_cta = (pairs * tiles + 5 * slots - 1) / (5 * slots);
-    if (per_cta < least) per_cta = least;
-    if (pairs >= (size_t)num_sms() && tiles <= 24) per_cta = tiles;
+    const size_t chunks = pairs < slots && pairs > 0 ? slots / pairs : 1;  // of a pair, in one wave
+    size_t per_cta = (tiles + chunks - 1) / chunks;
+    if (per_cta > 20) {
+        per_cta = (pairs * tiles + 5 * slots - 1) / (5 * slots);
+        if (per_cta < 20) per_cta = 20;
+    }
+    if (pairs >= (size_t)num_sms() && tiles <= 32) per_cta = tiles;
     if (per_cta * kJoinMaxParts < tiles) per_cta = (tiles + kJoinMaxParts - 1) / kJoinMaxParts;
     if (per_cta > tiles) per_cta = tiles;
     if (per_cta < 1) per_cta = 1;
