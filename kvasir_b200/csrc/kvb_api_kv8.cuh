@@ -229,7 +229,9 @@ static bool q8_tensor_shape(size_t head_dim, size_t n_q, size_t n_kv) {
 // per SM holds the worst case (every sequence at max_len); beyond that about five waves, of
 // at least 20 tiles: shorter chunks pay more starts and a longer join, longer ones leave a
 // longer last wave.  Pairs of (sequence, KV head) that fill the SMs by themselves with at most
-// 32 tiles take one chunk each and no join.  Against the best of 4 to 128 tiles over 140 shapes
+// 32 tiles take one chunk each and no join; so do 12 tiles (768 keys of 64 dims) in any case:
+// one sequence of 513 keys 5.7 us in a graph against 5.3 in three chunks, but 9.6 against 12.2
+// where the host launches it, as the second launch is 2 us of the host's time.  Against the best of 4 to 128 tiles over 140 shapes
 // (full and ragged batches, n_kv 1 to 8, both head_dims) 3.9 % slower on average, 24 % at worst.
 // Measured on B200, tiles per CTA: one sequence x 8 heads at 65536 keys 12 / 16 / 20 / 32:
 // 23.5 / 25.0 / 19.5 / 22.2 us (16 is a wave and a bit); 16 x 8 at 4096 8 / 16 / 20 / 32: 22.3 /
@@ -245,7 +247,7 @@ static int q8_chunk_keys(size_t n_seq, size_t n_kv, size_t max_len, size_t head_
         per_cta = (pairs * tiles + 5 * slots - 1) / (5 * slots);
         if (per_cta < 20) per_cta = 20;
     }
-    if (pairs >= (size_t)num_sms() && tiles <= 32) per_cta = tiles;
+    if (tiles <= 12 || (pairs >= (size_t)num_sms() && tiles <= 32)) per_cta = tiles;
     if (per_cta * kJoinMaxParts < tiles) per_cta = (tiles + kJoinMaxParts - 1) / kJoinMaxParts;
     if (per_cta > tiles) per_cta = tiles;
     if (per_cta < 1) per_cta = 1;
