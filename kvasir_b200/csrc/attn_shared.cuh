@@ -25,8 +25,10 @@
 // the youngest alone (measured 41 to 71 us for equal slices).  A thread reads its scores from
 // TMEM 32 at a time (maximum, then exponentials).  There is no causal mask; a row's keys end
 // at the prefix's end, or earlier for a paged sequence shorter than the prefix.
+// Measured no better: a part of the exponentials as polynomials on the FMA pipe, halves of 32 keys
+// with an S buffer each (110 us; N = 32 products cost the tensor pipe as much as N = 64).
 // Measured on B200 with the own keys and the join: 256 sequences of 32 + 8 heads on 16384 keys
-// with up to 1000 own, 105 us (f16) and 111 us (bf16, P in two halves).
+// with up to 1000 own, 97 us (f16) and 106 us (bf16, P in two halves).
 #pragma once
 
 #include "attn_decode_q8.cuh"
