@@ -70,6 +70,11 @@ struct Q8DecodeArgs {
     const float* rope_cos;
     const float* rope_sin;
     int rope_max_pos;
+    // kRope: the cache rows before each new key, their scales, the lengths and the block table are
+    // final (no kernel that may still be running writes them: the decode-step driver's launches).
+    // The first tiles are then requested before griddepcontrol.wait; otherwise nothing is read
+    // before it.
+    int kv_ready;
 };
 
 // One warp's share of the append: a K (rotated) or V row of HD 16-bit elements, quantised to
@@ -223,13 +228,15 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
         mbar_init(&bars[0][0][0] + threadIdx.x, 1 + 32);  // one expect_tx, 32 scale arrivals
     fence_mbar_init();
     __syncthreads();
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const bool early = kRope && a.kv_ready;
+    if (!early) asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const int len = q8_len(a.lens, a.max_len, b);
     const int n_chunks = (len + a.chunk_keys - 1) / a.chunk_keys;
     const int from_end = a.max_chunks - 1 - (int)blockIdx.z;
     T* outb = reinterpret_cast<T*>(a.out) + (size_t)b * a.out_row_stride + (size_t)kvh * G * HD;
     if (len == 0) {  // no keys: a zero row
+        if (early) asm volatile("griddepcontrol.wait;" ::: "memory");
         if (from_end == 0)
             for (int i = threadIdx.x; i < G * HD; i += blockDim.x) outb[i] = Elem<T>::from_f(0.f);
         return;
@@ -329,6 +336,7 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
         }
     };
     first_tiles(false);
+    if (early) asm volatile("griddepcontrol.wait;" ::: "memory");  // q, the new row
     if (appends) {
         size_t crow = 0, head_rows = 0;
         if (warp < 2 && kv8_row(a.c, b, rope_p, crow, head_rows, threadIdx.x == 0)) {

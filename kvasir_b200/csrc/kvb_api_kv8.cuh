@@ -352,6 +352,7 @@ struct Q8Rope {
     const float* cos_t = nullptr;
     const float* sin_t = nullptr;
     int max_pos = 0;
+    bool kv_ready = false;  // Q8DecodeArgs::kv_ready
 };
 template <typename T, int kFmt>
 static int launch_q8_decode(kvb_stream_t stream, const GeneralDecodeArgs& a, const Kv8Place& c,
@@ -388,6 +389,7 @@ static int launch_q8_decode(kvb_stream_t stream, const GeneralDecodeArgs& a, con
     d.rope_cos = rope.cos_t;
     d.rope_sin = rope.sin_t;
     d.rope_max_pos = rope.max_pos;
+    d.kv_ready = rope.kv_ready ? 1 : 0;
     if (a.hd == 64)
         return d.group <= 8 ? launch_q8_tensor<T, kFmt, 64, 1>(stream, d, n_seq, cache_rows, ws, ws_len)
                             : launch_q8_tensor<T, kFmt, 64, 2>(stream, d, n_seq, cache_rows, ws, ws_len);
@@ -778,40 +780,73 @@ int kvb_attention_decode_q8_paged(kvb_stream_t stream, const void* q, size_t q_r
                            workspace, workspace_len, kv_format, dtype, Q8Rope());
 }
 
-int kvb_rope_attention_decode_q8(kvb_stream_t stream, const void* qkv, size_t qkv_len,
-                                 const float* cos_t, const float* sin_t, size_t table_len, void* kc,
-                                 void* vc, float* ks, float* vs, size_t seq_stride, size_t cache_len,
-                                 size_t scale_len, const int32_t* lens, size_t n_seq, size_t max_len,
-                                 size_t n_q, size_t n_kv, size_t head_dim, size_t max_seq, float scale,
-                                 void* out, size_t out_row_stride, void* workspace,
-                                 size_t workspace_len, int kv_format, int dtype) {
+static int rope_attention_q8(kvb_stream_t stream, const void* qkv, size_t qkv_len,
+                             const float* cos_t, const float* sin_t, size_t table_len, void* kc,
+                             void* vc, float* ks, float* vs, size_t seq_stride, size_t cache_len,
+                             size_t scale_len, const int32_t* lens, size_t n_seq, size_t max_len,
+                             size_t n_q, size_t n_kv, size_t head_dim, size_t max_seq, float scale,
+                             void* out, size_t out_row_stride, void* workspace,
+                             size_t workspace_len, int kv_format, int dtype, bool kv_ready) {
     Q8Rope r;
     const int st = q8_rope("rope_attention_decode_q8", r, qkv, qkv_len, cos_t, sin_t, table_len, n_seq,
                            n_q, n_kv, head_dim);
     if (st) return st;
+    r.kv_ready = kv_ready;
     return q8_decode_contiguous("rope_attention_decode_q8", stream, qkv, (n_q + 2 * n_kv) * head_dim,
                                 kc, vc, ks, vs, seq_stride, cache_len, scale_len, lens, n_seq, max_len,
                                 n_q, n_kv, head_dim, max_seq, scale, out, out_row_stride, workspace,
                                 workspace_len, kv_format, dtype, r);
 }
 
-int kvb_rope_attention_decode_q8_paged(kvb_stream_t stream, const void* qkv, size_t qkv_len,
-                                       const float* cos_t, const float* sin_t, size_t table_len,
-                                       void* k_pool, void* v_pool, float* k_scales, float* v_scales,
-                                       size_t pool_len, size_t scale_len, const int32_t* block_table,
-                                       size_t max_blocks, size_t block_size, const int32_t* lens,
-                                       size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
-                                       size_t head_dim, float scale, void* out, size_t out_row_stride,
-                                       void* workspace, size_t workspace_len, int kv_format,
-                                       int dtype) {
+static int rope_attention_q8_paged(kvb_stream_t stream, const void* qkv, size_t qkv_len,
+                                   const float* cos_t, const float* sin_t, size_t table_len,
+                                   void* k_pool, void* v_pool, float* k_scales, float* v_scales,
+                                   size_t pool_len, size_t scale_len, const int32_t* block_table,
+                                   size_t max_blocks, size_t block_size, const int32_t* lens,
+                                   size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
+                                   size_t head_dim, float scale, void* out, size_t out_row_stride,
+                                   void* workspace, size_t workspace_len, int kv_format, int dtype,
+                                   bool kv_ready) {
     Q8Rope r;
     const int st = q8_rope("rope_attention_decode_q8_paged", r, qkv, qkv_len, cos_t, sin_t, table_len,
                            n_seq, n_q, n_kv, head_dim);
     if (st) return st;
+    r.kv_ready = kv_ready;
     return q8_decode_paged("rope_attention_decode_q8_paged", stream, qkv, (n_q + 2 * n_kv) * head_dim,
                            k_pool, v_pool, k_scales, v_scales, pool_len, scale_len, block_table,
                            max_blocks, block_size, lens, n_seq, max_len, n_q, n_kv, head_dim, scale,
                            out, out_row_stride, workspace, workspace_len, kv_format, dtype, r);
+}
+
+int kvb_rope_attention_decode_q8(kvb_stream_t stream, const void* qkv, size_t qkv_len,
+                                 const float* cos_t, const float* sin_t, size_t table_len, void* kc,
+                                 void* vc, float* ks, float* vs, size_t seq_stride,
+                                 size_t cache_len, size_t scale_len, const int32_t* lens,
+                                 size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
+                                 size_t head_dim, size_t max_seq, float scale, void* out,
+                                 size_t out_row_stride, void* workspace, size_t workspace_len,
+                                 int kv_format, int dtype) {
+    return rope_attention_q8(stream, qkv, qkv_len, cos_t, sin_t, table_len, kc, vc, ks, vs,
+                             seq_stride, cache_len, scale_len, lens, n_seq, max_len, n_q, n_kv,
+                             head_dim, max_seq, scale, out, out_row_stride, workspace,
+                             workspace_len, kv_format, dtype, false);
+}
+
+int kvb_rope_attention_decode_q8_paged(kvb_stream_t stream, const void* qkv, size_t qkv_len,
+                                       const float* cos_t, const float* sin_t, size_t table_len,
+                                       void* k_pool, void* v_pool, float* k_scales, float* v_scales,
+                                       size_t pool_len, size_t scale_len,
+                                       const int32_t* block_table, size_t max_blocks,
+                                       size_t block_size, const int32_t* lens, size_t n_seq,
+                                       size_t max_len, size_t n_q, size_t n_kv, size_t head_dim,
+                                       float scale, void* out, size_t out_row_stride,
+                                       void* workspace, size_t workspace_len, int kv_format,
+                                       int dtype) {
+    return rope_attention_q8_paged(stream, qkv, qkv_len, cos_t, sin_t, table_len, k_pool, v_pool,
+                                   k_scales, v_scales, pool_len, scale_len, block_table, max_blocks,
+                                   block_size, lens, n_seq, max_len, n_q, n_kv, head_dim, scale,
+                                   out, out_row_stride, workspace, workspace_len, kv_format, dtype,
+                                   false);
 }
 
 size_t kvb_attention_decode_shared_workspace_bytes(size_t n_seq, size_t shared_len, size_t max_own,
@@ -919,3 +954,39 @@ int kvb_attention_decode_shared_paged(kvb_stream_t stream, const void* q, size_t
 }
 
 }  // extern "C"
+
+// ------------------------------------------------------------------ decode-step forms
+namespace kvb {
+
+int rope_attention_decode_q8_in_step(kvb_stream_t stream, const void* qkv, size_t qkv_len,
+                                     const float* cos_t, const float* sin_t, size_t table_len,
+                                     void* kc, void* vc, float* ks, float* vs, size_t seq_stride,
+                                     size_t cache_len, size_t scale_len, const int32_t* lens,
+                                     size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
+                                     size_t head_dim, size_t max_seq, float scale, void* out,
+                                     size_t out_row_stride, void* workspace, size_t workspace_len,
+                                     int kv_format, int dtype) {
+    return ::rope_attention_q8(stream, qkv, qkv_len, cos_t, sin_t, table_len, kc, vc, ks, vs,
+                               seq_stride, cache_len, scale_len, lens, n_seq, max_len, n_q, n_kv,
+                               head_dim, max_seq, scale, out, out_row_stride, workspace,
+                               workspace_len, kv_format, dtype, true);
+}
+
+int rope_attention_decode_q8_paged_in_step(kvb_stream_t stream, const void* qkv, size_t qkv_len,
+                                           const float* cos_t, const float* sin_t, size_t table_len,
+                                           void* k_pool, void* v_pool, float* k_scales,
+                                           float* v_scales, size_t pool_len, size_t scale_len,
+                                           const int32_t* block_table, size_t max_blocks,
+                                           size_t block_size, const int32_t* lens, size_t n_seq,
+                                           size_t max_len, size_t n_q, size_t n_kv, size_t head_dim,
+                                           float scale, void* out, size_t out_row_stride,
+                                           void* workspace, size_t workspace_len, int kv_format,
+                                           int dtype) {
+    return ::rope_attention_q8_paged(stream, qkv, qkv_len, cos_t, sin_t, table_len, k_pool, v_pool,
+                                     k_scales, v_scales, pool_len, scale_len, block_table,
+                                     max_blocks, block_size, lens, n_seq, max_len, n_q, n_kv,
+                                     head_dim, scale, out, out_row_stride, workspace, workspace_len,
+                                     kv_format, dtype, true);
+}
+
+}  // namespace kvb

@@ -170,16 +170,15 @@ static int record_step(kvb_decoder_s* d, kvb_stream_t s) {
             int32_t* lens = d->at<int32_t>(L.lens);
             int32_t* pos = d->at<int32_t>(L.pos);
             st = d->block_table
-                     ? kvb_rope_attention_decode_q8_paged(
+                     ? kvb::rope_attention_decode_q8_paged_in_step(
                            s, d->at(L.qkv), B * qkvd, d->cos_t, d->sin_t, table_len, kl, vl, ksl, vsl,
                            codes, codes / hd, d->block_table, d->max_blocks, d->block_size, lens, B,
                            max_seq, nq, nkv, hd, scale, d->at(L.attn), qd, d->at(L.attn_ws),
                            L.attn_ws_len, fmt, dt)
-                     : kvb_rope_attention_decode_q8(s, d->at(L.qkv), B * qkvd, d->cos_t, d->sin_t,
-                                                    table_len, kl, vl, ksl, vsl, seq_stride, codes,
-                                                    codes / hd, lens, B, max_seq, nq, nkv, hd, max_seq,
-                                                    scale, d->at(L.attn), qd, d->at(L.attn_ws),
-                                                    L.attn_ws_len, fmt, dt);
+                     : kvb::rope_attention_decode_q8_in_step(
+                           s, d->at(L.qkv), B * qkvd, d->cos_t, d->sin_t, table_len, kl, vl, ksl, vsl,
+                           seq_stride, codes, codes / hd, lens, B, max_seq, nq, nkv, hd, max_seq,
+                           scale, d->at(L.attn), qd, d->at(L.attn_ws), L.attn_ws_len, fmt, dt);
             if (st == KVB_OK) {
                 ++own;
             } else if (st != KVB_ERR_UNSUPPORTED) {

@@ -64,6 +64,26 @@ int rope_attention_decode_paged_in_step(kvb_stream_t stream, const void* qkv, si
                                         float scale, void* out, size_t out_row_stride,
                                         void* workspace, size_t workspace_len, int dtype);
 
+// The same for kvb_rope_attention_decode_q8(_paged); the scales of those rows are final too.
+int rope_attention_decode_q8_in_step(kvb_stream_t stream, const void* qkv, size_t qkv_len,
+                                     const float* cos_t, const float* sin_t, size_t table_len,
+                                     void* kc, void* vc, float* ks, float* vs, size_t seq_stride,
+                                     size_t cache_len, size_t scale_len, const int32_t* lens,
+                                     size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
+                                     size_t head_dim, size_t max_seq, float scale, void* out,
+                                     size_t out_row_stride, void* workspace, size_t workspace_len,
+                                     int kv_format, int dtype);
+int rope_attention_decode_q8_paged_in_step(kvb_stream_t stream, const void* qkv, size_t qkv_len,
+                                           const float* cos_t, const float* sin_t, size_t table_len,
+                                           void* k_pool, void* v_pool, float* k_scales,
+                                           float* v_scales, size_t pool_len, size_t scale_len,
+                                           const int32_t* block_table, size_t max_blocks,
+                                           size_t block_size, const int32_t* lens, size_t n_seq,
+                                           size_t max_len, size_t n_q, size_t n_kv, size_t head_dim,
+                                           float scale, void* out, size_t out_row_stride,
+                                           void* workspace, size_t workspace_len, int kv_format,
+                                           int dtype);
+
 // Launches of a split-KV combine pass (0 or 1) that a split-KV decode call of this
 // shape and workspace makes after its decode kernel (head_dim 64, aligned buffers).
 int decode_combine_launches(size_t n_seq, size_t max_len, size_t n_q, size_t n_kv,
