@@ -486,7 +486,8 @@ int kvb_rope_attention_decode_q8_paged(kvb_stream_t stream, const void* qkv, siz
  * n_q / n_kv <= 16, scale > 0, block_size a multiple of 64, 16-byte aligned q and caches,
  * q_row_stride a multiple of 8, and a workspace of
  * kvb_attention_decode_shared_workspace_bytes (no initialisation; one call at a time, as
- * above); a general kernel, many times slower, takes the rest, NULL workspaces too. */
+ * above; a smaller one, down to one prefix part and one own part, takes fewer and longer
+ * parts); a general kernel, many times slower, takes the rest, NULL workspaces too. */
 int kvb_attention_decode_shared(kvb_stream_t stream, const void* q, size_t q_row_stride,
                                 const void* pk, const void* pv, size_t prefix_len,
                                 size_t prefix_rows, const void* kc, const void* vc,

@@ -406,7 +406,10 @@ struct SharedPlan {
     int chunk_keys, max_chunks, part_floats;
     size_t ws_bytes;
 };
-static SharedPlan shared_plan(size_t n_seq, size_t prefix, size_t max_own, size_t n_q, size_t n_kv) {
+// A workspace for a larger call may be a little small for this one: then fewer slices, and own
+// keys in longer chunks; ws_bytes is above ws_len only where not even one of each fits.
+static SharedPlan shared_plan(size_t n_seq, size_t prefix, size_t max_own, size_t n_q, size_t n_kv,
+                              size_t ws_len) {
     SharedPlan p;
     const size_t group = n_q / n_kv;
     p.key0 = (int)prefix;
@@ -443,12 +446,18 @@ static SharedPlan shared_plan(size_t n_seq, size_t prefix, size_t max_own, size_
         }
     }
     size_t ck = max_own ? (size_t)decode_chunk_keys(n_seq, n_kv, max_own) : 256;
-    const size_t most = kJoinMaxParts - 64;
-    if ((max_own + ck - 1) / ck > most) ck = ((max_own + most - 1) / most + 255) / 256 * 256;
+    p.part_floats = q8_part_floats((int)group, 64);
+    const size_t part_bytes = n_seq * n_kv * (size_t)p.part_floats * sizeof(float);
+    const size_t fit = part_bytes ? ws_len / part_bytes : 0;  // parts of a (sequence, KV head)
+    size_t chunks = (max_own + ck - 1) / ck;
+    if ((size_t)p.splits + chunks > fit && p.splits > 1)
+        p.splits = fit > chunks + 1 ? (int)(fit - chunks) : 1;
+    size_t most = kJoinMaxParts - 64;
+    if (fit > (size_t)p.splits && fit - p.splits < most) most = fit - p.splits;
+    if (chunks > most) ck = ((max_own + most - 1) / most + 255) / 256 * 256;
     p.chunk_keys = (int)ck;
     p.max_chunks = (int)((max_own + ck - 1) / ck);
-    p.part_floats = q8_part_floats((int)group, 64);
-    p.ws_bytes = n_seq * n_kv * (size_t)(p.splits + p.max_chunks) * p.part_floats * sizeof(float);
+    p.ws_bytes = part_bytes * (size_t)(p.splits + p.max_chunks);
     return p;
 }
 
@@ -582,7 +591,8 @@ template <typename T>
 static int launch_shared(kvb_stream_t stream, const GeneralDecodeArgs& a, const SharedSource<T>& src,
                          size_t n_seq, size_t own_rows, void* ws, size_t ws_len) {
     const bool paged = src.block_table != nullptr;
-    if (a.hd == 64 && a.n_q / a.n_kv <= kQ8MaxGroup && a.scale_log2 > 0.f && a.q_row_stride % 8 == 0 && aligned(a.q, 16) &&
+    if (a.hd == 64 && a.n_q / a.n_kv <= kQ8MaxGroup && a.scale_log2 > 0.f &&
+        a.q_row_stride % 8 == 0 && aligned(a.q, 16) &&
         aligned(src.kc, 16) && aligned(src.vc, 16) && aligned(src.pk, 16) && aligned(src.pv, 16) &&
         n_seq <= 65535 && a.n_kv <= 65535 && a.max_len <= 1 << 30 && src.prefix <= 1 << 30 &&
         ws != nullptr && aligned(ws, 16) &&
@@ -594,7 +604,8 @@ static int launch_shared(kvb_stream_t stream, const GeneralDecodeArgs& a, const 
         const size_t shared = paged ? (size_t)src.prefix / 64 * 64 : (size_t)src.prefix;
         const size_t own = paged ? (size_t)(a.max_len > (int)shared ? a.max_len - (int)shared : 0)
                                  : (size_t)a.max_len;
-        const SharedPlan p = shared_plan(n_seq, shared, own, (size_t)a.n_q, (size_t)a.n_kv);
+        const SharedPlan p =
+            shared_plan(n_seq, shared, own, (size_t)a.n_q, (size_t)a.n_kv, ws_len);
         if (ws_len >= p.ws_bytes)
             return launch_shared_tensor<T>(stream, a, src, p, n_seq, own_rows,
                                            static_cast<float*>(ws));
@@ -855,8 +866,9 @@ size_t kvb_attention_decode_shared_workspace_bytes(size_t n_seq, size_t shared_l
         n_q / n_kv > (size_t)kQ8MaxGroup || !fits_i32(shared_len) || !fits_i32(max_own))
         return 0;
     // contiguous, or paged with the prefix cut to whole 64-key tiles: the larger need
-    const size_t a = shared_plan(n_seq, shared_len, max_own, n_q, n_kv).ws_bytes;
-    const size_t b = shared_plan(n_seq, shared_len / 64 * 64, max_own + shared_len % 64, n_q, n_kv).ws_bytes;
+    const size_t a = shared_plan(n_seq, shared_len, max_own, n_q, n_kv, SIZE_MAX).ws_bytes;
+    const size_t b = shared_plan(n_seq, shared_len / 64 * 64, max_own + shared_len % 64, n_q, n_kv,
+                                 SIZE_MAX).ws_bytes;
     return a > b ? a : b;
 }
 

@@ -335,3 +335,20 @@ def test_rows_past_32_bit_offsets(g, hd):
 
     assert torch.equal(contiguous((2 ** 32 // hd + 3) * hd), contiguous(per))
     assert torch.equal(paged(2 ** 32 // per_block + 9), paged(8))
+
+
+@pytest.mark.parametrize("parts", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("paged", [False, True])
+def test_smaller_workspaces(g, parts, paged):
+    """A workspace of fewer parts than the call would take: fewer slices and longer chunks, the same
+    attention; nothing behind the workspace is written.  Too small for one part of each: the
+    general kernel."""
+    c = Case(np.random.default_rng(71), 5000, [1500, 0, 700, 3, 64], 8, 2, 64, "bf16")
+    part = (4 * (64 + 2) + 3) // 4 * 4 * 4  # bytes of O, m, l of a group of 4 heads
+    n = c.n_seq * c.n_kv * parts * part
+    assert n < g.attention_decode_shared_workspace_bytes(c.n_seq, c.prefix, 1500, 8, 2, 64)
+    whole = torch.full((n + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
+    c.ws = lambda *_: whole[:n]
+    c.check(c.paged(g, 64) if paged else c.contiguous(g))
+    assert bool((whole[n:] == 0xA5).all())
+    assert g.device_error() == 0
