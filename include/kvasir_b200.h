@@ -424,9 +424,10 @@ int kvb_kv_read_q8_paged(kvb_stream_t stream, const void* k_pool, const void* v_
  * pool sets kvb_device_error code 4 and those keys read as zeros.  The tensor-core kernel
  * takes head_dim 64 and 128 with n_q / n_kv <= 16, block_size a multiple of 16, codes 16-byte
  * and q 8-byte aligned with q_row_stride a multiple of 4; a general kernel, several times
- * slower, takes the rest.  The workspace (kvb_attention_decode_q8_workspace_bytes; NULL: no
- * KV split) needs no initialisation and belongs to one call at a time: calls that may overlap
- * on the GPU, replayed graphs among them, need one each. */
+ * slower, takes the rest.  The workspace (kvb_attention_decode_q8_workspace_bytes; a smaller
+ * one splits into fewer chunks, NULL not at all) needs no initialisation and belongs to one
+ * call at a time: calls that may overlap on the GPU, replayed graphs among them, need one
+ * each. */
 int kvb_attention_decode_q8(kvb_stream_t stream, const void* q, size_t q_row_stride, const void* kc,
                             const void* vc, const float* ks, const float* vs, size_t seq_stride,
                             size_t cache_len, size_t scale_len, const int32_t* lens, size_t n_seq,

@@ -271,11 +271,17 @@ struct Q8Plan {
 };
 static Q8Plan q8_plan(size_t n_seq, size_t max_len, size_t n_q, size_t n_kv, size_t head_dim,
                       const void* ws, size_t ws_len) {
-    const size_t need = q8_ws_bytes(n_seq, max_len, n_q, n_kv, head_dim);
-    const bool split = need > 0 && ws != nullptr && ws_len >= need && aligned(ws, 16);
     const size_t unit = (size_t)kQ8Warps * q8_tile_keys((int)head_dim);
-    size_t ck = split ? (size_t)q8_chunk_keys(n_seq, n_kv, max_len, head_dim)
-                      : (max_len + unit - 1) / unit * unit;
+    const bool split = q8_ws_bytes(n_seq, max_len, n_q, n_kv, head_dim) > 0 && ws != nullptr &&
+                       aligned(ws, 16);
+    size_t ck = (max_len + unit - 1) / unit * unit;  // one chunk
+    if (split) {  // a smaller workspace takes fewer and longer chunks
+        const size_t fit = ws_len / (n_seq * n_kv * q8_part_floats((int)(n_q / n_kv), (int)head_dim) *
+                                     sizeof(float));
+        const size_t want = (size_t)q8_chunk_keys(n_seq, n_kv, max_len, head_dim);
+        if (fit >= (max_len + want - 1) / want) ck = want;
+        else if (fit >= 2) ck = ((max_len + fit - 1) / fit + unit - 1) / unit * unit;
+    }
     if (ck == 0) ck = unit;
     Q8Plan p;
     p.chunk_keys = (int)ck;

@@ -774,3 +774,25 @@ def test_int8_codes_of_minus_128(g, hd):
         want = torch.from_numpy(c[:, :, :30].astype(np.float32) * s[:, :, :30, None]).to(torch.bfloat16)
         assert torch.equal(got.cpu(), want)
     assert g.device_error() == 0
+
+
+@pytest.mark.parametrize("chunks", [1, 2, 3, 7])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_decode_smaller_workspaces(g, chunks, hd):
+    """A workspace for fewer chunks than the call would take: longer ones, the same attention, and
+    nothing behind the workspace is written."""
+    rng = np.random.default_rng(72)
+    n_q, n_kv, lens = 8, 2, [5000, 0, 4400, 63]
+    q, qf, cache, kv_of, max_seq = _decode_case(rng, lens, n_q, n_kv, hd, "int8", "bf16")
+    n = len(lens) * n_kv * chunks * ((4 * (hd + 2) + 3) // 4 * 4) * 4
+    assert n < g.attention_decode_q8_workspace_bytes(len(lens), max(lens), n_q, n_kv, hd)
+    whole = torch.full((n + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
+    out = torch.empty(len(lens), n_q * hd, dtype=torch.bfloat16, device="cuda")
+    kc, vc, ks, vs = cache
+    g.attention_decode_q8(dev(q), n_q * hd, R.to_dev(kc, "int8"), R.to_dev(vc, "int8"),
+                          torch.from_numpy(ks).cuda(), torch.from_numpy(vs).cuda(), n_kv * max_seq * hd,
+                          torch.tensor(lens, dtype=torch.int32, device="cuda"), max(lens), n_q, n_kv, hd,
+                          max_seq, out, n_q * hd, workspace=whole[:n])
+    R.check_attention(out, qf, kv_of, n_kv, R.default_scale(hd), "bf16", W_EPS, q_eps=R.Q_EPS["int8"])
+    assert bool((whole[n:] == 0xA5).all())
+    assert g.device_error() == 0
