@@ -219,7 +219,6 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
     __shared__ float w_ml[kQ8Warps][2][kQ8MaxGroup];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~uintptr_t(1023));
-    asm volatile("griddepcontrol.launch_dependents;");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, c = lane & 3;
     const int kvh = blockIdx.x, b = blockIdx.y;
@@ -229,14 +228,20 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
     fence_mbar_init();
     __syncthreads();
     const bool early = kRope && a.kv_ready;
-    if (!early) asm volatile("griddepcontrol.wait;" ::: "memory");
+    // The join may start once every CTA has waited: the lengths, which an earlier kernel may have
+    // written, are then final for it.
+    auto wait = [] {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("griddepcontrol.launch_dependents;");
+    };
+    if (!early) wait();
 
     const int len = q8_len(a.lens, a.max_len, b);
     const int n_chunks = (len + a.chunk_keys - 1) / a.chunk_keys;
     const int from_end = a.max_chunks - 1 - (int)blockIdx.z;
     T* outb = reinterpret_cast<T*>(a.out) + (size_t)b * a.out_row_stride + (size_t)kvh * G * HD;
     if (len == 0) {  // no keys: a zero row
-        if (early) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (early) wait();
         if (from_end == 0)
             for (int i = threadIdx.x; i < G * HD; i += blockDim.x) outb[i] = Elem<T>::from_f(0.f);
         return;
@@ -336,7 +341,7 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
         }
     };
     first_tiles(false);
-    if (early) asm volatile("griddepcontrol.wait;" ::: "memory");  // q, the new row
+    if (early) wait();  // q, the new row
     if (appends) {
         size_t crow = 0, head_rows = 0;
         if (warp < 2 && kv8_row(a.c, b, rope_p, crow, head_rows, threadIdx.x == 0)) {
@@ -741,6 +746,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
     __shared__ float ml[kJoinWarps][2];
     __shared__ float4 sums[W > 1 ? kJoinWarps : 1][kCols];
     asm volatile("griddepcontrol.launch_dependents;");
+    // What the lengths come from has completed when this grid starts; the partials have not.
+    int len = a.lens[blockIdx.y];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.group, b = blockIdx.y, n_q = a.n_kv * G;
@@ -754,14 +761,6 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
     const int side = lane / kCols;
     // this warp's parts: w + W q
     auto part = [&](int q) { return w + W * q; };
-    int len = a.lens[b];
-    float4 ahead[kAhead];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-        const int p = part(kLanes * k + side);
-        ahead[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (p < a.fixed) ahead[k] = o4[(size_t)p * per4];
-    }
     if (len < 0 || len > a.max_len) {
         if (threadIdx.x == 0) raise_dev_error(kDevErrBadLength);
         len = len < 0 ? 0 : a.max_len;
@@ -769,10 +768,12 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
     const int own = len > a.key0 ? (len - a.key0 + a.chunk_keys - 1) / a.chunk_keys : 0;
     const int parts = a.fixed + own;
     if (!a.write_all && parts <= 1) return;  // the same for the whole CTA
+    float4 ahead[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
         const int p = part(kLanes * k + side);
-        if (p >= a.fixed && p < parts) ahead[k] = o4[(size_t)p * per4];
+        ahead[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p < parts) ahead[k] = o4[(size_t)p * per4];
     }
     float M = -INFINITY, L = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);

@@ -581,7 +581,7 @@ static int launch_shared_tensor(kvb_stream_t stream, const GeneralDecodeArgs& a,
     j.key0 = paged ? p.key0 : 0;
     j.chunk_keys = p.chunk_keys;
     j.fixed = p.splits;
-    j.max_parts = max_parts > 0 ? max_parts : 1;
+    j.max_parts = max_parts;
     j.part_floats = p.part_floats;
     j.n_kv = a.n_kv;
     j.group = group;
@@ -612,7 +612,8 @@ static int launch_shared(kvb_stream_t stream, const GeneralDecodeArgs& a, const 
                                  : (size_t)a.max_len;
         const SharedPlan p =
             shared_plan(n_seq, shared, own, (size_t)a.n_q, (size_t)a.n_kv, ws_len);
-        if (ws_len >= p.ws_bytes)
+        // (no keys at all: no kernel of this call for the join to follow)
+        if (ws_len >= p.ws_bytes && p.splits + p.max_chunks > 0)
             return launch_shared_tensor<T>(stream, a, src, p, n_seq, own_rows,
                                            static_cast<float*>(ws));
     }

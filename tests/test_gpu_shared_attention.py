@@ -159,6 +159,17 @@ def test_empty_rows(g):
         c.check(out)
 
 
+def test_no_keys_at_all(g):
+    """No prefix and max_len 0, with and without a workspace: zeros, and no report although the
+    lengths are written right before the call."""
+    c = Case(np.random.default_rng(6), 0, [0, 0, 0], 8, 2, 64, "bf16")
+    for ws in (True, False):
+        c.ld.fill_(7)
+        c.ld.zero_()
+        assert bool((c.contiguous(g, ws) == 0).all())
+    assert g.device_error() == 0
+
+
 @pytest.mark.parametrize("hd", [64, 80])
 def test_paged_lengths_below_the_prefix(g, hd):
     """A sequence shorter than shared_len attends to its own first keys only; 0 gives zeros."""
