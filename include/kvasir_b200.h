@@ -480,8 +480,7 @@ int kvb_rope_attention_decode_q8_paged(kvb_stream_t stream, const void* qkv, siz
  * sequence are the same, and are read through row 0 of the block table (whole blocks
  * of a prefix appear in every row, a block that the prefix ends in may be copied for
  * each sequence); row 0 holds them whatever lens[0] is; lens[b] counts them, and a length
- * below shared_len attends to that many of them (V rows of the prefix that hold a NaN or
- * an infinity may then reach that sequence all the same).  Both equal
+ * below shared_len attends to that many of them.  Both equal
  * kvb_attention_decode(_paged) over the same keys up to the order of the f32 sums.  Any
  * head_dim up to 256, any group size.  The tensor-core kernels take head_dim 64 with
  * n_q / n_kv <= 16, scale > 0, block_size a multiple of 64, 16-byte aligned q and caches,

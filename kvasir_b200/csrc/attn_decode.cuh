@@ -68,7 +68,8 @@ struct DecodeArgs {
     // are then requested before griddepcontrol.wait; otherwise nothing is read before it.
     int kv_ready;
     // Partial form (kPart, kvb_attention_decode_shared): keys [key0, lens[b]), key0 a multiple
-    // of 64; every chunk's state goes to the workspace as part part0 + chunk of max_parts.
+    // of 64; every chunk's state goes to the workspace as part part0 + chunk of max_parts.  A
+    // sequence that ends before key0 has its keys past its last whole 64 here, through table row 0.
     int key0 = 0, part0 = 0, max_parts = 0, part_floats = 0;
 };
 
@@ -100,6 +101,10 @@ __device__ __forceinline__ int decode_len(const DecodeArgs& a, int b) {
     return len;
 }
 
+// First own key of a sequence of len keys whose first key0 (a multiple of 64) are shared: the
+// prefix's kernel takes whole 64-key tiles of it.
+__device__ __forceinline__ int own_key0(int len, int key0) { return min(key0, len & ~63); }
+
 // One chunk of attn_decode_kernel: chunk slot `from_end` (counted from the end of
 // the sequence) of kv head kvh of sequence b.  Called by every thread of the CTA.
 // Its result goes to the output row (a one-chunk sequence), to `fold` (this CTA's
@@ -113,7 +118,8 @@ __device__ __forceinline__ void decode_chunk(const CUtensorMap& kmap, const CUte
     const int G = a.group;
 
     const int len = decode_len(a, b);
-    const int key0 = kPart ? a.key0 : 0;
+    const int key0 = kPart ? own_key0(len, a.key0) : 0;
+    const int table_row = kPart && len < a.key0 ? 0 : b;
     const int n_chunks = (len - key0 + a.chunk_keys - 1) / a.chunk_keys;
     T* outb = reinterpret_cast<T*>(a.out) + (size_t)b * a.out_row_stride + (size_t)kvh * G * 64;
     if (kPart && len <= key0) return;  // no own keys: no part
@@ -151,11 +157,11 @@ __device__ __forceinline__ void decode_chunk(const CUtensorMap& kmap, const CUte
     uint64_t* bar_v = &bars[kDecWarps + warp];  // and its V tile, completed separately
     const int row_base = (int)((long long)b * a.seq_rows + (long long)kvh * a.max_seq);
     // paged: lane 0 reads the block of its next tile while the current one loads
-    int blk_next = lane == 0 ? decode_block_of(a, b, key_begin + warp * kDecTileKeys) : 0;
+    int blk_next = lane == 0 ? decode_block_of(a, table_row, key_begin + warp * kDecTileKeys) : 0;
     auto tile_row = [&](int kt0) {  // lane 0: cache row of keys kt0 .. kt0 + 63
         const int row = decode_tile_row(a, b, kvh, row_base, kt0, blk_next);
         const int kn = kt0 + kDecWarps * kDecTileKeys;
-        if (kn < key_end) blk_next = decode_block_of(a, b, kn);
+        if (kn < key_end) blk_next = decode_block_of(a, table_row, kn);
         return row;
     };
     auto issue_k = [&](int row) {

@@ -28,6 +28,7 @@
 // maximum, the sums and O are f32.
 #pragma once
 
+#include "attn_decode.cuh"
 #include "kv8.cuh"
 
 namespace kvb {
@@ -716,7 +717,7 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
 }
 
 // Joins the partial states of every (sequence, head): parts 0 .. fixed - 1, which every
-// sequence has, then one for each chunk of its keys past key0.  Written rows: those with more
+// sequence has, then one for each chunk of its keys past own_key0.  Written rows: those with more
 // than one part (write_all: every row, zeros where a sequence has none).  A programmatic
 // dependent of the kernel that writes the partials.  Latency bounds it, so a row is one warp's (or
 // W of its CTA's eight, parts w, w + W, ..., where there are more than 32): the lanes are laid
@@ -765,7 +766,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
         if (threadIdx.x == 0) raise_dev_error(kDevErrBadLength);
         len = len < 0 ? 0 : a.max_len;
     }
-    const int own = len > a.key0 ? (len - a.key0 + a.chunk_keys - 1) / a.chunk_keys : 0;
+    const int own = (len - own_key0(len, a.key0) + a.chunk_keys - 1) / a.chunk_keys;
     const int parts = a.fixed + own;
     if (!a.write_all && parts <= 1) return;  // the same for the whole CTA
     float4 ahead[kAhead];

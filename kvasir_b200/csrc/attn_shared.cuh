@@ -24,7 +24,10 @@
 // group each do not -- the SM's schedulers favour the oldest, whose slices end early and leave
 // the youngest alone (measured 41 to 71 us for equal slices).  A thread reads its scores from
 // TMEM 32 at a time (maximum, then exponentials).  There is no causal mask; a row's keys end
-// at the prefix's end, or earlier for a paged sequence shorter than the prefix.
+// at the prefix's end, or for a paged sequence shorter than the prefix at its last whole 64 keys
+// (the rest of them are its own kernel's).  The row's O is stored when the first tile past them
+// comes: the products go on for the other rows, and 0 * V is not 0 where V holds a NaN or an
+// infinity.
 // Measured no better: a part of the exponentials as polynomials on the FMA pipe, halves of 32 keys
 // with an S buffer each (110 us; N = 32 products cost the tensor pipe as much as N = 64).
 // Measured on B200 with the own keys and the join: 256 sequences of 32 + 8 heads on 16384 keys
@@ -319,9 +322,13 @@ __global__ void __launch_bounds__(sp_threads(kGroups), kSpMaxGroups / kGroups)
         const int seq = (tile0 + grp) * a.seqs_per_tile + row / a.group, head = row % a.group;
         const bool valid = row < rows && seq < a.n_seq;
         int limit = a.prefix;  // this row's keys
-        if (a.lens && valid) limit = min(limit, max(0, min(a.lens[seq], a.max_len)));
+        if (a.lens && valid) limit = own_key0(max(0, min(a.lens[seq], a.max_len)), limit);
         float m = -INFINITY, l = 0.f;
         bool ok = true;
+        auto part_of_row = [&] {
+            return (((size_t)(valid ? seq : 0) * a.n_kv + kvh) * a.max_parts + split) *
+                   (size_t)a.part_floats;
+        };
         for (int j = 0; j < nt; ++j) {
             ok = warp_all(!s_err && mbar_wait(&bars.s_full[grp], j & 1));
             if (!ok) break;
@@ -329,6 +336,21 @@ __global__ void __launch_bounds__(sp_threads(kGroups), kSpMaxGroups / kGroups)
             const int n_here = limit - (key0 + j * kSpKeys);
             const bool masked = __any_sync(0xffffffffu, n_here < kSpKeys);
             float s[32];
+            // The first tile past a shorter row's keys (whole tiles; where the slice begins past
+            // them the part has no weight)
+            if (masked && j > 0 && __any_sync(0xffffffffu, n_here == 0)) {
+                float* to = a.ws + part_of_row() + head * 64;
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    tmem_ld32(t_o + 32 * hf, s);
+                    tmem_wait_ld();
+                    if (n_here == 0)
+#pragma unroll
+                        for (int c = 0; c < 32; c += 4)
+                            *reinterpret_cast<float4*>(to + 32 * hf + c) =
+                                make_float4(s[c], s[c + 1], s[c + 2], s[c + 3]);
+                }
+            }
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int c = 0; c < kSpKeys; c += 32) {
@@ -407,13 +429,13 @@ __global__ void __launch_bounds__(sp_threads(kGroups), kSpMaxGroups / kGroups)
         // warp's 32 rows go through its quarter of the group's Q tile (its MMAs are done), 32
         // dims at a time, so that eight lanes store a row's 128 bytes: a thread storing its own
         // row touches 32 lines an instruction.
-        const size_t off = (((size_t)(valid ? seq : 0) * a.n_kv + kvh) * a.max_parts + split) *
-                           (size_t)a.part_floats;
+        const size_t off = part_of_row();
         if (valid) {
             a.ws[off + a.group * 64 + head] = ok ? m : -INFINITY;
             a.ws[off + a.group * 65 + head] = ok ? l : 0.f;
         }
-        const long long dst = valid ? (long long)(off + head * 64) : -1;
+        const bool whole = valid && limit > key0 + (nt - 1) * kSpKeys;  // else O is stored, or void
+        const long long dst = whole ? (long long)(off + head * 64) : -1;
         float4* stage = reinterpret_cast<float4*>(sq + grp * kSpQBytes + quarter * 4096);
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {

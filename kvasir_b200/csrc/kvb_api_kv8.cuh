@@ -591,6 +591,12 @@ static int launch_shared_tensor(kvb_stream_t stream, const GeneralDecodeArgs& a,
     return launch_join<T, 64>(stream, j, n_seq);
 }
 
+// The most keys that the own kernel of a paged call has of a sequence, `shared` (whole tiles) by the
+// prefix's: one at least where a sequence may end inside the prefix.
+static size_t shared_paged_own(size_t max_len, size_t shared) {
+    return max_len > shared ? max_len - shared : shared > 0 ? 1 : 0;
+}
+
 // The tensor-core kernels where shape, alignment and workspace allow them (own_rows: rows of 64
 // elements of the contiguous caches), else the general kernel.
 template <typename T>
@@ -608,8 +614,7 @@ static int launch_shared(kvb_stream_t stream, const GeneralDecodeArgs& a, const 
         // Paged: whole 64-key tiles of the prefix for all at once; each sequence reads the rest
         // through its own table row.  Contiguous: all of the prefix.
         const size_t shared = paged ? (size_t)src.prefix / 64 * 64 : (size_t)src.prefix;
-        const size_t own = paged ? (size_t)(a.max_len > (int)shared ? a.max_len - (int)shared : 0)
-                                 : (size_t)a.max_len;
+        const size_t own = paged ? shared_paged_own(a.max_len, shared) : (size_t)a.max_len;
         const SharedPlan p =
             shared_plan(n_seq, shared, own, (size_t)a.n_q, (size_t)a.n_kv, ws_len);
         // (no keys at all: no kernel of this call for the join to follow)
@@ -874,8 +879,9 @@ size_t kvb_attention_decode_shared_workspace_bytes(size_t n_seq, size_t shared_l
         return 0;
     // contiguous, or paged with the prefix cut to whole 64-key tiles: the larger need
     const size_t a = shared_plan(n_seq, shared_len, max_own, n_q, n_kv, SIZE_MAX).ws_bytes;
-    const size_t b = shared_plan(n_seq, shared_len / 64 * 64, max_own + shared_len % 64, n_q, n_kv,
-                                 SIZE_MAX).ws_bytes;
+    const size_t tiles = shared_len / 64 * 64;
+    const size_t b = shared_plan(n_seq, tiles, kvb::shared_paged_own(shared_len + max_own, tiles), n_q,
+                                 n_kv, SIZE_MAX).ws_bytes;
     return a > b ? a : b;
 }
 

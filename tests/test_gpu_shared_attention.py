@@ -363,3 +363,37 @@ def test_smaller_workspaces(g, parts, paged):
     c.check(c.paged(g, 64) if paged else c.contiguous(g))
     assert bool((whole[n:] == 0xA5).all())
     assert g.device_error() == 0
+
+
+@pytest.mark.parametrize("prefix,max_len", [(256, 256), (300, 340), (300, 150), (5000, 5003)])
+@pytest.mark.parametrize("n_seq", [5, 40, 80])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_paged_lengths_below_the_prefix_ignore_later_values(g, prefix, max_len, n_seq, dtype):
+    """NaN and infinities in V (and NaN in K) past a sequence's length do not reach it, wherever in
+    the prefix it ends, with one, two and four row tiles to a CTA, and with the general kernel;
+    the sequences that attend to such a V row are NaN."""
+    rng = np.random.default_rng(prefix + n_seq)
+    c = Case(rng, prefix, [40] * n_seq, 8, 2, 64, dtype)
+    bad = prefix // 2 + 3  # in the middle of a tile
+    (kp, vp), table = c.pools(64)
+    blk, at = table[0, bad // 64], bad % 64
+    vp[blk, :, at] = 0x7FFF
+    if bad + 30 < prefix:
+        vp[table[0, (bad + 30) // 64], :, (bad + 30) % 64] = 0x7F80 if dtype == "bf16" else 0x7C00
+    last = table[0, prefix // 64 - 1]
+    kp[last, :, 63] = 0x7FFF  # the last key of the prefix's last whole tile
+    short = [0, 1, 63, 64, 65, bad - 1, bad, bad + 1, prefix // 64 * 64 - 1, max_len]
+    short = [min(short[3 * i % len(short)], max_len) for i in range(n_seq)]
+    clean = [i for i, n in enumerate(short) if n <= bad]
+    lens = torch.tensor(short, dtype=torch.int32, device="cuda")
+    for ws in (c.ws(g, max(max_len - prefix, 0)), None):
+        out = c.out()
+        g.attention_decode_shared_paged(dev(c.q, dtype), 512, dev(kp, dtype), dev(vp, dtype),
+                                        torch.from_numpy(table).cuda(), table.shape[1], 64, prefix, lens,
+                                        max_len, 8, 2, 64, out, 512, workspace=ws)
+        assert g.device_error() == 0
+        R.check_attention(out[clean], c.qf[clean],
+                          lambda i, h: (c.f[0][h, :short[clean[i]]], c.f[1][h, :short[clean[i]]]), c.n_kv,
+                          R.default_scale(64), dtype, W_EPS[dtype])
+        rest = [i for i in range(n_seq) if i not in clean]
+        assert bool(out[rest].isnan().all())
