@@ -21,8 +21,11 @@
 // 128 dims).  Q, e4m3: f16 as it is; bf16 scaled by a power of two to a largest element in
 // [2^14, 2^15) and rounded to f16, which is exact for elements down to 2^-31 of the
 // largest.  Weights: w = p * v_scale * 2^n, n such that the largest V scale seen makes
-// w < 2^14, rounded once to f16 (half a step, 2^-11 of a weight; steps of 2^-24 below
-// 2^-14, so a key whose V scale is 2^28 times smaller than the largest keeps ten bits).
+// w <= 2^14, rounded once to f16: half a step, 2^-11 of a weight, or 2^-25 where w is below
+// 2^-14.  That holds while the V scales, a tile's and those before it, lie in two neighbouring
+// magnitudes of 2^8: p = 1 then gives w >= 2^-2, and the second term is at most 2^-23 of such a
+// key's weight.  Where they do not (a V row far above the others may have no weight at all), the
+// tile's products are f32 multiply-adds on the CUDA cores, three times the instructions.
 // A remainder as in the 16-bit kernels would double the P V products; the codes
 // themselves are within 2^-8 of a row's largest value at best.  Scores, the running
 // maximum, the sums and O are f32.
@@ -196,6 +199,23 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int byt
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
                  : "memory");
+}
+
+// Magnitude of a V scale: bit i for exponents 8 i .. 8 i + 7 (2^(8 i + 8 - 127) itself included,
+// 2^(8 i - 127) not); no bit for 0, whose shift is beyond 31.
+__device__ __forceinline__ uint32_t mag_bit(float scale) {
+    uint32_t r;
+    asm("shl.b32 %0, %1, %2;" : "=r"(r) : "r"(1u), "r"((abs_bits(scale) - 1u) >> 26));
+    return r;
+}
+// 2^(133 - 8 i): takes magnitude i (1 .. 31) to 2^14 at most.
+__device__ __forceinline__ float q8_v_factor(int i) {
+    return __uint_as_float((uint32_t)(260 - 8 * i) << 23);
+}
+// to / from, powers of two, or 0 where that is below f32's normal numbers.
+__device__ __forceinline__ float q8_v_rescale(float from, float to) {
+    const int e = 127 + (int)(__float_as_uint(to) >> 23) - (int)(__float_as_uint(from) >> 23);
+    return e > 0 ? __uint_as_float((uint32_t)e << 23) : 0.f;
 }
 
 // Byte offset of 16-byte chunk `ch` of row r in a tile that the tensor copy wrote with a
@@ -451,7 +471,10 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
 #pragma unroll
         for (int j = 0; j < DT; ++j) o[j][nt][0] = o[j][nt][1] = o[j][nt][2] = o[j][nt][3] = 0.f;
     }
-    int ev = 14;  // biased exponent of the largest V scale seen; O is in units of 2^(ev - 140)
+    // Magnitudes (eighths of the exponent range, a bit each) of the V scales so far, two
+    // neighbours at most; O is in units of 1 / vf, the factor that takes the upper one below 2^14.
+    uint32_t seen = 0;
+    float vf = q8_v_factor(1);
     // Two tiles per warp in flight, K and V on barriers of their own: the K of the tile
     // after next is requested once the scores are out of this one, its V once P V has read
     // this V.
@@ -586,29 +609,103 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
                              : "memory");
             __syncwarp();
         }
-        // ---- V scale exponent: O is rescaled where a larger one appears
-        uint32_t vmax = __float_as_uint(vs[lane]) & 0x7fffffffu;
-        if (KT == 64) vmax = max(vmax, __float_as_uint(vs[lane + 32]) & 0x7fffffffu);
-        const int en = max(ev, (int)(__reduce_max_sync(0xffffffffu, vmax) >> 23));
-        const float vf = __uint_as_float((uint32_t)(267 - en) << 23);  // 2^(140 - en)
-        const int down = 127 + ev - en;  // exponent field of 2^(ev - en)
-        const float rv = down > 0 ? __uint_as_float((uint32_t)down << 23) : 0.f;
-        ev = en;
+        // ---- V scale magnitudes: O is rescaled where larger ones appear.  (The first V fragment
+        // is read beside them: this check costs 1.1 % of a long pass, 2.3 % with its latency bare.)
+        uint32_t first[4];
+        ldsm_x4_t(vb + q8_smem_off<HD>(lane & 15, lane >> 4), first[0], first[1], first[2], first[3]);
+        uint32_t mags = mag_bit(vs[lane]);
+        if (KT == 64) mags |= mag_bit(vs[lane + 32]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float ao = al[nt][e] * rv;
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
                 for (int j = 0; j < DT; ++j) {
-                    o[j][nt][e] *= ao;
-                    o[j][nt][e + 2] *= ao;
+                    o[j][nt][e] *= al[nt][e];
+                    o[j][nt][e + 2] *= al[nt][e];
                 }
+        float vt = vf;  // the MMA's factor: 0 where the tile is done without it
+        if (__any_sync(0xffffffffu, mags & ~seen)) {
+            mags = __reduce_or_sync(0xffffffffu, mags) | seen;
+            auto rescale = [&](float r) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int j = 0; j < DT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[j][nt][e] *= r;
+            };
+            const int top = max(31 - __clz(mags), 1);
+            float r = 1.f;  // 2^ of the change of O's unit
+            if (mags & ~(3u << (top - 1))) {
+                // Far apart: w = p * scale in f32, its largest sets the unit, and the products
+                // are multiply-adds.
+                uint32_t wmax = 0;
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            s[t][nt][e] *= vs[16 * t + g + 8 * (e >> 1)];
+                            wmax = max(wmax, abs_bits(s[t][nt][e]));
+                        }
+                const int wtop = max((int)(__reduce_max_sync(0xffffffffu, wmax) >> 26), 1);
+                if (q8_v_factor(wtop) < vf) {
+                    r = q8_v_rescale(vf, q8_v_factor(wtop));
+                    vf = q8_v_factor(wtop);
+                    seen = 1u << wtop;
+                }
+                rescale(r);
+#pragma unroll
+                for (int t = 0; t < 2 * MT; ++t)
+#pragma unroll 1
+                    for (int i = 0; i < 8; ++i) {  // key 8 t + i: its weights are in the lanes of row i
+                        float w[NT][2];
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                w[nt][e] = vf * __shfl_sync(0xffffffffu, s[t / 2][nt][2 * (t % 2) + e],
+                                                            4 * i + c);
+#pragma unroll
+                        for (int j = 0; j < DT; ++j) {
+                            uint16_t v;
+                            asm volatile("ld.shared.u16 %0, [%1];"
+                                         : "=h"(v)
+                                         : "r"(vb + q8_smem_off<HD>(8 * t + i, j) + 2 * g)
+                                         : "memory");
+                            const float x0 = kv8_value<kFmt>((uint8_t)v);
+                            const float x1 = kv8_value<kFmt>((uint8_t)(v >> 8));
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    o[j][nt][e] += w[nt][e] * x0;
+                                    o[j][nt][e + 2] += w[nt][e] * x1;
+                                }
+                        }
+                    }
+                vt = 0.f;
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        s[t][nt][0] = s[t][nt][1] = s[t][nt][2] = s[t][nt][3] = 0.f;
+            } else {
+                if (q8_v_factor(top) < vf) {
+                    r = q8_v_rescale(vf, q8_v_factor(top));
+                    vf = q8_v_factor(top);
+                }
+                seen = mags;
+                vt = vf;
+                rescale(r);
             }
+        }
         // ---- O^T += V^T P^T
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            const float v0 = vs[16 * t + g] * vf, v1 = vs[16 * t + g + 8] * vf;
+            const float v0 = vs[16 * t + g] * vt, v1 = vs[16 * t + g + 8] * vt;
             uint32_t pf[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -619,7 +716,14 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
 #pragma unroll
             for (int j = 0; j < DT; j += 2) {
                 uint32_t w0, w1, w2, w3, af[4];
-                ldsm_x4_t(vb + q8_smem_off<HD>(r, j + (lane >> 4)), w0, w1, w2, w3);
+                if (t == 0 && j == 0) {
+                    w0 = first[0];
+                    w1 = first[1];
+                    w2 = first[2];
+                    w3 = first[3];
+                } else {
+                    ldsm_x4_t(vb + q8_smem_off<HD>(r, j + (lane >> 4)), w0, w1, w2, w3);
+                }
                 codes_evens_odds<kFmt>(w0, af[0], af[1]);
                 codes_evens_odds<kFmt>(w1, af[2], af[3]);
 #pragma unroll
@@ -655,7 +759,7 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
         __syncwarp();
     }
     // ---- merge the four warps' states through shared memory
-    const float unit = __uint_as_float((uint32_t)(ev - 13) << 23);  // 2^(ev - 140)
+    const float unit = __uint_as_float((254u << 23) - __float_as_uint(vf));  // 1 / vf, a power of two
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll

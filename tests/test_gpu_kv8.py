@@ -796,3 +796,32 @@ def test_decode_smaller_workspaces(g, chunks, hd):
     R.check_attention(out, qf, kv_of, n_kv, R.default_scale(hd), "bf16", W_EPS, q_eps=R.Q_EPS["int8"])
     assert bool((whole[n:] == 0xA5).all())
     assert g.device_error() == 0
+
+
+@pytest.mark.parametrize("hd", [64, 128, 80])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("ratio", [2.0 ** 12, 2.0 ** 13, 2.0 ** 30, 2.0 ** 45, 2.0 ** 100])
+@pytest.mark.parametrize("group", [4, 12])
+def test_a_large_v_row_without_weight(g, hd, fmt, ratio, group):
+    """A V row far above the others leaves them their precision: where no head gives its key weight,
+    and where one head of the group does and the others do not.  The f64 bound per head."""
+    rng = np.random.default_rng(group)
+    n_kv, lens = 2, [700, 64, 33, 3000]
+    n_q = n_kv * group
+    for heads_on in (0, 1):
+        q, qf, cache, kv_of, max_seq = _decode_case(rng, lens, n_q, n_kv, hd, fmt, "bf16")
+        x = np.abs(qf) + 0.5
+        x[:, ::group] *= -1 if heads_on else 1  # the first head of each group
+        q = O.from_f32(x.astype(np.float32).ravel())
+        qf = O.to_f32(q).astype(np.float64).reshape(x.shape)
+        kc, vc, ks, vs = cache
+        for b, n in enumerate(lens):
+            for key in (5, n // 2, n - 1):
+                kc[b, :, key] = R.quantise(np.full((1, hd), -8.0, np.float32), fmt)[0]
+                ks[b, :, key] = R.quantise(np.full((1, hd), -8.0, np.float32), fmt)[1]
+                vs[b, :, key] *= np.float32(ratio)
+        for ws in (True, False):
+            out = _run_decode(g, q, cache, lens, n_q, n_kv, hd, max_seq, fmt, "bf16", workspace=ws)
+            assert g.device_error() == 0
+            R.check_attention(out, qf, kv_of, n_kv, R.default_scale(hd), "bf16", W_EPS,
+                              f"heads_on {heads_on}", q_eps=R.Q_EPS[fmt])
