@@ -480,9 +480,12 @@ int kvb_rope_attention_decode_q8_paged(kvb_stream_t stream, const void* qkv, siz
  * sequence are the same, and are read through row 0 of the block table (whole blocks
  * of a prefix appear in every row, a block that the prefix ends in may be copied for
  * each sequence); row 0 holds them whatever lens[0] is; lens[b] counts them, and a length
- * below shared_len attends to that many of them.  Both equal
- * kvb_attention_decode(_paged) over the same keys up to the order of the f32 sums.  Any
- * head_dim up to 256, any group size.  The tensor-core kernels take head_dim 64 with
+ * below shared_len attends to that many of them.  Both compute
+ * kvb_attention_decode(_paged) over the same keys: f32 scores, maxima, sums and accumulation.
+ * The tensor-core kernels multiply V by a key's weight in 16 bits: bf16 head and remainder (2^-15
+ * of a weight) as kvb_attention_decode does; for f16 caches a prefix key's weight is one f16 (2^-11
+ * of it, 2^-32 of the largest for weights below 2^-21), where kvb_attention_decode adds the
+ * remainder.  Any head_dim up to 256, any group size.  The tensor-core kernels take head_dim 64 with
  * n_q / n_kv <= 16, scale > 0, block_size a multiple of 64, 16-byte aligned q and caches,
  * q_row_stride a multiple of 8, and a workspace of
  * kvb_attention_decode_shared_workspace_bytes (no initialisation; one call at a time, as

@@ -147,7 +147,11 @@ __global__ void __launch_bounds__(sp_threads(kGroups), kSpMaxGroups / kGroups)
     __shared__ SharedBars bars;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int s_err;
-    constexpr bool kSplitP = Elem<T>::kDtype == KVB_BF16;  // P as head + remainder
+    // bf16: P as head + remainder (2^-15 of a weight).  f16: one f16, P = 2^(7 + s - m) of at most
+    // 2^15 (m is within 2^8 of the row's maximum): half a step, 2^-11 of a weight, or 2^-32 of 2^m
+    // where it is below 2^-21 of that; a remainder would double the P V products.
+    constexpr bool kSplitP = Elem<T>::kDtype == KVB_BF16;
+    constexpr float kShift = kSplitP ? 0.f : 7.f;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~uintptr_t(1023));
     constexpr int kStages = sp_stages(kGroups);
@@ -367,7 +371,7 @@ __global__ void __launch_bounds__(sp_threads(kGroups), kSpMaxGroups / kGroups)
                     for (int u = 0; u < 4; ++u) mx[u] = max3f(mx[u], s[i + 2 * u], s[i + 2 * u + 1]);
             }
             const float mt = fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]) * a.scale_log2;
-            // m is raised only past 2^8: P <= 256 then, and O and l are rescaled rarely
+            // m is raised only past 2^8: P <= 2^(8 + kShift) then, and O and l are rescaled rarely
             float alpha = 1.f;
             bool rescale = false;
             if (mt > m + kPfRescaleLog2) {
@@ -375,7 +379,7 @@ __global__ void __launch_bounds__(sp_threads(kGroups), kSpMaxGroups / kGroups)
                 rescale = m != -INFINITY;
                 m = mt;
             }
-            const float ref = m == -INFINITY ? 0.f : m;  // no key yet: P = 2^(-inf) = 0
+            const float ref = (m == -INFINITY ? 0.f : m) - kShift;  // no key yet: P = 2^(-inf) = 0
             if (__any_sync(0xffffffffu, rescale)) {  // S(j) is there, so P(j-1) V is complete
                 const float f = rescale ? alpha : 1.f;
 #pragma unroll
@@ -431,7 +435,7 @@ __global__ void __launch_bounds__(sp_threads(kGroups), kSpMaxGroups / kGroups)
         // row touches 32 lines an instruction.
         const size_t off = part_of_row();
         if (valid) {
-            a.ws[off + a.group * 64 + head] = ok ? m : -INFINITY;
+            a.ws[off + a.group * 64 + head] = ok ? m - kShift : -INFINITY;  // what O and l are relative to
             a.ws[off + a.group * 65 + head] = ok ? l : 0.f;
         }
         const bool whole = valid && limit > key0 + (nt - 1) * kSpKeys;  // else O is stored, or void

@@ -397,3 +397,36 @@ def test_paged_lengths_below_the_prefix_ignore_later_values(g, prefix, max_len, 
                           R.default_scale(64), dtype, W_EPS[dtype])
         rest = [i for i in range(n_seq) if i not in clean]
         assert bool(out[rest].isnan().all())
+
+
+def test_f16_weights_far_below_the_largest(g):
+    """One key 17 above 16384 others whose V rows have one sign, in a single slice of the prefix.
+    A weight is one f16 of at most 2^15 (the reference is within 2^8 of the row's maximum, and
+    here equals it): half a step is 2^-11 of the weight, or 2^-25 below 2^-14, which is 2^-32 of
+    the largest weight for each key.  Scores: multiples of 1/8, exact."""
+    n_q, n_kv, hd, n = 4, 2, 64, 16384
+    q = np.zeros((1, n_q, hd), np.float32)
+    q[:, :, 0] = 17.0
+    k = np.zeros((n_kv, n, hd), np.float32)
+    k[:, 0, 0] = 8.0
+    v = np.abs(np.random.default_rng(81).normal(1.0, 0.1, (n_kv, n, hd))).astype(np.float32)
+    v[:, 0] = 0.0
+    qb, kb, vb = (O.from_f32(x.ravel(), "f16") for x in (q, k, v))
+    vf = _f64(vb, "f16", n_kv, n, hd)
+    own = torch.zeros(1, n_kv, 1, hd, dtype=torch.float16, device="cuda")
+    out = torch.empty(1, n_q * hd, dtype=torch.float16, device="cuda")
+    ws = torch.empty(n_kv * 2 * (hd + 2) * 4, dtype=torch.uint8, device="cuda")  # one part: O, m, l
+    g.attention_decode_shared(dev(qb, "f16"), n_q * hd, dev(kb, "f16").view(n_kv, n, hd),
+                              dev(vb, "f16").view(n_kv, n, hd), n, n, own, own, n_kv * hd,
+                              torch.zeros(1, dtype=torch.int32, device="cuda"), 0, n_q, n_kv, hd, 1, out,
+                              n_q * hd, workspace=ws)
+    p = np.full(n, np.exp(-17.0))
+    p[0] = 1.0
+    p /= p.sum()
+    want = np.stack([p @ vf[h // 2] for h in range(n_q)])
+    A = want  # all terms have one sign
+    tol = (2.0 ** -11 + 2.0 ** -11 + 2.0 ** -13 + np.expm1(2 * 68 * 2.0 ** -24 * 17)) * A + \
+        2.0 ** -32 * np.abs(vf).sum(1)[[h // 2 for h in range(n_q)]]
+    err = np.abs(out.float().cpu().numpy().astype(np.float64).reshape(n_q, hd) - want)
+    assert np.all(err <= tol), np.max(err / tol)
+    assert g.device_error() == 0
