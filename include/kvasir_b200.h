@@ -420,7 +420,8 @@ int kvb_kv_read_q8_paged(kvb_stream_t stream, const void* k_pool, const void* v_
 
 /* Batched single-query decode attention over an 8-bit cache: kvb_attention_decode's
  * arguments and result (f32 scores, sums and accumulation) on the values that the
- * rows stand for.  Any head_dim up to 256, any group size; a block entry outside the
+ * rows stand for.  A sequence without keys gives a zero row, one whose scores are all
+ * -infinity (f32 overflow) NaN.  Any head_dim up to 256, any group size; a block entry outside the
  * pool sets kvb_device_error code 4 and those keys read as zeros.  The tensor-core kernel
  * takes head_dim 64 and 128 with n_q / n_kv <= 16, block_size a multiple of 16, codes 16-byte
  * and q 8-byte aligned with q_row_stride a multiple of 4; a general kernel, several times
@@ -475,7 +476,8 @@ int kvb_rope_attention_decode_q8_paged(kvb_stream_t stream, const void* qkv, siz
  * of pk / pv [n_kv, prefix_rows, head_dim], then to its own keys [0, lens[b]) of its
  * cache (kc/vc + b*seq_stride, [n_kv, max_seq, head_dim]; lens does not count the
  * prefix, 0 <= lens[b] <= max_len <= max_seq).  Positions are the caller's: own keys
- * are rotated at prefix_len + i.  A sequence with neither gives a zero row.  Paged:
+ * are rotated at prefix_len + i.  A sequence with neither gives a zero row, one whose scores
+ * are all -infinity NaN.  Paged:
  * the caches of kvb_attention_decode_paged; the first shared_len keys of every
  * sequence are the same, and are read through row 0 of the block table (whole blocks
  * of a prefix appear in every row, a block that the prefix ends in may be copied for

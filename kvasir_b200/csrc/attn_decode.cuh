@@ -318,14 +318,18 @@ __device__ __forceinline__ void decode_chunk(const CUtensorMap& kmap, const CUte
         mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
         mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
         const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
-        const float al0 = exp2f(m0 - mn0), al1 = exp2f(m1 - mn1);
+        // kPart: a state without weight where every score so far is -infinity (the other parts of
+        // the row may have keys)
+        const float ref0 = kPart && mn0 == -INFINITY ? 0.f : mn0;
+        const float ref1 = kPart && mn1 == -INFINITY ? 0.f : mn1;
+        const float al0 = exp2f(m0 - ref0), al1 = exp2f(m1 - ref1);
         float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            s[j][0] = exp2f(s[j][0] - mn0);
-            s[j][1] = exp2f(s[j][1] - mn0);
-            s[j][2] = exp2f(s[j][2] - mn1);
-            s[j][3] = exp2f(s[j][3] - mn1);
+            s[j][0] = exp2f(s[j][0] - ref0);
+            s[j][1] = exp2f(s[j][1] - ref0);
+            s[j][2] = exp2f(s[j][2] - ref1);
+            s[j][3] = exp2f(s[j][3] - ref1);
             sum0 += s[j][0] + s[j][1];
             sum1 += s[j][2] + s[j][3];
         }

@@ -822,7 +822,8 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
 
 // Joins the partial states of every (sequence, head): parts 0 .. fixed - 1, which every
 // sequence has, then one for each chunk of its keys past own_key0.  Written rows: those with more
-// than one part (write_all: every row, zeros where a sequence has none).  A programmatic
+// than one part (write_all: every row, zeros where a sequence has no keys).  A row that has keys
+// but no score above -infinity is 0 / 0, as it is in one chunk.  A programmatic
 // dependent of the kernel that writes the partials.  Latency bounds it, so a row is one warp's (or
 // W of its CTA's eight, parts w, w + W, ..., where there are more than 32): the lanes are laid
 // out as (part, four neighbouring outputs), each requests its first kAhead parts' O, 16 bytes
@@ -839,6 +840,7 @@ struct JoinArgs {
     int fixed, max_parts, part_floats;
     int n_kv, group;
     int write_all;
+    int prefix;  // keys of every sequence that its length does not count
     uint16_t* out;
     long long out_row_stride;
 };
@@ -949,7 +951,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
         }
     }
     if (!have || lane >= kCols) return;
-    const float inv = L == 0.f ? 0.f : 1.f / L;  // no keys at all: zeros
+    const float inv = len + a.prefix > 0 ? 1.f / L : 0.f;
     T* out = reinterpret_cast<T*>(a.out) + (size_t)b * a.out_row_stride + (size_t)head * HD + 4 * lane;
     if ((reinterpret_cast<uintptr_t>(out) & 7) == 0) {
         *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack(x.x * inv, x.y * inv),

@@ -347,6 +347,7 @@ static int launch_q8_tensor(kvb_stream_t stream, Q8DecodeArgs& a, size_t n_seq, 
     j.n_kv = a.c.n_kv;
     j.group = a.group;
     j.write_all = 0;
+    j.prefix = 0;
     j.out = a.out;
     j.out_row_stride = a.out_row_stride;
     return launch_join<T, HD>(stream, j, n_seq);
@@ -586,6 +587,7 @@ static int launch_shared_tensor(kvb_stream_t stream, const GeneralDecodeArgs& a,
     j.n_kv = a.n_kv;
     j.group = group;
     j.write_all = 1;
+    j.prefix = paged ? 0 : src.prefix;
     j.out = a.out;
     j.out_row_stride = a.out_row_stride;
     return launch_join<T, 64>(stream, j, n_seq);

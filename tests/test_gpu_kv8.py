@@ -825,3 +825,31 @@ def test_a_large_v_row_without_weight(g, hd, fmt, ratio, group):
             assert g.device_error() == 0
             R.check_attention(out, qf, kv_of, n_kv, R.default_scale(hd), "bf16", W_EPS,
                               f"heads_on {heads_on}", q_eps=R.Q_EPS[fmt])
+
+
+@pytest.mark.parametrize("hd", [64, 128, 80])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_scores_of_minus_infinity(g, fmt, hd):
+    """Scores that overflow to -infinity: NaN where a row has no other (whatever the workspace),
+    and no weight beside finite ones."""
+    rng = np.random.default_rng(92)
+    n_q, n_kv, lens = 8, 2, [5000, 40, 0]
+    q, qf, cache, kv_of, max_seq = _decode_case(rng, lens, n_q, n_kv, hd, fmt, "bf16")
+    x = (np.abs(qf) + 0.5) * 2.0 ** 60
+    q = O.from_f32(x.astype(np.float32).ravel())
+    kc, vc, ks, vs = cache
+    one = R.quantise(np.full((1, hd), -1.0, np.float32), fmt)[0]
+    kc[0, :], ks[0, :] = one, 2.0 ** 90  # every key of sequence 0
+    kc[1, 0, :33], ks[1, 0, :33] = one, 2.0 ** 90  # KV head 0 of sequence 1: keys 33 .. 39 are left
+    ks[1] = np.where(ks[1] < 1e10, ks[1] * np.float32(2.0 ** -60), ks[1])  # those score as usual
+
+    def left(b, h):
+        k, v = kv_of(b, h)
+        return (k[33:], v[33:]) if h == 0 else (k, v)
+    qs = O.to_f32(q).astype(np.float64).reshape(x.shape)
+    for ws in (True, False):
+        out = _run_decode(g, q, cache, lens, n_q, n_kv, hd, max_seq, fmt, "bf16", workspace=ws)
+        assert g.device_error() == 0
+        assert bool(out[0].isnan().all()) and bool((out[2] == 0).all())
+        R.check_attention(out[1:2], qs[1:2], lambda b, h: left(1, h), n_kv, R.default_scale(hd), "bf16",
+                          W_EPS, q_eps=R.Q_EPS[fmt])

@@ -430,3 +430,33 @@ def test_f16_weights_far_below_the_largest(g):
     err = np.abs(out.float().cpu().numpy().astype(np.float64).reshape(n_q, hd) - want)
     assert np.all(err <= tol), np.max(err / tol)
     assert g.device_error() == 0
+
+
+@pytest.mark.parametrize("hd", [64, 80])
+def test_scores_of_minus_infinity(g, hd):
+    """Keys whose scores are all -infinity have no weight beside others, in the prefix or among a
+    sequence's own; a row that has keys and no other scores is NaN, one without keys zeros; the
+    same with and without a workspace."""
+    rng = np.random.default_rng(91)
+    for prefix, own, inf_prefix, inf_own in ((300, 200, 300, 200), (300, 200, 300, 0), (300, 200, 0, 200),
+                                             (300, 200, 64, 70), (0, 200, 0, 200), (0, 200, 0, 130)):
+        c = Case(rng, prefix, [own, 0, own - 3], 8, 2, hd, "bf16")
+        c.q = O.from_f32(np.abs(O.to_f32(c.q)) + np.float32(0.5))
+        c.qf = _f64(c.q, "bf16", 3, 8, hd)
+        c.pk[:, :inf_prefix] = c.kc[:, :, :inf_own] = 0xFF80
+        want = c.qf * 0
+        for b in range(3):
+            n = c.lens[b]
+            for h in range(2):
+                k = np.concatenate([c.f[0][h, inf_prefix:prefix], c.f[2][b, h, min(inf_own, n):n]])
+                v = np.concatenate([c.f[1][h, inf_prefix:prefix], c.f[3][b, h, min(inf_own, n):n]])
+                want[b, 4 * h:4 * h + 4] = R.attention(c.qf[b, 4 * h:4 * h + 4], k, v,
+                                                       R.default_scale(hd))[0] if len(k) else \
+                    (np.nan if prefix + n else 0.0)
+        for ws in (True, False):
+            for out in (c.contiguous(g, ws), c.paged(g, 64, ws)):
+                got = out.float().cpu().numpy().reshape(want.shape)
+                # half a bf16 step is 2^-8 of a value; the averages of unit normals here are below 4, and the
+                # weights (2^-15 of each) and f32 sums far below 2^-8
+                np.testing.assert_allclose(got, want, rtol=2.0 ** -8, atol=2.0 ** -8, equal_nan=True)
+    assert g.device_error() == 0
