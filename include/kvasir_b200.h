@@ -450,7 +450,9 @@ size_t kvb_attention_decode_q8_workspace_bytes(size_t n_seq, size_t max_len, siz
  * kvb_rope_kv_append_q8 of one row per sequence at position lens[b] - 1, then
  * kvb_attention_decode_q8, bit for bit, as kvb_rope_attention_decode does for 16-bit
  * caches: qkv [n_seq, (n_q + 2 n_kv) * head_dim] stays unrotated, the codes and scales of
- * the new rows are written.  head_dim 64 or 128, n_q / n_kv <= 16, block_size a multiple
+ * the new rows are written.  A sequence of length 0 has no new row and gives a zero row; a length
+ * past max_len is reported as by both calls, and a new row of which the block lies outside the pool
+ * is reported and not written (its q is rotated all the same).  head_dim 64 or 128, n_q / n_kv <= 16, block_size a multiple
  * of 16, 16-byte aligned buffers; otherwise KVB_ERR_UNSUPPORTED.  Workspace as for
  * kvb_attention_decode_q8. */
 int kvb_rope_attention_decode_q8(kvb_stream_t stream, const void* qkv, size_t qkv_len,

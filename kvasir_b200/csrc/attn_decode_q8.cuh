@@ -277,10 +277,12 @@ __global__ void __launch_bounds__(128, kQ8CtasPerSm)
     const int key_end = min(len, key_begin + a.chunk_keys);
     const int row_base = (int)(b * a.c.seq_rows + (long long)kvh * a.c.max_seq);
     const int pshift = __ffs(a.piece) - 1;
-    int rope_p = -1;  // the new token's position (-1: none, or outside the tables)
+    // The new token's position (-1: none, or outside the tables or the cache).  A length past
+    // max_len is clamped for the attention alone: row max_len - 1 holds another token.
+    int rope_p = -1;
     if (kRope) {
-        rope_p = len - 1;
-        if (rope_p >= a.rope_max_pos) {
+        rope_p = a.lens[b] - 1;
+        if (rope_p >= a.rope_max_pos || rope_p >= a.c.max_seq) {
             if (threadIdx.x == 0) raise_dev_error(kDevErrBadPosition);
             rope_p = -1;
         }

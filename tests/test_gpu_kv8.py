@@ -853,3 +853,50 @@ def test_scores_of_minus_infinity(g, fmt, hd):
         assert bool(out[0].isnan().all()) and bool((out[2] == 0).all())
         R.check_attention(out[1:2], qs[1:2], lambda b, h: left(1, h), n_kv, R.default_scale(hd), "bf16",
                           W_EPS, q_eps=R.Q_EPS[fmt])
+
+
+@pytest.mark.parametrize("hd,block", [(64, 0), (128, 0), (64, 16)])
+def test_fused_step_with_lengths_out_of_range(g, hd, block):
+    """Lengths past max_len and past the cache, and negative ones: reported, and no row that is in
+    the cache is lost -- the step writes what the append writes at lens - 1, and attends as the
+    attention does."""
+    rng = np.random.default_rng(93)
+    n_q, n_kv, max_seq, max_len, fmt = 8, 2, 96, 50, "int8"
+    lens = [51, 50, 80, 97, 120, -2, -2 ** 31, 2 ** 31 - 1, 7]
+    n_seq, heads = len(lens), n_q + 2 * n_kv
+    qkv = dev(normal16(rng, n_seq * heads * hd)).view(n_seq, -1)
+    dcos, dsin = (torch.from_numpy(x).cuda() for x in _tables(hd, 88))
+    arrays = [x for _ in range(2) for x in R.cache(rng, (n_seq, n_kv), max_seq, hd, fmt)]
+    arrays = [arrays[0], arrays[2], arrays[1], arrays[3]]
+    table = None
+    if block:
+        pools = []
+        for x in arrays:
+            pool, table = R.page(np.random.default_rng(3), x, block, table=table)
+            pools.append(pool)
+        arrays, table = pools, torch.from_numpy(table).cuda()
+    a, b = ([R.to_dev(arrays[0], fmt), R.to_dev(arrays[1], fmt), torch.from_numpy(arrays[2]).cuda(),
+             torch.from_numpy(arrays[3]).cuda()] for _ in range(2))
+    ld = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    pos = torch.tensor([max(n - 1, -2 ** 31) for n in lens], dtype=torch.int32, device="cuda")
+    want, got = (torch.empty(n_seq, n_q * hd, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    rot, stride = qkv.clone(), n_kv * max_seq * hd
+    if block:
+        tab = (table, table.shape[1], block)
+        g.rope_kv_append_q8_paged(rot, n_seq, 1, pos, dcos, dsin, *a, *tab, n_q, n_kv, hd)
+        g.attention_decode_q8_paged(rot, heads * hd, *a, *tab, ld, max_len, n_q, n_kv, hd, want, n_q * hd)
+        assert g.device_error() == 6
+        g.rope_attention_decode_q8_paged(qkv, dcos, dsin, *b, *tab, ld, max_len, n_q, n_kv, hd, got,
+                                         n_q * hd)
+    else:
+        g.rope_kv_append_q8(rot, n_seq, 1, pos, dcos, dsin, *a, stride, n_q, n_kv, hd, max_seq)
+        g.attention_decode_q8(rot, heads * hd, *a, stride, ld, max_len, n_q, n_kv, hd, max_seq, want,
+                              n_q * hd)
+        assert g.device_error() == 6
+        g.rope_attention_decode_q8(qkv, dcos, dsin, *b, stride, ld, max_len, n_q, n_kv, hd, max_seq, got,
+                                   n_q * hd)
+    assert g.device_error() == 6
+    for x, y in zip(a, b):
+        kind = torch.int32 if x.dtype == torch.float32 else torch.int8
+        assert torch.equal(x.view(kind), y.view(kind))
+    assert torch.equal(got, want)
