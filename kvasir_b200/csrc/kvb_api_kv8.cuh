@@ -369,7 +369,8 @@ static int launch_q8_decode(kvb_stream_t stream, const GeneralDecodeArgs& a, con
                         (!c.block_table || c.block_size % 16 == 0) && a.q_row_stride % 4 == 0 &&
                         aligned(a.q, 8) && aligned(c.kc, 16) && aligned(c.vc, 16) &&
                         aligned(c.ks, 4) && aligned(c.vs, 4) && n_seq <= 65535 &&
-                        a.n_kv <= 65535 && fits_i32(cache_rows + 64) && a.max_len <= 1 << 30;
+                        a.n_kv <= 65535 && cache_rows > 0 && fits_i32(cache_rows + 64) &&
+                        a.max_len <= 1 << 30;
     if (rope.cos_t && !(tensor && aligned(rope.cos_t, 16) && aligned(rope.sin_t, 16)))
         return fail(KVB_ERR_UNSUPPORTED,
                     "rope_attention_decode_q8: needs head_dim 64 or 128, n_q/n_kv <= 16, block_size "
@@ -610,7 +611,7 @@ static int launch_shared(kvb_stream_t stream, const GeneralDecodeArgs& a, const 
         aligned(src.kc, 16) && aligned(src.vc, 16) && aligned(src.pk, 16) && aligned(src.pv, 16) &&
         n_seq <= 65535 && a.n_kv <= 65535 && a.max_len <= 1 << 30 && src.prefix <= 1 << 30 &&
         ws != nullptr && aligned(ws, 16) &&
-        (paged ? src.block_size % 64 == 0 &&
+        (paged ? src.block_size % 64 == 0 && src.n_blocks > 0 &&
                      fits_i32((size_t)src.n_blocks * src.n_kv * src.block_size + 64)
                : fits_i32(own_rows + 64))) {
         // Paged: whole 64-key tiles of the prefix for all at once; each sequence reads the rest

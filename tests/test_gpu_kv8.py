@@ -900,3 +900,27 @@ def test_fused_step_with_lengths_out_of_range(g, hd, block):
         kind = torch.int32 if x.dtype == torch.float32 else torch.int8
         assert torch.equal(x.view(kind), y.view(kind))
     assert torch.equal(got, want)
+
+
+def test_decode_over_a_cache_without_rows(g):
+    """max_len 0 on a cache of no rows, contiguous and paged: zero rows."""
+    import ctypes as C
+    one = torch.zeros(64, device="cuda")  # never read
+    lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+    table = torch.zeros(1, dtype=torch.int32, device="cuda")
+    q = torch.ones(2, 512, dtype=torch.bfloat16, device="cuda")
+    p = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+    s = C.c_void_p(g.stream.cuda_stream)
+    for paged in (False, True):
+        out = torch.ones(2, 512, dtype=torch.bfloat16, device="cuda")
+        if paged:
+            st = g._lib.kvb_attention_decode_q8_paged(
+                s, p(q), 512, p(one), p(one), p(one), p(one), 0, 0, p(table), 0, 16, p(lens), 2, 0, 8, 2, 64,
+                0.125, p(out), 512, None, 0, 0, 0)
+        else:
+            st = g._lib.kvb_attention_decode_q8(s, p(q), 512, p(one), p(one), p(one), p(one), 0, 0, 0, p(lens),
+                                                2, 0, 8, 2, 64, 0, 0.125, p(out), 512, None, 0, 0, 0)
+        assert st == 0
+        torch.cuda.synchronize()
+        assert bool((out == 0).all())
+    assert g.device_error() == 0

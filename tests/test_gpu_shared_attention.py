@@ -460,3 +460,24 @@ def test_scores_of_minus_infinity(g, hd):
                 # weights (2^-15 of each) and f32 sums far below 2^-8
                 np.testing.assert_allclose(got, want, rtol=2.0 ** -8, atol=2.0 ** -8, equal_nan=True)
     assert g.device_error() == 0
+
+
+def test_paged_over_a_pool_without_blocks(g):
+    """Sequences of length 0 on an empty pool: zero rows; longer ones are reported (their keys read
+    as zeros)."""
+    import ctypes as C
+    one = torch.zeros(64, device="cuda")  # never read
+    q = torch.ones(2, 512, dtype=torch.bfloat16, device="cuda")
+    table = torch.zeros(2, dtype=torch.int32, device="cuda")
+    n = g.attention_decode_shared_workspace_bytes(2, 64, 0, 8, 2, 64)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    p = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+    for length, err in ((0, 0), (64, 4)):
+        lens = torch.full((2,), length, dtype=torch.int32, device="cuda")
+        out = torch.ones(2, 512, dtype=torch.bfloat16, device="cuda")
+        st = g._lib.kvb_attention_decode_shared_paged(
+            C.c_void_p(g.stream.cuda_stream), p(q), 512, p(one), p(one), 0, p(table), 1, 64, 64, p(lens), 2,
+            64, 8, 2, 64, 0.125, p(out), 512, p(ws), n, 0)
+        assert st == 0
+        assert g.device_error() == err
+        assert bool((out == 0).all())
