@@ -158,39 +158,39 @@ class Decoder:
         sequence b is filled from generators seeded by (seed, g + b, layer, k|v)
         only, so a sequence's context does not depend on how the sequences are
         split over ranks (a paged cache gets the same contents through its
-        block table)."""
+        block table).  After use_paged_cache: the pools given there."""
         g = torch.Generator(device=self.device)
         if self.ks is not None:
             if first_seq is None:
                 g.manual_seed(seed)
             self._fill_q8(g, seed, std, first_seq)
             return
+        kc, vc, table = getattr(self, "_paged", (self.kc, self.vc, None))
         if first_seq is None:
             g.manual_seed(seed)
             for l in range(self.cfg.num_layers):
-                self.kc[l].normal_(0.0, std, generator=g)
-                self.vc[l].normal_(0.0, std, generator=g)
+                kc[l].normal_(0.0, std, generator=g)
+                vc[l].normal_(0.0, std, generator=g)
             return
         nkv, hd = self.cfg.num_kv_heads, self.cfg.head_dim
-        paged = getattr(self, "_paged", None)
         tmp = seq = None
-        if paged is not None:
-            bs = self.kc.shape[3]
-            mb = self.block_table.shape[1]
+        if table is not None:
+            bs = kc.shape[3]
+            mb = table.shape[1]
             tmp = torch.zeros(nkv, mb * bs, hd, dtype=self.dtype, device=self.device)
             seq = torch.empty(nkv, self.max_seq, hd, dtype=self.dtype, device=self.device)
         for b in range(self.n_seq):
             for l in range(self.cfg.num_layers):
-                for kind, cache in ((0, self.kc), (1, self.vc)):
+                for kind, cache in ((0, kc), (1, vc)):
                     s = (((seed * 1000003 + first_seq + b) * 1024 + l) * 2 + kind) & (2 ** 63 - 1)
                     g.manual_seed(s)
-                    if paged is None:
+                    if table is None:
                         cache[l, b].normal_(0.0, std, generator=g)
                     else:  # the contiguous contents, scattered into the pool's blocks
                         seq.normal_(0.0, std, generator=g)
                         tmp[:, :self.max_seq] = seq
                         blocks = tmp.view(nkv, mb, bs, hd).permute(1, 0, 2, 3)
-                        cache[l][self.block_table[b].long()] = blocks
+                        cache[l][table[b].long()] = blocks
 
     def _fill_q8(self, g, seed, std, first_seq) -> None:
         """fill_kv_normal of an 8-bit cache: 16-bit rows N(0, std), quantised into it."""
@@ -220,10 +220,11 @@ class Decoder:
         [n_seq, max_blocks], shared by all layers.  The tensors are kept alive here."""
         if block_table.dtype != torch.int32:
             raise ShapeError("block table must be int32")
-        self._paged = (k_pools, v_pools, block_table)
         check(self._lib.kvb_decoder_use_paged_cache(self._h, k_pools.data_ptr(),
                                                     v_pools.data_ptr(), k_pools[0].numel(),
                                                     block_table.data_ptr(), max_blocks, block_size))
+        self._paged = (k_pools, v_pools, block_table)
+        self.ks = self.vs = None  # an 8-bit cache is no longer used
 
     def set_sampling(self, temperature: float, top_p: float = 1.0, seed: int = 0) -> None:
         """Temperature / top-p sampling for the following steps (kvb_decoder_set_sampling);

@@ -184,3 +184,29 @@ def test_rows_past_two_to_the_31():
                           max_seq, n_q, n_kv, hd, max_seq, out1, n_q * hd)
     assert torch.equal(out[-1:], out1) and bool((out[:-1] == 0).all())
     assert g.device_error() == 0
+
+
+@pytest.mark.parametrize("block", [None, 16])
+@pytest.mark.parametrize("first_seq", [None, 0])
+def test_fill_after_the_switch_to_a_16_bit_pool(block, first_seq):
+    """fill_kv_normal fills the cache that the steps read: after use_paged_cache, the pools given
+    there, as it fills a 16-bit decoder's own."""
+    from kvasir_b200.decoder import Decoder
+    cfg, n_seq, max_seq, bs = _cfg(), 3, 150, 64
+    ref = Decoder(cfg, n_seq, max_seq, seed=9, paged_block_size=bs)
+    ref.fill_kv_normal(seed=4, first_seq=first_seq)
+    dec = Decoder(cfg, n_seq, max_seq, weights=ref.w, seed=9, paged_block_size=block, kv_dtype=torch.int8)
+    dec.fill_kv_normal(seed=2)
+    kp, vp = torch.zeros_like(ref.kc), torch.zeros_like(ref.vc)
+    dec.use_paged_cache(kp, vp, ref.block_table, ref.block_table.shape[1], bs)
+    dec.fill_kv_normal(seed=4, first_seq=first_seq)
+    assert torch.equal(kp, ref.kc) and torch.equal(vp, ref.vc)
+    ids = torch.tensor([1, 2, 3], dtype=torch.int32, device="cuda")
+    for d in (ref, dec):
+        d.set_lengths(100)
+        d.ids_in.copy_(ids)
+        d.step()
+    torch.cuda.synchronize()
+    assert torch.equal(ref.logits, dec.logits)
+    for d in (ref, dec):
+        d.close()
