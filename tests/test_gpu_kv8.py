@@ -924,3 +924,26 @@ def test_decode_over_a_cache_without_rows(g):
         torch.cuda.synchronize()
         assert bool((out == 0).all())
     assert g.device_error() == 0
+
+
+@pytest.mark.parametrize("hd,counts", [(64, [4, 8, 9, 16, 17, 32, 33, 64, 65, 128, 129]),
+                                       (128, [4, 8, 9, 16, 17, 32, 33, 64, 65, 140])])
+@pytest.mark.parametrize("n_q", [1, 5])
+def test_every_form_of_the_join(g, hd, counts, n_q):
+    """Part counts on both sides of each number of warps a row and loads a lane, with sequences of
+    fewer parts, of one part and of none beside them: some warps of a row have no part then."""
+    unit = 256 if hd == 64 else 128  # a chunk of one tile for each warp
+    part = (n_q * (hd + 2) + 3) // 4 * 4 * 4
+    for parts in counts:
+        lens = [unit * parts - 5, unit * (parts // 3) + 1, 7, 0][:3 if parts > 100 else 4]
+        n = g.attention_decode_q8_workspace_bytes(len(lens), max(lens), n_q, 1, hd)
+        if parts <= 3 * 148 // len(lens):  # of 148 SMs
+            assert n == len(lens) * parts * part
+        rng = np.random.default_rng(parts)
+        q, qf, cache, kv_of, max_seq = _decode_case(rng, lens, n_q, 1, hd, "int8", "bf16")
+        out = _run_decode(g, q, cache, lens, n_q, 1, hd, max_seq, "int8", "bf16")
+        assert g.device_error() == 0
+        R.check_attention(out, qf, kv_of, 1, R.default_scale(hd), "bf16", W_EPS, f"{parts} parts",
+                          R.Q_EPS["int8"])
+        if len(lens) == 4:
+            assert bool((out[3] == 0).all())
