@@ -86,14 +86,22 @@ __device__ __forceinline__ int decode_tile_row(const DecodeArgs& a, int b, int k
     }
     return (blk * a.n_kv + kvh) * a.block_size + kt0 % a.block_size;
 }
+// A global load; kL2: past L1, for memory that an earlier kernel of the stream wrote and that is read
+// without a griddepcontrol.wait of the reading grid's own.
+template <bool kL2, typename V>
+__device__ __forceinline__ V ld_from(const V* p) {
+    return kL2 ? __ldcg(p) : *p;
+}
+template <bool kL2 = false>
 __device__ __forceinline__ int decode_block_of(const DecodeArgs& a, int b, int kt0) {
     if (!a.block_table) return 0;
     const int lb = kt0 / a.block_size;
-    return lb < a.max_blocks ? a.block_table[(size_t)b * a.max_blocks + lb] : -1;
+    return lb < a.max_blocks ? ld_from<kL2>(a.block_table + (size_t)b * a.max_blocks + lb) : -1;
 }
 
+template <bool kL2 = false>
 __device__ __forceinline__ int decode_len(const DecodeArgs& a, int b) {
-    int len = a.lens ? a.lens[b] : a.len_const;
+    int len = a.lens ? ld_from<kL2>(a.lens + b) : a.len_const;
     if (len < 0 || len > a.max_len) {
         if (threadIdx.x == 0) raise_dev_error(kDevErrBadLength);
         len = len < 0 ? 0 : a.max_len;
@@ -117,7 +125,7 @@ __device__ __forceinline__ void decode_chunk(const CUtensorMap& kmap, const CUte
     const int g = lane >> 2, c = lane & 3;
     const int G = a.group;
 
-    const int len = decode_len(a, b);
+    const int len = decode_len<kPart>(a, b);
     const int key0 = kPart ? own_key0(len, a.key0) : 0;
     const int table_row = kPart && len < a.key0 ? 0 : b;
     const int n_chunks = (len - key0 + a.chunk_keys - 1) / a.chunk_keys;
@@ -157,11 +165,11 @@ __device__ __forceinline__ void decode_chunk(const CUtensorMap& kmap, const CUte
     uint64_t* bar_v = &bars[kDecWarps + warp];  // and its V tile, completed separately
     const int row_base = (int)((long long)b * a.seq_rows + (long long)kvh * a.max_seq);
     // paged: lane 0 reads the block of its next tile while the current one loads
-    int blk_next = lane == 0 ? decode_block_of(a, table_row, key_begin + warp * kDecTileKeys) : 0;
+    int blk_next = lane == 0 ? decode_block_of<kPart>(a, table_row, key_begin + warp * kDecTileKeys) : 0;
     auto tile_row = [&](int kt0) {  // lane 0: cache row of keys kt0 .. kt0 + 63
         const int row = decode_tile_row(a, b, kvh, row_base, kt0, blk_next);
         const int kn = kt0 + kDecWarps * kDecTileKeys;
-        if (kn < key_end) blk_next = decode_block_of(a, table_row, kn);
+        if (kn < key_end) blk_next = decode_block_of<kPart>(a, table_row, kn);
         return row;
     };
     auto issue_k = [&](int row) {
@@ -225,10 +233,13 @@ __device__ __forceinline__ void decode_chunk(const CUtensorMap& kmap, const CUte
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             const int d0 = 16 * s + 2 * c;
-            qa[s][0] = g < G ? *reinterpret_cast<const uint32_t*>(qb + g * 64 + d0) : 0u;
-            qa[s][1] = g + 8 < G ? *reinterpret_cast<const uint32_t*>(qb + (g + 8) * 64 + d0) : 0u;
-            qa[s][2] = g < G ? *reinterpret_cast<const uint32_t*>(qb + g * 64 + d0 + 8) : 0u;
-            qa[s][3] = g + 8 < G ? *reinterpret_cast<const uint32_t*>(qb + (g + 8) * 64 + d0 + 8) : 0u;
+            auto pair = [&](int h, int d) {
+                return h < G ? ld_from<kPart>(reinterpret_cast<const uint32_t*>(qb + h * 64 + d)) : 0u;
+            };
+            qa[s][0] = pair(g, d0);
+            qa[s][1] = pair(g + 8, d0);
+            qa[s][2] = pair(g, d0 + 8);
+            qa[s][3] = pair(g + 8, d0 + 8);
         }
         if (kRope && rope_p >= 0) {
             // rotate_half in registers: dims j (s = 0, 1) pair with j + 32 (s = 2, 3);
@@ -512,7 +523,8 @@ __global__ void __launch_bounds__(128, 3) attn_decode_kernel(const __grid_consta
 
 // The partial form (DecodeArgs::key0), grid (kv head, sequence, chunk slot): the own keys of
 // kvb_attention_decode_shared.  Launched as a programmatic dependent of the prefix's kernel,
-// from which it reads nothing (everything before that kernel has completed when it starts).
+// from which it reads nothing (everything before that kernel has completed when it starts; K and V
+// come through L2 by tensor copies, lengths, table and q by loads that pass L1).
 // Only the grid's last CTA waits for it, before it ends: the grid then completes after the
 // prefix's kernel, and the join pass after it finds both kernels' parts, while the other CTAs
 // leave their slots at once and run on the SMs that the prefix's grid leaves free.

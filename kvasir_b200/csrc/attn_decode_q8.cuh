@@ -856,7 +856,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(JoinArgs a) 
     __shared__ float4 sums[W > 1 ? kJoinWarps : 1][kCols];
     asm volatile("griddepcontrol.launch_dependents;");
     // What the lengths come from has completed when this grid starts; the partials have not.
-    int len = a.lens[blockIdx.y];
+    int len = ld_from<true>(a.lens + blockIdx.y);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.group, b = blockIdx.y, n_q = a.n_kv * G;

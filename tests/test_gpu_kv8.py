@@ -947,3 +947,44 @@ def test_every_form_of_the_join(g, hd, counts, n_q):
                           R.Q_EPS["int8"])
         if len(lens) == 4:
             assert bool((out[3] == 0).all())
+
+
+def test_inputs_rewritten_between_captured_calls(g):
+    """Several split calls in one graph, q and lengths rewritten on the stream before each: every
+    call and its join read what was written last."""
+    from kvasir_b200 import Gpu
+    rng = np.random.default_rng(103)
+    n_q, n_kv, hd, fmt, lens = 8, 2, 64, "int8", [3000, 900, 2100]
+    q, _, cache, kv_of, max_seq = _decode_case(rng, lens, n_q, n_kv, hd, fmt, "bf16")
+    kc, vc, ks, vs = R.to_dev(cache[0], fmt), R.to_dev(cache[1], fmt), *(torch.from_numpy(x).cuda()
+                                                                        for x in cache[2:])
+    qs = [normal16(rng, 3 * n_q * hd) for _ in range(4)]
+    ns = [[int(rng.integers(0, n + 1)) for n in lens] for _ in qs]
+    ns[1] = [5, 900, 0]  # one chunk, all of the keys, none
+    s = torch.cuda.Stream()
+    gs = Gpu(0, stream=s)
+    dq, dn = [dev(x) for x in qs], [torch.tensor(n, dtype=torch.int32, device="cuda") for n in ns]
+    cq, cn = torch.empty_like(dq[0]), torch.empty_like(dn[0])
+    outs = [torch.empty(3, n_q * hd, dtype=torch.bfloat16, device="cuda") for _ in qs]
+    ws = torch.empty(g.attention_decode_q8_workspace_bytes(3, 3000, n_q, n_kv, hd), dtype=torch.uint8,
+                     device="cuda")
+    assert ws.numel() > 0
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        for i in range(4):
+            cq.copy_(dq[i])
+            cn.copy_(dn[i])
+            gs.attention_decode_q8(cq, n_q * hd, kc, vc, ks, vs, n_kv * max_seq * hd, cn, 3000, n_q, n_kv, hd,
+                                   max_seq, outs[i], n_q * hd, workspace=ws)
+    for _ in range(5):
+        for o in outs:
+            o.fill_(9.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for i in range(4):
+            qf = O.to_f32(qs[i]).astype(np.float64).reshape(3, n_q, hd)
+            R.check_attention(outs[i], qf, lambda b, h: tuple(x[:ns[i][b]] for x in kv_of(b, h)), n_kv,
+                              R.default_scale(hd), "bf16", W_EPS, f"call {i}", R.Q_EPS[fmt])
+    assert g.device_error() == 0

@@ -481,3 +481,59 @@ def test_paged_over_a_pool_without_blocks(g):
         assert st == 0
         assert g.device_error() == err
         assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_inputs_rewritten_between_captured_calls(g, paged):
+    """Several calls in one graph, q, lengths and block table rewritten on the stream before each:
+    every call reads what was written last, although its launches start before their own waits."""
+    from kvasir_b200 import Gpu
+    rng = np.random.default_rng(101)
+    cases = [Case(rng, 640, [int(n) for n in rng.integers(0, 300, 6)], 8, 2, 64, "bf16") for _ in range(4)]
+    c0 = cases[0]
+    for c in cases:  # the same caches for all
+        c.pk, c.pv, c.kc, c.vc, c.f, c.max_seq, c.rows = c0.pk, c0.pv, c0.kc, c0.vc, c0.f, c0.max_seq, c0.rows
+        c.lens = [min(n, m) for n, m in zip(c.lens, c0.lens)]
+        c.ld = torch.tensor(c.lens, dtype=torch.int32, device="cuda")
+    s = torch.cuda.Stream()
+    gs = Gpu(0, stream=s)
+    n = max(c0.lens)
+    (kp, vp), table = c0.pools(64)
+    kp, vp, pk, pv, kc, vc = (dev(x) for x in (kp, vp, c0.pk, c0.pv, c0.kc, c0.vc))
+    # every call's table: the sequences' rows in another order, their lengths and q with them
+    orders = [np.roll(np.arange(6), i) for i in range(4)]
+    tables = [torch.from_numpy(table[o]).cuda() for o in orders]
+    for t in tables:  # row 0 holds the prefix in every order
+        assert torch.equal(t[0, :10], t[1, :10])
+    order = (lambda i: torch.from_numpy(orders[i]).cuda()) if paged else (lambda i: torch.arange(6).cuda())
+    qs = [dev(c.q).view(6, 512)[order(i)].contiguous() for i, c in enumerate(cases)]
+    lens = [(c.ld + (640 if paged else 0))[order(i)].contiguous() for i, c in enumerate(cases)]
+    q, ld, tab = torch.empty_like(qs[0]), torch.empty_like(lens[0]), torch.empty_like(tables[0])
+    outs, ws = [c.out() for c in cases], c0.ws(g, n)
+
+    def calls():
+        for i in range(4):
+            q.copy_(qs[i])
+            ld.copy_(lens[i])
+            tab.copy_(tables[i])
+            if paged:
+                gs.attention_decode_shared_paged(q, 512, kp, vp, tab, tab.shape[1], 64, 640, ld, 640 + n, 8, 2,
+                                                 64, outs[i], 512, workspace=ws)
+            else:
+                gs.attention_decode_shared(q, 512, pk, pv, 640, c0.rows, kc, vc, 2 * c0.max_seq * 64, ld, n, 8,
+                                           2, 64, c0.max_seq, outs[i], 512, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        calls()
+    for _ in range(5):
+        for o in outs:
+            o.fill_(9.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for i, c in enumerate(cases):
+            got = torch.empty_like(outs[i])
+            got[order(i)] = outs[i]
+            c.check(got, f"call {i}")
+    assert g.device_error() == 0
