@@ -419,8 +419,12 @@ int kvb_kv_read_q8_paged(kvb_stream_t stream, const void* k_pool, const void* v_
                          int kv_format, int dtype);
 
 /* Batched single-query decode attention over an 8-bit cache: kvb_attention_decode's
- * arguments and result (f32 scores, sums and accumulation) on the values that the
- * rows stand for.  A sequence without keys gives a zero row, one whose scores are all
+ * arguments, on the values that the rows stand for.  Scores, maxima, sums and accumulation are
+ * f32.  In fewer bits, in the tensor-core kernel: on int8 codes each element of q, to 16-bit
+ * integers (within 1.6e-5 of its head's largest magnitude; on e4m3 codes q keeps all its bits
+ * down to 2^-31 of that), and each key's weight times V scale, once to f16 (2^-11 of it; f32
+ * where the V scales of 64 keys lie further apart than 2^8 to 2^16).  kvb_attention_decode
+ * multiplies q in its own type and weights as 16-bit head and remainder.  A sequence without keys gives a zero row, one whose scores are all
  * -infinity (f32 overflow) NaN.  Any head_dim up to 256, any group size; a block entry outside the
  * pool sets kvb_device_error code 4 and those keys read as zeros.  The tensor-core kernel
  * takes head_dim 64 and 128 with n_q / n_kv <= 16, block_size a multiple of 16, codes 16-byte

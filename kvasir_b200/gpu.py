@@ -464,7 +464,8 @@ class Gpu:
     def attention_decode_q8(self, q, q_row_stride, kc, vc, ks, vs, seq_stride, lens, max_len, n_q,
                             n_kv, head_dim, max_seq, out, out_row_stride, scale=None,
                             workspace=None):
-        """kvb_attention_decode_q8: attention_decode over an 8-bit cache."""
+        """kvb_attention_decode_q8: attention_decode over an 8-bit cache.  workspace
+        (attention_decode_q8_workspace_bytes): without one long sequences are not split."""
         name = "attention_decode_q8"
         p = self._ptrs(name, q, kc, vc, ks, vs, lens, out, workspace)
         fmt, n, n_scales = self._check_q8(name, kc, vc, ks, vs)
@@ -546,7 +547,9 @@ class Gpu:
                                 seq_stride, lens, max_len, n_q, n_kv, head_dim, max_seq, out,
                                 out_row_stride, scale=None, workspace=None):
         """kvb_attention_decode_shared: every sequence attends to the keys [0, prefix_len) of
-        pk / pv [n_kv, prefix_rows, head_dim], read once for all, then to its own lens[b]."""
+        pk / pv [n_kv, prefix_rows, head_dim], read once for all, then to its own lens[b].
+        Give it a workspace (attention_decode_shared_workspace_bytes): without one a general
+        kernel runs, hundreds of times slower on a large batch."""
         name = "attention_decode_shared"
         p = self._ptrs(name, q, pk, pv, kc, vc, lens, out, workspace)
         n_seq = self._check_attention(name, q, q_row_stride, lens, out, out_row_stride,
@@ -565,7 +568,8 @@ class Gpu:
                                       max_blocks, block_size, shared_len, lens, max_len, n_q, n_kv,
                                       head_dim, out, out_row_stride, scale=None, workspace=None):
         """kvb_attention_decode_shared_paged: attention_decode_paged where the first shared_len
-        keys of every sequence are the same (read through row 0 of the block table)."""
+        keys of every sequence are the same (read through row 0 of the block table).  Give it a
+        workspace, as attention_decode_shared."""
         name = "attention_decode_shared_paged"
         p = self._ptrs(name, q, k_pool, v_pool, block_table, lens, out, workspace)
         n_seq = self._check_attention(name, q, q_row_stride, lens, out, out_row_stride,
