@@ -988,3 +988,27 @@ def test_inputs_rewritten_between_captured_calls(g):
             R.check_attention(outs[i], qf, lambda b, h: tuple(x[:ns[i][b]] for x in kv_of(b, h)), n_kv,
                               R.default_scale(hd), "bf16", W_EPS, f"call {i}", R.Q_EPS[fmt])
     assert g.device_error() == 0
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_a_large_v_row_beside_nan(g, fmt, hd):
+    """V rows far apart with a NaN in one head's q, or in one KV head's V: the other heads keep the
+    f64 bound, those are NaN."""
+    rng = np.random.default_rng(104)
+    n_q, n_kv, lens = 8, 2, [900, 70]
+    rs = [None, np.where(rng.random((2, n_kv, 903)) < 0.02, 2.0 ** 40, 1.0)]
+    q, qf, cache, kv_of, max_seq = _decode_case(rng, lens, n_q, n_kv, hd, fmt, "bf16", rs)
+    x = qf.copy()
+    x[0, 2, 5] = np.nan
+    cache[3][1, 1, 33] = np.nan
+    out = _run_decode(g, O.from_f32(x.astype(np.float32).ravel()), cache, lens, n_q, n_kv, hd, max_seq, fmt,
+                      "bf16").view(2, n_q, hd)
+    assert bool(out[0, 2].isnan().all()) and bool(out[1, 4:].isnan().all())
+    keep = {0: [0, 1, 3, 4, 5, 6, 7], 1: [0, 1, 2, 3]}
+    for b, heads in keep.items():
+        for h in heads:
+            R.check_attention(out[b:b + 1, h].contiguous(), qf[b:b + 1, h:h + 1],
+                              lambda _, __: kv_of(b, h // 4), 1, R.default_scale(hd), "bf16", W_EPS,
+                              f"sequence {b} head {h}", R.Q_EPS[fmt])
+    assert g.device_error() == 0
