@@ -66,7 +66,7 @@ struct SharedPrefixArgs {
     int prefix;           // keys of the prefix
     int n_tiles, splits;  // 64-key tiles of the prefix, slices they are dealt to
     float scale_log2;
-    const int32_t* lens;  // paged: lengths that may end inside the prefix; else nullptr
+    const int32_t* lens;  // kShort: lengths that may end inside the prefix
     int max_len;
     float* ws;  // partials [n_seq][n_kv][max_parts][part_floats]; slice i is part i
     int max_parts, part_floats;
@@ -138,7 +138,8 @@ __device__ __forceinline__ void umma_pv_64(uint32_t d, uint32_t p, uint64_t v, u
     }
 }
 
-template <typename T, int kGroups>
+// kShort: a.lens may end a row inside the prefix (paged).
+template <typename T, int kGroups, bool kShort>
 __global__ void __launch_bounds__(sp_threads(kGroups), kSpMaxGroups / kGroups)
     attn_shared_prefix_kernel(const __grid_constant__ CUtensorMap qmap,
                               const __grid_constant__ CUtensorMap kmap,
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(sp_threads(kGroups), kSpMaxGroups / kGroups)
         const int seq = (tile0 + grp) * a.seqs_per_tile + row / a.group, head = row % a.group;
         const bool valid = row < rows && seq < a.n_seq;
         int limit = a.prefix;  // this row's keys
-        if (a.lens && valid) limit = own_key0(max(0, min(a.lens[seq], a.max_len)), limit);
+        if (kShort && valid) limit = own_key0(max(0, min(a.lens[seq], a.max_len)), limit);
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         auto part_of_row = [&] {
@@ -342,7 +343,7 @@ __global__ void __launch_bounds__(sp_threads(kGroups), kSpMaxGroups / kGroups)
             float s[32];
             // The first tile past a shorter row's keys (whole tiles; where the slice begins past
             // them the part has no weight)
-            if (masked && j > 0 && __any_sync(0xffffffffu, n_here == 0)) {
+            if (kShort && masked && j > 0 && __any_sync(0xffffffffu, n_here == 0)) {
                 float* to = a.ws + part_of_row() + head * 64;
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
@@ -438,7 +439,8 @@ __global__ void __launch_bounds__(sp_threads(kGroups), kSpMaxGroups / kGroups)
             a.ws[off + a.group * 64 + head] = ok ? m - kShift : -INFINITY;  // what O and l are relative to
             a.ws[off + a.group * 65 + head] = ok ? l : 0.f;
         }
-        const bool whole = valid && limit > key0 + (nt - 1) * kSpKeys;  // else O is stored, or void
+        // else O is stored, or void
+        const bool whole = valid && (!kShort || limit > key0 + (nt - 1) * kSpKeys);
         const long long dst = whole ? (long long)(off + head * 64) : -1;
         float4* stage = reinterpret_cast<float4*>(sq + grp * kSpQBytes + quarter * 4096);
 #pragma unroll

@@ -472,7 +472,8 @@ static SharedPlan shared_plan(size_t n_seq, size_t prefix, size_t max_own, size_
 template <typename T, int kGroups>
 static int launch_shared_prefix(kvb_stream_t stream, const CUtensorMap& qmap, const CUtensorMap& kmap,
                                 const CUtensorMap& vmap, const SharedPrefixArgs& s) {
-    auto* kernel = attn_shared_prefix_kernel<T, kGroups>;
+    auto* kernel = s.lens ? attn_shared_prefix_kernel<T, kGroups, true>
+                          : attn_shared_prefix_kernel<T, kGroups, false>;
     set_max_smem(kernel, sp_smem_bytes(kGroups));
     const dim3 grid((unsigned)s.n_kv, (unsigned)s.splits,
                     (unsigned)((s.row_tiles + kGroups - 1) / kGroups));
