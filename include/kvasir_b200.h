@@ -423,10 +423,11 @@ int kvb_kv_read_q8_paged(kvb_stream_t stream, const void* k_pool, const void* v_
  * f32.  In fewer bits, in the tensor-core kernel: on int8 codes each element of q, to 16-bit
  * integers (within 1.6e-5 of its head's largest magnitude; on e4m3 codes q keeps all its bits
  * down to 2^-31 of that), and each key's weight times V scale, once to f16 (2^-11 of it; f32
- * where the V scales of 64 keys lie further apart than 2^8 to 2^16).  kvb_attention_decode
- * multiplies q in its own type and weights as 16-bit head and remainder.  A sequence without keys gives a zero row, one whose scores are all
- * -infinity (f32 overflow) NaN.  Any head_dim up to 256, any group size; a block entry outside the
- * pool sets kvb_device_error code 4 and those keys read as zeros.  The tensor-core kernel
+ * where the V scales of a tile of 64 or 32 keys lie further apart than 2^8 to 2^16).
+ * kvb_attention_decode multiplies q in its own type and weights as 16-bit head and remainder.  A
+ * sequence without keys gives a zero row, one whose scores are all -infinity (f32 overflow) NaN.
+ * Any head_dim up to 256, any group size; a block entry outside the pool sets kvb_device_error
+ * code 4 and those keys read as zeros.  The tensor-core kernel
  * takes head_dim 64 and 128 with n_q / n_kv <= 16, block_size a multiple of 16, codes 16-byte
  * and q 8-byte aligned with q_row_stride a multiple of 4; a general kernel, several times
  * slower, takes the rest.  The workspace (kvb_attention_decode_q8_workspace_bytes; a smaller
@@ -456,8 +457,9 @@ size_t kvb_attention_decode_q8_workspace_bytes(size_t n_seq, size_t max_len, siz
  * caches: qkv [n_seq, (n_q + 2 n_kv) * head_dim] stays unrotated, the codes and scales of
  * the new rows are written.  A sequence of length 0 has no new row and gives a zero row; a length
  * past max_len is reported as by both calls, and a new row of which the block lies outside the pool
- * is reported and not written (its q is rotated all the same).  head_dim 64 or 128, n_q / n_kv <= 16, block_size a multiple
- * of 16, 16-byte aligned buffers; otherwise KVB_ERR_UNSUPPORTED.  Workspace as for
+ * is reported and not written (its q is rotated all the same).  head_dim 64 or 128,
+ * n_q / n_kv <= 16, block_size a multiple of 16, 16-byte aligned buffers; otherwise
+ * KVB_ERR_UNSUPPORTED.  Workspace as for
  * kvb_attention_decode_q8. */
 int kvb_rope_attention_decode_q8(kvb_stream_t stream, const void* qkv, size_t qkv_len,
                                  const float* cos_t, const float* sin_t, size_t table_len, void* kc,

@@ -31,7 +31,8 @@
 // Measured no better: a part of the exponentials as polynomials on the FMA pipe, halves of 32 keys
 // with an S buffer each (110 us; N = 32 products cost the tensor pipe as much as N = 64).
 // Measured on B200 with the own keys and the join: 256 sequences of 32 + 8 heads on 16384 keys
-// with up to 1000 own, 97 us (f16) and 106 us (bf16, P in two halves).
+// with up to 1000 own, in a graph, 101 us (f16) and 107 to 114 us (bf16, P in two halves).  One row
+// tile a CTA is held to 80 registers for four CTAs per SM and spills (bf16: 64 bytes a thread).
 #pragma once
 
 #include "attn_decode_q8.cuh"

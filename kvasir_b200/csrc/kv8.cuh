@@ -241,7 +241,8 @@ __device__ __forceinline__ uint32_t widen_bits(uint32_t h) {
 // shuffles.  Both 16-byte loads of a thread are issued before its position is known, the
 // rotation goes four pairs at a time and the maximum over packed elements: 40 registers,
 // so that 1,536 threads (48 KB of loads) are in flight on an SM -- at 62 registers 960 were,
-// and 4 x 2048 tokens of 32 + 16 heads (103 MB) took 25 us instead of 21.2.  Measured no
+// and 4 x 2048 tokens of 32 + 16 heads (103 MB) took 25 us instead of 21.2 (with 24 bytes a thread
+// spilled).  Measured no
 // better: 48 registers with several short rows per CTA (21.2), a persistent grid that requests
 // the next row ahead (28.3).  What bounds it is issue (61 % of slots, 75 % of an SM's busy
 // time).  Packed f32x2 multiplies and adds would halve the arithmetic, but the assembler
